@@ -10,11 +10,14 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # HELEN_HIP_LIB: developer override to A/B-test kernel variants built side by side.
 LIB_PATH = os.environ.get("HELEN_HIP_LIB") or os.path.join(_HERE, "csrc", "libhelen_hip.so")
 
-HELEN_ABI_VERSION = 4
+HELEN_ABI_VERSION = 5
 HELEN_OK = 0
 HELEN_PRECISION_FP32 = 0
 HELEN_PRECISION_BF16 = 1
 HELEN_PRECISION_FP32X3 = 2
+HELEN_TYPE_FP32 = 0
+HELEN_TYPE_BF16 = 1
+HELEN_TYPE_FP16 = 2
 
 KERNEL_CLASSES = ("pack", "gemm_enc", "gru_enc", "gemm_dec", "gru_dec", "heads")
 
@@ -26,6 +29,8 @@ EXPORTS = (
     "helen_reset_kernel_stats",
     "helen_get_kernel_stats", "helen_reload_overrides", "helen_describe_dispatch", "helen_plan_call",
     "helen_device_count", "helen_host_alloc", "helen_host_free", "helen_polish_slot_submit", "helen_polish_slot_wait",
+    "helen_delta_rule_bytes", "helen_delta_rule_forward", "helen_delta_rule_backward", "helen_delta_rule_step",
+    "helen_layer_norm_forward", "helen_layer_norm_bytes", "helen_layer_norm_backward",
 )
 RECURRENCE_KERNELS = ("gru_kernel", "gru_single8_kernel", "gru_half8_kernel", "gru_quarter4_kernel", "gru_pair_kernel")
 DECODER_PROJECTIONS = ("gemm_gi_kernel<16>", "gemm_dec_ws_kernel", "gemm_dec_wsp_kernel")
@@ -44,6 +49,48 @@ class HelenWeightsC(ctypes.Structure):
         ("dec_w_ih", _f32p * 2), ("dec_w_hh", _f32p * 2),
         ("dec_b_ih", _f32p * 2), ("dec_b_hh", _f32p * 2),
         ("base_w", _f32p), ("base_b", _f32p), ("rle_w", _f32p), ("rle_b", _f32p),
+    ]
+
+
+_i32, _i64, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
+
+
+class HelenDeltaRuleC(ctypes.Structure):
+    """`HelenDeltaRule` of include/helen_hip.h."""
+    _fields_ = [
+        ("struct_size", ctypes.c_size_t), ("device", _i32), ("dtype", _i32),
+        ("heads_k", _i32), ("heads_v", _i32), ("width_k", _i32), ("width_v", _i32),
+        ("tokens", _i32), ("sequences", _i32), ("zero_tail", _i32), ("scale", ctypes.c_float),
+        ("offsets", _vp), ("q", _vp), ("k", _vp), ("v", _vp), ("g", _vp), ("beta", _vp),
+        ("q_stride", _i64 * 2), ("k_stride", _i64 * 2), ("v_stride", _i64 * 2), ("g_stride", _i64 * 2),
+        ("beta_stride", _i64 * 2),
+        ("initial_state", _vp), ("o", _vp), ("o_stride", _i64 * 2), ("final_state", _vp),
+        ("d_o", _vp), ("d_o_stride", _i64 * 2), ("d_final_state", _vp),
+        ("grad_q", _vp), ("grad_k", _vp), ("grad_v", _vp), ("grad_g", _vp), ("grad_beta", _vp),
+        ("grad_initial_state", _vp),
+    ]
+
+
+class HelenDeltaStepC(ctypes.Structure):
+    """`HelenDeltaStep` of include/helen_hip.h."""
+    _fields_ = [
+        ("struct_size", ctypes.c_size_t), ("device", _i32), ("dtype", _i32),
+        ("heads_k", _i32), ("heads_v", _i32), ("width_k", _i32), ("width_v", _i32),
+        ("rows", _i32), ("pool", _i32), ("scale", ctypes.c_float),
+        ("slots", _vp), ("q", _vp), ("k", _vp), ("v", _vp), ("g", _vp), ("beta", _vp),
+        ("q_stride", _i64 * 2), ("k_stride", _i64 * 2), ("v_stride", _i64 * 2), ("g_stride", _i64 * 2),
+        ("beta_stride", _i64 * 2),
+        ("state", _vp), ("state_stride", _i64), ("o", _vp), ("o_stride", _i64 * 2),
+    ]
+
+
+class HelenLayerNormC(ctypes.Structure):
+    """`HelenLayerNorm` of include/helen_hip.h."""
+    _fields_ = [
+        ("struct_size", ctypes.c_size_t), ("device", _i32), ("dtype", _i32), ("weight_dtype", _i32), ("width", _i32),
+        ("rows", _i64), ("eps", ctypes.c_float), ("x", _vp), ("x_stride", _i64), ("weight", _vp), ("bias", _vp),
+        ("y", _vp), ("y_stride", _i64), ("mean", _vp), ("rstd", _vp), ("dy", _vp), ("dy_stride", _i64),
+        ("dx", _vp), ("dx_stride", _i64), ("dweight", _vp), ("dbias", _vp),
     ]
 
 
@@ -137,6 +184,21 @@ def load(with_torch=True):
     lib.helen_polish_slot_submit.argtypes = [vp, vp, ci, vp, vp, vp]
     lib.helen_polish_slot_wait.restype = ci
     lib.helen_polish_slot_wait.argtypes = [vp]
+    sz = ctypes.POINTER(ctypes.c_size_t)
+    lib.helen_delta_rule_bytes.restype = ci
+    lib.helen_delta_rule_bytes.argtypes = [ctypes.POINTER(HelenDeltaRuleC), sz, sz, sz]
+    lib.helen_delta_rule_forward.restype = ci
+    lib.helen_delta_rule_forward.argtypes = [ctypes.POINTER(HelenDeltaRuleC), ci, vp, ctypes.c_size_t, vp]
+    lib.helen_delta_rule_backward.restype = ci
+    lib.helen_delta_rule_backward.argtypes = [ctypes.POINTER(HelenDeltaRuleC), vp, ctypes.c_size_t, vp, ctypes.c_size_t, vp]
+    lib.helen_delta_rule_step.restype = ci
+    lib.helen_delta_rule_step.argtypes = [ctypes.POINTER(HelenDeltaStepC), vp]
+    lib.helen_layer_norm_forward.restype = ci
+    lib.helen_layer_norm_forward.argtypes = [ctypes.POINTER(HelenLayerNormC), vp]
+    lib.helen_layer_norm_bytes.restype = ci
+    lib.helen_layer_norm_bytes.argtypes = [ctypes.POINTER(HelenLayerNormC), sz]
+    lib.helen_layer_norm_backward.restype = ci
+    lib.helen_layer_norm_backward.argtypes = [ctypes.POINTER(HelenLayerNormC), vp, ctypes.c_size_t, vp]
     got = lib.helen_abi_version()
     if got != HELEN_ABI_VERSION:
         raise ImportError("libhelen_hip.so ABI %d != binding ABI %d; rebuild" % (got, HELEN_ABI_VERSION))

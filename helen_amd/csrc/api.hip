@@ -19,22 +19,25 @@
 #include "../../include/helen_hip.h"
 #include "kernels.h"
 #include "dispatch.h"
+#include "error.h"
 
 using namespace helen;
 
 static_assert(kDecStagePositions == HELEN_DWS_PB, "dispatch.h's stage sizes are the kernels'");
 
 namespace {
-
 thread_local char g_err[512] = "";
+}
 
-int fail(int code, const char* fmt, ...) {
+int helen::fail(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof(g_err), fmt, ap);
     va_end(ap);
     return code;
 }
+
+namespace {
 
 #define HIP_TRY(expr)                                                                       \
     do {                                                                                    \

@@ -1,0 +1,319 @@
+// kernels_norm.h -- layer norm over the last dimension and its gradients
+//
+//     y = (x - mean) rstd w + b,   rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+//     dx = rstd (e - mean(e) - h mean(e h)),  e = dy w,  h = (x - mean) rstd;   dw = sum over rows of dy h,  db = sum of dy
+// A row is read once into registers and both moments are taken from there (the second one around the mean: no cancellation).
+// L lanes share a row: 16 for narrow rows (four rows a wave), 64, or a whole workgroup for wide ones.  Rows of any alignment
+// are read in 16-byte pieces (gfx950 takes unaligned wide loads), only a row's last piece element by element.
+// The weight's gradient is a sum over all rows: a workgroup keeps its columns' sums in registers over all the rows it takes,
+// writes them once, and a second small kernel adds the workgroups' sums in their order -- no atomics, the same bits each time.
+#pragma once
+#include "kernels_delta.h"
+
+namespace helen {
+
+struct NormArgs {
+    const void *x, *w, *b, *dy;
+    void *y, *dx, *dw, *db;
+    float *mean, *rstd, *partial;
+    long rows, x_t, y_t, dy_t, dx_t;
+    int width, groups;
+    float eps;
+};
+
+template <typename In>
+struct Pieces {
+    typedef typename In::raw raw;
+    static constexpr int V = 16 / (int)sizeof(raw);
+    typedef raw vec __attribute__((ext_vector_type(16 / sizeof(raw)), aligned(sizeof(raw))));
+    static __device__ __forceinline__ void load(const raw* p, int left, float (&to)[V]) {
+        if (left >= V) {
+            const vec t = *(const vec*)p;
+#pragma unroll
+            for (int i = 0; i < V; ++i) to[i] = In::to_f32(t[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) to[i] = i < left ? In::to_f32(p[i]) : 0.f;
+        }
+    }
+    static __device__ __forceinline__ void store(raw* p, int left, const float (&from)[V]) {
+        if (left >= V) {
+            vec t;
+#pragma unroll
+            for (int i = 0; i < V; ++i) t[i] = In::from_f32(from[i]);
+            *(vec*)p = t;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i < left) p[i] = In::from_f32(from[i]);
+        }
+    }
+};
+// V elements of a weight (its own type) from column `at`
+template <typename W, int V>
+__device__ __forceinline__ void load_weight(const void* w, int at, int left, float (&to)[V], float otherwise) {
+    const typename W::raw* p = (const typename W::raw*)w + at;
+    if (w && left >= V) {
+        constexpr int PV = Pieces<W>::V < V ? Pieces<W>::V : V;
+        typedef typename W::raw vec __attribute__((ext_vector_type(PV), aligned(sizeof(typename W::raw))));
+#pragma unroll
+        for (int c = 0; c < V / PV; ++c) {
+            const vec t = *(const vec*)(p + c * PV);
+#pragma unroll
+            for (int i = 0; i < PV; ++i) to[c * PV + i] = W::to_f32(t[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) to[i] = w && i < left ? W::to_f32(p[i]) : otherwise;
+    }
+}
+
+// sum over the L lanes of a row; L = 256: over the workgroup (`red` has four floats and is free again after the call)
+template <int L, int N>
+__device__ __forceinline__ void row_sum(float (&x)[N], float (*red)[N]) {
+#pragma unroll
+    for (int m = 1; m < (L < 64 ? L : 64); m <<= 1)
+#pragma unroll
+        for (int n = 0; n < N; ++n) x[n] += __shfl_xor(x[n], m);
+    if constexpr (L == 256) {
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int n = 0; n < N; ++n) red[w][n] = x[n];
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < N; ++n) x[n] = (red[0][n] + red[1][n]) + (red[2][n] + red[3][n]);
+        __syncthreads();
+    }
+}
+
+template <typename In, typename W, int L, int NV>
+__global__ __launch_bounds__(256) void norm_forward_kernel(const NormArgs a) {
+    typedef typename In::raw raw;
+    constexpr int V = Pieces<In>::V;
+    __shared__ float red[4][1];
+    const int t = threadIdx.x % L;
+    const long row = blockIdx.x * (long)(256 / L) + threadIdx.x / L;
+    if (row >= a.rows) return;          // (L = 256: the whole workgroup)
+    const raw* x = (const raw*)a.x + row * a.x_t;
+    float v[NV][V], s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int at = (t + i * L) * V;
+        Pieces<In>::load(x + at, a.width - at, v[i]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[0] += v[i][e];
+    }
+    row_sum<L, 1>(s, red);
+    const float mean = s[0] / a.width;
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            v[i][e] -= mean;
+            s[0] += (t + i * L) * V + e < a.width ? v[i][e] * v[i][e] : 0.f;
+        }
+    row_sum<L, 1>(s, red);
+    const float rstd = 1.f / sqrtf(s[0] / a.width + a.eps);
+    if (t == 0) {
+        if (a.mean) a.mean[row] = mean;
+        if (a.rstd) a.rstd[row] = rstd;
+    }
+    raw* y = (raw*)a.y + row * a.y_t;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int at = (t + i * L) * V, left = a.width - at;
+        if (left <= 0) continue;
+        float w[V], b[V];
+        load_weight<W, V>(a.w, at, left, w, 1.f);
+        load_weight<W, V>(a.b, at, left, b, 0.f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[i][e] = v[i][e] * rstd * w[e] + b[e];
+        Pieces<In>::store(y + at, left, v[i]);
+    }
+}
+
+template <typename In, typename W, int L, int NV>
+__global__ __launch_bounds__(256) void norm_backward_kernel(const NormArgs a) {
+    typedef typename In::raw raw;
+    constexpr int V = Pieces<In>::V, R = 256 / L;
+    __shared__ float red[4][2];
+    __shared__ float cols[R > 1 ? 256 * V : 1];
+    const int t = threadIdx.x % L;
+    float w[NV][V], dw[NV][V], db[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int at = (t + i * L) * V;
+        load_weight<W, V>(a.w, at, a.width - at, w[i], 1.f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) dw[i][e] = db[i][e] = 0.f;
+    }
+    for (long row = blockIdx.x * (long)R + threadIdx.x / L; row < a.rows; row += (long)a.groups * R) {
+        const raw* x = (const raw*)a.x + row * a.x_t;
+        const raw* dy = (const raw*)a.dy + row * a.dy_t;
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float h[NV][V], g[NV][V], s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int at = (t + i * L) * V;
+            Pieces<In>::load(x + at, a.width - at, h[i]);
+            Pieces<In>::load(dy + at, a.width - at, g[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                h[i][e] = (h[i][e] - mean) * rstd;
+                dw[i][e] += g[i][e] * h[i][e];
+                db[i][e] += g[i][e];
+                g[i][e] *= w[i][e];
+                s[0] += g[i][e];
+                s[1] += g[i][e] * h[i][e];
+            }
+        row_sum<L, 2>(s, red);
+        const float c0 = s[0] / a.width, c1 = s[1] / a.width;
+        raw* dx = (raw*)a.dx + row * a.dx_t;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int at = (t + i * L) * V, left = a.width - at;
+            if (left <= 0) continue;
+#pragma unroll
+            for (int e = 0; e < V; ++e) h[i][e] = rstd * (g[i][e] - c0 - h[i][e] * c1);
+            Pieces<In>::store(dx + at, left, h[i]);
+        }
+    }
+    // the workgroup's sums of its columns: [group][dw | db][width]
+    float* const out = a.partial + (long)blockIdx.x * 2 * a.width;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float x[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] = k ? db[i][e] : dw[i][e];
+            if constexpr (R > 1) {
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < V; ++e) cols[e * 256 + threadIdx.x] = x[e];
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    x[e] = 0.f;
+                    for (int r = 0; r < R; ++r) x[e] += cols[e * 256 + r * L + t];
+                }
+            }
+            if ((int)threadIdx.x < L) {
+                const int at = (t + i * L) * V;
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (at + e < a.width) out[(long)k * a.width + at + e] = x[e];
+            }
+        }
+}
+
+// rows wider than the registers hold: the row is read again for each of its sums (it stays in the caches)
+template <typename In, typename W>
+__global__ __launch_bounds__(256) void norm_forward_wide_kernel(const NormArgs a) {
+    typedef typename In::raw raw;
+    constexpr int V = Pieces<In>::V;
+    __shared__ float red[4][1];
+    const long row = blockIdx.x;
+    const raw* x = (const raw*)a.x + row * a.x_t;
+    float v[V], s[1] = {0.f};
+    for (int at = threadIdx.x * V; at < a.width; at += 256 * V) {
+        Pieces<In>::load(x + at, a.width - at, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[0] += v[e];
+    }
+    row_sum<256, 1>(s, red);
+    const float mean = s[0] / a.width;
+    s[0] = 0.f;
+    for (int at = threadIdx.x * V; at < a.width; at += 256 * V) {
+        Pieces<In>::load(x + at, a.width - at, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[0] += at + e < a.width ? (v[e] - mean) * (v[e] - mean) : 0.f;
+    }
+    row_sum<256, 1>(s, red);
+    const float rstd = 1.f / sqrtf(s[0] / a.width + a.eps);
+    if (threadIdx.x == 0) {
+        if (a.mean) a.mean[row] = mean;
+        if (a.rstd) a.rstd[row] = rstd;
+    }
+    raw* y = (raw*)a.y + row * a.y_t;
+    for (int at = threadIdx.x * V; at < a.width; at += 256 * V) {
+        const int left = a.width - at;
+        float w[V], b[V];
+        Pieces<In>::load(x + at, left, v);
+        load_weight<W, V>(a.w, at, left, w, 1.f);
+        load_weight<W, V>(a.b, at, left, b, 0.f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = (v[e] - mean) * rstd * w[e] + b[e];
+        Pieces<In>::store(y + at, left, v);
+    }
+}
+template <typename In, typename W>
+__global__ __launch_bounds__(256) void norm_backward_wide_kernel(const NormArgs a) {
+    typedef typename In::raw raw;
+    constexpr int V = Pieces<In>::V;
+    __shared__ float red[4][2];
+    float* const out = a.partial + (long)blockIdx.x * 2 * a.width;
+    for (int at = threadIdx.x; at < 2 * a.width; at += 256) out[at] = 0.f;
+    __syncthreads();                    // (a thread adds to other elements than it cleared)
+    for (long row = blockIdx.x; row < a.rows; row += a.groups) {
+        const raw* x = (const raw*)a.x + row * a.x_t;
+        const raw* dy = (const raw*)a.dy + row * a.dy_t;
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float h[V], g[V], w[V], s[2] = {0.f, 0.f};
+        for (int at = threadIdx.x * V; at < a.width; at += 256 * V) {
+            const int left = a.width - at;
+            Pieces<In>::load(x + at, left, h);
+            Pieces<In>::load(dy + at, left, g);
+            load_weight<W, V>(a.w, at, left, w, 1.f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                h[e] = (h[e] - mean) * rstd;
+                s[0] += g[e] * w[e];
+                s[1] += g[e] * w[e] * h[e];
+                if (e < left) {
+                    out[at + e] += g[e] * h[e];
+                    out[(long)a.width + at + e] += g[e];
+                }
+            }
+        }
+        row_sum<256, 2>(s, red);
+        const float c0 = s[0] / a.width, c1 = s[1] / a.width;
+        raw* dx = (raw*)a.dx + row * a.dx_t;
+        for (int at = threadIdx.x * V; at < a.width; at += 256 * V) {
+            const int left = a.width - at;
+            Pieces<In>::load(x + at, left, h);
+            Pieces<In>::load(dy + at, left, g);
+            load_weight<W, V>(a.w, at, left, w, 1.f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) h[e] = rstd * (g[e] * w[e] - c0 - (h[e] - mean) * rstd * c1);
+            Pieces<In>::store(dx + at, left, h);
+        }
+    }
+}
+
+// the workgroups' sums, added in their order: 32 columns and 8 runs of groups a workgroup
+template <typename W>
+__global__ __launch_bounds__(256) void norm_reduce_kernel(const NormArgs a) {
+    __shared__ float part[8][33];
+    const int c = threadIdx.x & 31, run = threadIdx.x >> 5;
+    const long at = blockIdx.x * 32l + c;
+    float x = 0.f;
+    if (at < 2l * a.width)
+        for (int g = run; g < a.groups; g += 8) x += a.partial[(long)g * 2 * a.width + at];
+    part[run][c] = x;
+    __syncthreads();
+    if (run == 0 && at < 2l * a.width) {
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) sum += part[r][c];
+        void* to = at < a.width ? a.dw : a.db;
+        if (to) ((typename W::raw*)to)[at < a.width ? at : at - a.width] = W::from_f32(sum);
+    }
+}
+
+}  // namespace helen

@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define HELEN_ABI_VERSION 4
+#define HELEN_ABI_VERSION 5
 
 enum {
     HELEN_OK = 0,
@@ -259,6 +259,127 @@ int helen_set_profiling(HelenModel* model, unsigned class_mask);
 int helen_reset_kernel_stats(HelenModel* model);
 int helen_get_kernel_stats(HelenModel* model, int kernel_class, double* out_total_ms,
                            long long* out_launches);
+
+/*
+ * Sequence operators: a recurrent layer with a matrix state (the gated delta rule) beside the GRU of
+ * helen_gru_chunk_forward, and the layer norm that stands before and behind such layers.  No reference counterpart.
+ *
+ * They hold no handle: every buffer, the workspace included, is the caller's, on `device`, and calls on different streams
+ * with different workspaces may run at once (a captured graph keeps its own workspace).  Work is enqueued on `stream`; no
+ * call allocates, waits or copies to the host.  Pointers are DEVICE pointers, strides count elements, the last dimension is
+ * contiguous.  Element types HELEN_TYPE_*; log decays g, steps beta, states and their gradients are always float32.
+ */
+enum { HELEN_TYPE_FP32 = 0, HELEN_TYPE_BF16 = 1, HELEN_TYPE_FP16 = 2 };
+
+/*
+ * The gated delta rule over whole sequences: per value head a state S [width_k, width_v], and per token
+ *     u = beta (v - e^g S^T k),   S <- e^g S + k u^T,   o = scale S^T q.
+ * heads_v value heads share heads_k query / key heads (heads_v a multiple of heads_k, neighbours share).
+ *   width_k        64 or 128;  width_v 64, 128, 192 or 256
+ *   offsets        int32 [sequences + 1], ascending from 0 within [0, tokens]: sequence i is rows offsets[i] ..
+ *                  offsets[i + 1] (empty ones are allowed; rows behind the last one belong to none); NULL: tokens is a
+ *                  multiple of sequences and all have the same length.  Offsets that break this give wrong values, never an
+ *                  access out of range.
+ *   q, k           [tokens, heads_k, width_k];  v, o, d_o  [tokens, heads_v, width_v];  g, beta  [tokens, heads_v];
+ *                  stride[0] between tokens, stride[1] between heads.  q, k, v, d_o: 16-byte aligned, strides too.
+ *   initial_state  float32 [sequences, heads_v, width_k, width_v] or NULL (zero);  final_state the same or NULL
+ *   o              NULL: only the states are wanted.  Rows behind the last sequence are left as they are, or set to zero
+ *                  where zero_tail is 1.
+ * Backward: d_o and d_final_state (or NULL) in, the gradients out: grad_q, grad_k [tokens, heads_k, width_k] (summed over
+ * the value heads that share a head), grad_v, grad_g, grad_beta contiguous, zero in rows behind the last sequence;
+ * grad_initial_state or NULL.
+ *
+ *   helen_delta_rule_bytes      workspace of a forward call (keep = 0), of one that keeps what the backward pass reads
+ *                               (keep = 1), and of the backward call itself
+ *   helen_delta_rule_forward    keep = 1: `workspace` holds, afterwards, what helen_delta_rule_backward takes as `kept`
+ *   helen_delta_rule_backward   the same description, inputs included, as the forward call that filled `kept`
+ */
+typedef struct HelenDeltaRule {
+    size_t struct_size;          /* sizeof(HelenDeltaRule) */
+    int32_t device;
+    int32_t dtype;
+    int32_t heads_k, heads_v, width_k, width_v;
+    int32_t tokens, sequences;
+    int32_t zero_tail;
+    float scale;
+    const int32_t* offsets;
+    const void *q, *k, *v;
+    const float *g, *beta;
+    int64_t q_stride[2], k_stride[2], v_stride[2], g_stride[2], beta_stride[2];
+    const float* initial_state;
+    void* o;
+    int64_t o_stride[2];
+    float* final_state;
+    const void* d_o;
+    int64_t d_o_stride[2];
+    const float* d_final_state;
+    void *grad_q, *grad_k, *grad_v;
+    float *grad_g, *grad_beta, *grad_initial_state;
+} HelenDeltaRule;
+
+int helen_delta_rule_bytes(const HelenDeltaRule* op, size_t* forward_bytes, size_t* kept_bytes, size_t* backward_bytes);
+int helen_delta_rule_forward(const HelenDeltaRule* op, int keep, void* workspace, size_t workspace_bytes, void* stream);
+int helen_delta_rule_backward(const HelenDeltaRule* op, const void* kept, size_t kept_bytes, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/*
+ * The same rule for single tokens over a pool of states, in place.
+ *   state    float32 [pool, heads_v, width_k, width_v]; state_stride (a multiple of 4) between entries of the pool
+ *   slots    int32 [rows]: the entry of each row, or NULL (row i is entry i, rows <= pool).  -1: a padded row, its output is
+ *            zero.  Rows that name the same entry are successive tokens of one stream, taken in the order of the rows.  Any
+ *            other number outside the pool: that row's output is NaN and no state changes.
+ *   q, k [rows, heads_k, width_k], v, o [rows, heads_v, width_v], g, beta [rows, heads_v]; v is aligned to four elements
+ */
+typedef struct HelenDeltaStep {
+    size_t struct_size;          /* sizeof(HelenDeltaStep) */
+    int32_t device;
+    int32_t dtype;
+    int32_t heads_k, heads_v, width_k, width_v;
+    int32_t rows, pool;
+    float scale;
+    const int32_t* slots;
+    const void *q, *k, *v;
+    const float *g, *beta;
+    int64_t q_stride[2], k_stride[2], v_stride[2], g_stride[2], beta_stride[2];
+    float* state;
+    int64_t state_stride;
+    void* o;
+    int64_t o_stride[2];
+} HelenDeltaStep;
+
+int helen_delta_rule_step(const HelenDeltaStep* op, void* stream);
+
+/*
+ * Layer norm over the last dimension: y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps), statistics float32.
+ *   x, y, dy, dx   [rows, width], rows `*_stride` elements apart, any alignment of their type
+ *   weight, bias   [width] of weight_dtype (dtype's own or float32), either may be NULL (one, zero)
+ *   mean, rstd     float32 [rows]: written by the forward call (or NULL), read by the backward call
+ * Backward: dx, and dweight / dbias of weight_dtype, either NULL if not wanted: sums over all rows in a fixed order
+ * (workspace of helen_layer_norm_bytes).
+ */
+typedef struct HelenLayerNorm {
+    size_t struct_size;          /* sizeof(HelenLayerNorm) */
+    int32_t device;
+    int32_t dtype, weight_dtype;
+    int32_t width;
+    int64_t rows;
+    float eps;
+    const void* x;
+    int64_t x_stride;
+    const void *weight, *bias;
+    void* y;
+    int64_t y_stride;
+    float *mean, *rstd;
+    const void* dy;
+    int64_t dy_stride;
+    void* dx;
+    int64_t dx_stride;
+    void *dweight, *dbias;
+} HelenLayerNorm;
+
+int helen_layer_norm_forward(const HelenLayerNorm* op, void* stream);
+int helen_layer_norm_bytes(const HelenLayerNorm* op, size_t* backward_bytes);
+int helen_layer_norm_backward(const HelenLayerNorm* op, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
