@@ -7,8 +7,7 @@
 //     A_ij = beta_i (k_i . k_j) e^{D_ij} (j < i),  T = (I + A)^-1,   R = V - e^{b} K S0,   U = T beta R,
 //     O = scale (e^{b} Q S0 + P U),  P_ij = (q_i . k_j) e^{D_ij} (j <= i),   S1 = e^{b_C} S0 + K^T (e^{c} U)
 // A, T and P do not depend on the state: delta_prep_kernel makes them for every chunk at once.  What is left, one chunk after
-// another, is delta_forward_kernel: a wave owns 16 columns of S in registers (a column of S needs no other column), so a
-// chain has no exchange between waves at all.
+// another, is delta_forward_kernel: a column of S needs no other column, so a chain is split over its columns.
 //
 // Arithmetic: as in the fp32x3 recurrence, an fp32 value is the sum of three bf16 terms and a product of two such values the
 // six leading products of terms on v_mfma_f32_16x16x32_bf16 with fp32 accumulation.  bf16 inputs are ONE term (their products
@@ -449,138 +448,284 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a) {
     }
 }
 
+// four values in N terms: the half of a fragment that one row tile is
+template <int N>
+__device__ __forceinline__ void split4(const f32x4 v, u32x2 (&t)[N]) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        f32x2 x = {v[2 * p], v[2 * p + 1]};
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const unsigned b = __builtin_bit_cast(unsigned, __builtin_convertvector(x, bf16x2_t));
+            t[n][p] = b;
+            if (n + 1 < N) {
+                x.x -= __builtin_bit_cast(float, b << 16);
+                x.y -= __builtin_bit_cast(float, b & 0xffff0000u);
+            }
+        }
+    }
+}
+// row tile mt of a [64 or DK x 16 NC] operand that the workgroup shares: fragments [k step][term][column tile][lane]
+template <int N, int NC>
+__device__ __forceinline__ void share_tile(bf16x8* buf, int mt, int nc, int lane, const f32x4 v) {
+    u32x2 t[N];
+    split4<N>(v, t);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+        ((u32x2*)(buf + (((mt >> 1) * N + n) * NC + nc) * 64 + lane))[mt & 1] = t[n];
+}
+template <int N, int NC>
+__device__ __forceinline__ void shared_frag(const bf16x8* buf, int ks, int nc, int lane, bf16x8 (&b)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) b[n] = buf[((ks * N + n) * NC + nc) * 64 + lane];
+}
+// LDS writes of every wave are visible behind this; loads from memory stay in flight over it
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+// workgroups go round the eight XCDs: neighbours in `logical` order (the column groups of one head, which read the same
+// fragments) stay on one of them.  The grid is padded to a multiple of eight.
+__device__ __forceinline__ unsigned xcd_order(unsigned block, unsigned grid) { return (block & 7) * (grid >> 3) + (block >> 3); }
+
 // ------------------------------------------------------------------------------------------------
-// The chain: one wave per (sequence, value head, 16 columns of the state).
+// The chain: a workgroup per (sequence, value head, 16 NC columns of the state).  Each of its four waves owns a quarter of
+// the ROWS of everything: token tile w of R, U and O, the dk tiles of S from w DK/64 on.  The other waves' rows of a right-hand
+// operand (S, X = beta R, U) come through LDS as bf16 terms, three barriers a chunk; every left-hand fragment is read by
+// one wave only, straight into registers, and the next chunk's are loaded into the registers the present chunk is done with.
 // ------------------------------------------------------------------------------------------------
-template <typename In, int DK, int PT, bool KEEP>
+template <typename In, int DK, int PT, bool KEEP, int NC>
 __global__ __launch_bounds__(256) void delta_forward_kernel(const DeltaArgs a) {
-    constexpr int NI = In::kTerms, KS = DK / 32, MT = DK / 16;
+    constexpr int NI = In::kTerms, KS = DK / 32, MW = DK / 64;
     typedef typename In::raw raw;
+    __shared__ bf16x8 sbuf[KS * 3 * NC * 64], xbuf[2 * 3 * NC * 64], ubuf[2 * PT * NC * 64], cbuf[2 * 3 * NC * 64];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int j = lane & 15, q = lane >> 4;
-    const int groups = (a.dv_width + 63) >> 6;
-    const int tile = 4 * (blockIdx.x % groups) + w, col = tile * 16 + j;
-    if (tile * 16 >= a.dv_width) return;
-    const int hv = blockIdx.x / groups % a.hv, s = blockIdx.x / groups / a.hv, h = hv / a.group;
+    const int groups = a.dv_width / (16 * NC);
+    const unsigned item = xcd_order(blockIdx.x, gridDim.x);
+    if (item >= (unsigned)a.nseq * a.hv * groups) return;
+    const int hv = item / groups % a.hv, s = item / groups / a.hv, h = hv / a.group;
+    const int col = 16 * NC * (item % groups) + j;
     const Span sp = span_of(a, s);
-    const size_t st = ((size_t)s * a.hv + hv) * DK * a.dv_width;
-    f32x4 S[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) S[m][r] = a.s0 ? a.s0[st + (size_t)(16 * m + 4 * q + r) * a.dv_width + col] : 0.f;
+    const int chunks = (sp.len + kDeltaChunk - 1) / kDeltaChunk;
+    const size_t st = (((size_t)s * a.hv + hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col;
 
-    for (int c = 0; c * kDeltaChunk < sp.len; ++c) {
-        const int start = sp.begin + c * kDeltaChunk, n = min(kDeltaChunk, sp.len - c * kDeltaChunk);
-        const size_t slot = (size_t)sp.slot + c, kslot = slot * a.hk + h, vslot = slot * a.hv + hv;
-        const float* sc = a.sc + vslot * 256;
+    f32x4 S[MW][NC];
+#pragma unroll
+    for (int i = 0; i < MW; ++i)
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) S[i][nc][r] = a.s0 ? a.s0[st + (size_t)(16 * i + r) * a.dv_width + 16 * nc] : 0.f;
+
+    bf16x8 kf[KS][NI], qf[KS][NI], kt[MW][2][NI], tf[2][3], pf[2][PT];
+    f32x4 beta, eb, ec;
+    float whole;
+    raw v[NC][4];
+    const bf16x8* const kf0 = a.kf + (size_t)sp.slot * a.hk * (DK / 8 * NI * 64) + (size_t)h * (DK / 8 * NI * 64) + lane;
+    const bf16x8* const qf0 = a.qf + (kf0 - a.kf);
+    const bf16x8* const kt0 = a.ktf + (kf0 - a.kf);
+    const size_t vslot0 = (size_t)sp.slot * a.hv + hv;
+    const int row = 16 * w + 4 * q;                 // this lane's tokens: row .. row + 3
+    auto load_rows = [&](int c) {
+        const size_t at = (size_t)c * a.hk * (DK / 8 * NI * 64) + w * KS * NI * 64;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int t = 0; t < NI; ++t) {
+                kf[ks][t] = kf0[at + (ks * NI + t) * 64];
+                qf[ks][t] = qf0[at + (ks * NI + t) * 64];
+            }
+    };
+    auto load_tokens = [&](int c) {
+        const float* sc = a.sc + (vslot0 + (size_t)c * a.hv) * 256;
+        beta = *(const f32x4*)(sc + row);
+        eb = *(const f32x4*)(sc + 64 + row);
+        ec = *(const f32x4*)(sc + 128 + row);
+        whole = sc[64 + 63];
+        const int n = sp.len - c * kDeltaChunk;
+        const raw* p = (const raw*)a.v + (sp.begin + c * kDeltaChunk + row) * a.v_t + hv * a.v_h + col;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc) v[nc][r] = row + r < n ? p[r * a.v_t + 16 * nc] : raw(0);
+    };
+    auto load_t = [&](int c) {
+        const size_t at = ((vslot0 + (size_t)c * a.hv) * kTriFrags + tri_index(w, 0)) * 3 * 64 + lane;
+#pragma unroll
+        for (int t = 0; t < 3; ++t) {
+            tf[0][t] = a.tf[at + t * 64];
+            if (w >= 2) tf[1][t] = a.tf[at + (3 + t) * 64];
+        }
+    };
+    auto load_p = [&](int c) {
+        const size_t at = ((vslot0 + (size_t)c * a.hv) * kTriFrags + tri_index(w, 0)) * PT * 64 + lane;
+#pragma unroll
+        for (int t = 0; t < PT; ++t) {
+            pf[0][t] = a.pf[at + t * 64];
+            if (w >= 2) pf[1][t] = a.pf[at + (PT + t) * 64];
+        }
+    };
+    auto load_kt = [&](int c) {
+        const size_t at = (size_t)c * a.hk * (DK / 8 * NI * 64) + w * MW * 2 * NI * 64;
+#pragma unroll
+        for (int i = 0; i < MW; ++i)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int t = 0; t < NI; ++t) kt[i][ks][t] = kt0[at + ((2 * i + ks) * NI + t) * 64];
+    };
+    auto share_state = [&](int c) {
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+            if constexpr (MW == 2) {
+                bf16x8 t[3];
+                split8<3>(S[0][nc], S[1][nc], t);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) sbuf[((w * 3 + k) * NC + nc) * 64 + lane] = t[k];
+            } else {
+                share_tile<3, NC>(sbuf, w, nc, lane, S[0][nc]);
+            }
+        }
         if constexpr (KEEP) {
-            float* to = a.states + vslot * DK * a.dv_width + col;
+            float* to = a.states + ((vslot0 + (size_t)c * a.hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col;
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int i = 0; i < MW; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) to[(size_t)(16 * m + 4 * q + r) * a.dv_width] = S[m][r];
+                for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) to[(size_t)(16 * i + r) * a.dv_width + 16 * nc] = S[i][nc][r];
         }
-        bf16x8 sb[KS][3];
+    };
+    if (chunks > 0) {
+        load_rows(0);
+        load_tokens(0);
+        load_t(0);
+        load_p(0);
+        load_kt(0);
+        share_state(0);
+    }
+    lds_barrier();
+    for (int c = 0; c < chunks; ++c) {
+        const bool more = c + 1 < chunks;
+        f32x4 R[NC], O[NC], U[NC];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) split8<3>(S[2 * ks], S[2 * ks + 1], sb[ks]);
-        f32x4 R[4], O[4];
+        for (int nc = 0; nc < NC; ++nc) R[nc] = O[nc] = U[nc] = splat4(0.f);
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-            R[mt] = O[mt] = splat4(0.f);
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                bf16x8 kf[NI], qf[NI];
-#pragma unroll
-                for (int t = 0; t < NI; ++t) {
-                    const size_t at = (((kslot * 4 + mt) * KS + ks) * NI + t) * 64 + lane;
-                    kf[t] = a.kf[at];
-                    qf[t] = a.qf[at];
-                }
-                R[mt] = mm(kf, sb[ks], R[mt]);
-                O[mt] = mm(qf, sb[ks], O[mt]);
+            for (int nc = 0; nc < NC; ++nc) {
+                bf16x8 b[3];
+                shared_frag<3, NC>(sbuf, ks, nc, lane, b);
+                R[nc] = mm(kf[ks], b, R[nc]);
+                O[nc] = mm(qf[ks], b, O[nc]);
             }
-        }
-        f32x4 X[4];
+        const f32x4 after = ec;
+        const float hold = whole;
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-            const f32x4 beta = *(const f32x4*)(sc + 16 * mt + 4 * q), eb = *(const f32x4*)(sc + 64 + 16 * mt + 4 * q);
+        for (int nc = 0; nc < NC; ++nc) {
+            f32x4 x;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int t = 16 * mt + 4 * q + r;
-                const float v = t < n ? In::to_f32(((const raw*)a.v)[(start + t) * a.v_t + hv * a.v_h + col]) : 0.f;
-                R[mt][r] = v - eb[r] * R[mt][r];
-                O[mt][r] *= eb[r];
-                X[mt][r] = beta[r] * R[mt][r];
-                if constexpr (KEEP) a.r[(vslot * kDeltaChunk + t) * a.dv_width + col] = R[mt][r];
+                R[nc][r] = In::to_f32(v[nc][r]) - eb[r] * R[nc][r];
+                O[nc][r] *= eb[r];
+                x[r] = beta[r] * R[nc][r];
             }
-        }
-        bf16x8 xb[2][3];
-        split8<3>(X[0], X[1], xb[0]);
-        split8<3>(X[2], X[3], xb[1]);
-        f32x4 U[4];
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-            U[mt] = splat4(0.f);
-#pragma unroll
-            for (int ks = 0; ks <= mt / 2; ++ks) {
-                bf16x8 tf[3];
-#pragma unroll
-                for (int t = 0; t < 3; ++t) tf[t] = a.tf[((vslot * kTriFrags + tri_index(mt, ks)) * 3 + t) * 64 + lane];
-                U[mt] = mm(tf, xb[ks], U[mt]);
-            }
+            share_tile<3, NC>(xbuf, w, nc, lane, x);
             if constexpr (KEEP) {
+                float* to = a.r + ((vslot0 + (size_t)c * a.hv) * kDeltaChunk + row) * a.dv_width + col + 16 * nc;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) a.u[(vslot * kDeltaChunk + 16 * mt + 4 * q + r) * a.dv_width + col] = U[mt][r];
+                for (int r = 0; r < 4; ++r) to[r * a.dv_width] = R[nc][r];
             }
         }
-        bf16x8 ub[2][PT];
-        split8<PT>(U[0], U[1], ub[0]);
-        split8<PT>(U[2], U[3], ub[1]);
+        if (more) {
+            load_rows(c + 1);
+            load_tokens(c + 1);
+        }
+        lds_barrier();
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-#pragma unroll
-            for (int ks = 0; ks <= mt / 2; ++ks) {
-                bf16x8 pf[PT];
-#pragma unroll
-                for (int t = 0; t < PT; ++t) pf[t] = a.pf[((vslot * kTriFrags + tri_index(mt, ks)) * PT + t) * 64 + lane];
-                O[mt] = mm<PT, PT, PT - 1>(pf, ub[ks], O[mt]);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = 16 * mt + 4 * q + r;
-                if (a.o && t < n) ((raw*)a.o)[(start + t) * a.o_t + hv * a.o_h + col] = In::from_f32(a.scale * O[mt][r]);
+        for (int nc = 0; nc < NC; ++nc) {
+            bf16x8 b[3];
+            shared_frag<3, NC>(xbuf, 0, nc, lane, b);
+            U[nc] = mm(tf[0], b, U[nc]);
+            if (w >= 2) {
+                shared_frag<3, NC>(xbuf, 1, nc, lane, b);
+                U[nc] = mm(tf[1], b, U[nc]);
             }
         }
+        if (more) load_t(c + 1);
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-            const f32x4 ec = *(const f32x4*)(sc + 128 + 16 * mt + 4 * q);
+        for (int nc = 0; nc < NC; ++nc) {
+            if constexpr (KEEP) {
+                float* to = a.u + ((vslot0 + (size_t)c * a.hv) * kDeltaChunk + row) * a.dv_width + col + 16 * nc;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) U[mt][r] *= ec[r];
+                for (int r = 0; r < 4; ++r) to[r * a.dv_width] = U[nc][r];
+            }
+            share_tile<PT, NC>(ubuf, w, nc, lane, U[nc]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) U[nc][r] *= after[r];
+            share_tile<3, NC>(cbuf, w, nc, lane, U[nc]);
         }
-        const float whole = sc[64 + 63];
-        bf16x8 uc[2][3];
-        split8<3>(U[0], U[1], uc[0]);
-        split8<3>(U[2], U[3], uc[1]);
+        lds_barrier();
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
+        for (int i = 0; i < MW; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) S[m][r] *= whole;
+            for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                bf16x8 kt[NI];
+                for (int r = 0; r < 4; ++r) S[i][nc][r] *= hold;
 #pragma unroll
-                for (int t = 0; t < NI; ++t) kt[t] = a.ktf[((kslot * MT * 2 + 2 * m + ks) * NI + t) * 64 + lane];
-                S[m] = mm(kt, uc[ks], S[m]);
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc) {
+                bf16x8 b[3];
+                shared_frag<3, NC>(cbuf, ks, nc, lane, b);
+#pragma unroll
+                for (int i = 0; i < MW; ++i) S[i][nc] = mm(kt[i][ks], b, S[i][nc]);
+            }
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+            bf16x8 b[PT];
+            shared_frag<PT, NC>(ubuf, 0, nc, lane, b);
+            O[nc] = mm<PT, PT, PT - 1>(pf[0], b, O[nc]);
+            if (w >= 2) {
+                shared_frag<PT, NC>(ubuf, 1, nc, lane, b);
+                O[nc] = mm<PT, PT, PT - 1>(pf[1], b, O[nc]);
             }
         }
+        if (more) {
+            share_state(c + 1);
+            load_kt(c + 1);
+            load_p(c + 1);
+        }
+        if (a.o) {
+            const int n = sp.len - c * kDeltaChunk;
+            raw* to = (raw*)a.o + (sp.begin + c * kDeltaChunk + row) * a.o_t + hv * a.o_h + col;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int nc = 0; nc < NC; ++nc)
+                    if (row + r < n) to[r * a.o_t + 16 * nc] = In::from_f32(a.scale * O[nc][r]);
+        }
+        lds_barrier();
     }
     if (a.s1) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int i = 0; i < MW; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) a.s1[st + (size_t)(16 * m + 4 * q + r) * a.dv_width + col] = S[m][r];
+            for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) a.s1[st + (size_t)(16 * i + r) * a.dv_width + 16 * nc] = S[i][nc][r];
     }
+}
+
+// column tiles of 16 a chain's workgroup takes
+inline int chain_tiles(const DeltaArgs& a) {
+    const long one = (long)a.nseq * a.hv * (a.dv_width / 16);
+    return one >= 1024 ? 2 : 1;
+}
+inline unsigned chain_grid(const DeltaArgs& a, int tiles) {
+    return (unsigned)(((long)a.nseq * a.hv * (a.dv_width / (16 * tiles)) + 7) / 8 * 8);
 }
 
 }  // namespace helen

@@ -8,133 +8,221 @@
 //     dbeta_i = Z_i . R_i + sum_j dA_ij (k_i . k_j) e^{D_ij}
 //     dg_m = sum_{j < m <= i} (dA A + dP P)_ij + sum_{i >= m} (q_i . dQ1_i + k_i . dK1_i) + sum_{i < m} k_i . dK2_i
 //            + e^{b_C} <S0, dS1>,   dQ1, dK1 = the S0 terms of dQ, dK;  dK2 = the dS1 term of dK
-// The reverse chain is the forward one with other operands (a wave owns 16 columns of dS); everything else of all chunks
-// follows at once.  dg is summed over the positions it reaches, not as a difference of running sums.
+// The reverse chain is the forward one with other operands; everything else of all chunks follows at once.  dg is summed over the positions it reaches, not as a difference of running sums.
 #pragma once
 #include "kernels_delta.h"
 
 namespace helen {
 
-template <typename In, int DK>
+// The reverse chain, built like delta_forward_kernel: wave w owns token tile w of dO, dU and Z and its quarter of dS's rows.
+template <typename In, int DK, int NC>
 __global__ __launch_bounds__(256) void delta_backward_kernel(const DeltaArgs a) {
-    constexpr int NI = In::kTerms, KS = DK / 32, MT = DK / 16;
+    constexpr int NI = In::kTerms, KS = DK / 32, MW = DK / 64;
     typedef typename In::raw raw;
+    __shared__ bf16x8 sbuf[KS * 3 * NC * 64], ybuf[2 * NI * NC * 64], wbuf[2 * 3 * NC * 64], dbuf[2 * 3 * NC * 64], zbuf[2 * 3 * NC * 64];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int j = lane & 15, q = lane >> 4;
-    const int groups = (a.dv_width + 63) >> 6;
-    const int tile = 4 * (blockIdx.x % groups) + w, col = tile * 16 + j;
-    if (tile * 16 >= a.dv_width) return;
-    const int hv = blockIdx.x / groups % a.hv, s = blockIdx.x / groups / a.hv, h = hv / a.group;
+    const int groups = a.dv_width / (16 * NC);
+    const unsigned item = xcd_order(blockIdx.x, gridDim.x);
+    if (item >= (unsigned)a.nseq * a.hv * groups) return;
+    const int hv = item / groups % a.hv, s = item / groups / a.hv, h = hv / a.group;
+    const int col = 16 * NC * (item % groups) + j;
     const Span sp = span_of(a, s);
-    const size_t st = ((size_t)s * a.hv + hv) * DK * a.dv_width;
-    f32x4 S[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) S[m][r] = a.ds1 ? a.ds1[st + (size_t)(16 * m + 4 * q + r) * a.dv_width + col] : 0.f;
+    const int chunks = (sp.len + kDeltaChunk - 1) / kDeltaChunk;
+    const size_t st = (((size_t)s * a.hv + hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col;
 
-    for (int c = (sp.len + kDeltaChunk - 1) / kDeltaChunk - 1; c >= 0; --c) {
-        const int start = sp.begin + c * kDeltaChunk, n = min(kDeltaChunk, sp.len - c * kDeltaChunk);
-        const size_t slot = (size_t)sp.slot + c, kslot = slot * a.hk + h, vslot = slot * a.hv + hv;
-        const float* sc = a.sc + vslot * 256;
-        {
-            float* to = a.dstates + vslot * DK * a.dv_width + col;
+    f32x4 S[MW][NC];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+    for (int i = 0; i < MW; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) to[(size_t)(16 * m + 4 * q + r) * a.dv_width] = S[m][r];
+        for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) S[i][nc][r] = a.ds1 ? a.ds1[st + (size_t)(16 * i + r) * a.dv_width + 16 * nc] : 0.f;
+
+    bf16x8 kf[KS][NI], kt[MW][2][NI], qt[MW][2][NI], tt[2][3], pt[2][3];
+    f32x4 beta, eb, ec;
+    float whole;
+    raw y[NC][4];
+    const bf16x8* const kf0 = a.kf + (size_t)sp.slot * a.hk * (DK / 8 * NI * 64) + (size_t)h * (DK / 8 * NI * 64) + lane;
+    const bf16x8* const kt0 = a.ktf + (kf0 - a.kf);
+    const bf16x8* const qt0 = a.qtf + (kf0 - a.kf);
+    const size_t vslot0 = (size_t)sp.slot * a.hv + hv;
+    const int row = 16 * w + 4 * q;
+    auto load_rows = [&](int c) {
+        const size_t at = (size_t)c * a.hk * (DK / 8 * NI * 64) + w * KS * NI * 64;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int t = 0; t < NI; ++t) kf[ks][t] = kf0[at + (ks * NI + t) * 64];
+    };
+    auto load_scales = [&](int c) {
+        const float* sc = a.sc + (vslot0 + (size_t)c * a.hv) * 256;
+        beta = *(const f32x4*)(sc + row);
+        eb = *(const f32x4*)(sc + 64 + row);
+        ec = *(const f32x4*)(sc + 128 + row);
+        whole = sc[64 + 63];
+    };
+    auto load_dout = [&](int c) {
+        const int n = sp.len - c * kDeltaChunk;
+        const raw* p = (const raw*)a.dout + (sp.begin + c * kDeltaChunk + row) * a.do_t + hv * a.do_h + col;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc) y[nc][r] = row + r < n ? p[r * a.do_t + 16 * nc] : raw(0);
+    };
+    auto load_tri = [&](int c, const bf16x8* from, bf16x8 (&to)[2][3]) {
+        const size_t at = (vslot0 + (size_t)c * a.hv) * kTriFrags * 3 * 64 + lane;
+#pragma unroll
+        for (int t = 0; t < 3; ++t) {
+            if (w < 2) to[0][t] = from[at + (trt_index(w, 0) * 3 + t) * 64];
+            to[1][t] = from[at + (trt_index(w, 1) * 3 + t) * 64];
         }
-        bf16x8 sb[KS][3];
+    };
+    auto load_columns = [&](int c) {
+        const size_t at = (size_t)c * a.hk * (DK / 8 * NI * 64) + w * MW * 2 * NI * 64;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) split8<3>(S[2 * ks], S[2 * ks + 1], sb[ks]);
-        f32x4 Y[4];      // dO
+        for (int i = 0; i < MW; ++i)
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = 16 * mt + 4 * q + r;
-                Y[mt][r] = t < n ? In::to_f32(((const raw*)a.dout)[(start + t) * a.do_t + hv * a.do_h + col]) : 0.f;
-            }
-        bf16x8 yb[2][NI];
-        split8<NI>(Y[0], Y[1], yb[0]);
-        split8<NI>(Y[2], Y[3], yb[1]);
-        f32x4 U[4];
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-            U[mt] = splat4(0.f);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                bf16x8 kf[NI];
-#pragma unroll
-                for (int t = 0; t < NI; ++t) kf[t] = a.kf[(((kslot * 4 + mt) * KS + ks) * NI + t) * 64 + lane];
-                U[mt] = mm(kf, sb[ks], U[mt]);
-            }
-            f32x4 p = splat4(0.f);
-#pragma unroll
-            for (int ks = mt / 2; ks < 2; ++ks) {
-                bf16x8 pt[3];
-#pragma unroll
-                for (int t = 0; t < 3; ++t) pt[t] = a.ptf[((vslot * kTriFrags + trt_index(mt, ks)) * 3 + t) * 64 + lane];
-                p = mm(pt, yb[ks], p);
-            }
-            const f32x4 ec = *(const f32x4*)(sc + 128 + 16 * mt + 4 * q);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) U[mt][r] = ec[r] * U[mt][r] + a.scale * p[r];
-        }
-        bf16x8 ub[2][3];
-        split8<3>(U[0], U[1], ub[0]);
-        split8<3>(U[2], U[3], ub[1]);
-        f32x4 Z[4];
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-            Z[mt] = splat4(0.f);
-#pragma unroll
-            for (int ks = mt / 2; ks < 2; ++ks) {
-                bf16x8 tt[3];
-#pragma unroll
-                for (int t = 0; t < 3; ++t) tt[t] = a.ttf[((vslot * kTriFrags + trt_index(mt, ks)) * 3 + t) * 64 + lane];
-                Z[mt] = mm(tt, ub[ks], Z[mt]);
-            }
-            const f32x4 beta = *(const f32x4*)(sc + 16 * mt + 4 * q), eb = *(const f32x4*)(sc + 64 + 16 * mt + 4 * q);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = 16 * mt + 4 * q + r;
-                a.z[(vslot * kDeltaChunk + t) * a.dv_width + col] = Z[mt][r];
-                const float dv = beta[r] * Z[mt][r];
-                if (t < n) ((raw*)a.dv)[((size_t)(start + t) * a.hv + hv) * a.dv_width + col] = In::from_f32(dv);
-                Z[mt][r] = -eb[r] * dv;
-                Y[mt][r] *= a.scale * eb[r];
-            }
-        }
-        bf16x8 zb[2][3], wb[2][3];
-        split8<3>(Z[0], Z[1], zb[0]);
-        split8<3>(Z[2], Z[3], zb[1]);
-        split8<3>(Y[0], Y[1], wb[0]);
-        split8<3>(Y[2], Y[3], wb[1]);
-        const float whole = sc[64 + 63];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) S[m][r] *= whole;
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                bf16x8 kt[NI], qt[NI];
+            for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int t = 0; t < NI; ++t) {
-                    const size_t at = ((kslot * MT * 2 + 2 * m + ks) * NI + t) * 64 + lane;
-                    kt[t] = a.ktf[at];
-                    qt[t] = a.qtf[at];
+                    kt[i][ks][t] = kt0[at + ((2 * i + ks) * NI + t) * 64];
+                    qt[i][ks][t] = qt0[at + ((2 * i + ks) * NI + t) * 64];
                 }
-                S[m] = mm(kt, zb[ks], S[m]);
-                S[m] = mm(qt, wb[ks], S[m]);
+    };
+    // dS (behind chunk c) and dO (of chunk c) for all waves
+    auto share = [&](int c) {
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+            if constexpr (MW == 2) {
+                bf16x8 t[3];
+                split8<3>(S[0][nc], S[1][nc], t);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) sbuf[((w * 3 + k) * NC + nc) * 64 + lane] = t[k];
+            } else {
+                share_tile<3, NC>(sbuf, w, nc, lane, S[0][nc]);
             }
+            share_tile<NI, NC>(ybuf, w, nc, lane,
+                               (f32x4){In::to_f32(y[nc][0]), In::to_f32(y[nc][1]), In::to_f32(y[nc][2]), In::to_f32(y[nc][3])});
         }
+        float* to = a.dstates + ((vslot0 + (size_t)c * a.hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col;
+#pragma unroll
+        for (int i = 0; i < MW; ++i)
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to[(size_t)(16 * i + r) * a.dv_width + 16 * nc] = S[i][nc][r];
+    };
+    if (chunks > 0) {
+        const int c = chunks - 1;
+        load_dout(c);
+        load_rows(c);
+        load_scales(c);
+        load_tri(c, a.ptf, pt);
+        load_tri(c, a.ttf, tt);
+        load_columns(c);
+        share(c);
+    }
+    lds_barrier();
+    for (int c = chunks - 1; c >= 0; --c) {
+        f32x4 E[NC], P[NC];
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) E[nc] = P[nc] = splat4(0.f);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc) {
+                bf16x8 b[3];
+                shared_frag<3, NC>(sbuf, ks, nc, lane, b);
+                E[nc] = mm(kf[ks], b, E[nc]);
+            }
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+            bf16x8 b[NI];
+            if (w < 2) {
+                shared_frag<NI, NC>(ybuf, 0, nc, lane, b);
+                P[nc] = mm(pt[0], b, P[nc]);
+            }
+            shared_frag<NI, NC>(ybuf, 1, nc, lane, b);
+            P[nc] = mm(pt[1], b, P[nc]);
+        }
+        const f32x4 step = beta, head = eb;
+        const float hold = whole;
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+            f32x4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                E[nc][r] = ec[r] * E[nc][r] + a.scale * P[nc][r];
+                x[r] = a.scale * eb[r] * In::to_f32(y[nc][r]);
+            }
+            share_tile<3, NC>(dbuf, w, nc, lane, E[nc]);
+            share_tile<3, NC>(wbuf, w, nc, lane, x);
+        }
+        if (c > 0) {
+            load_dout(c - 1);
+            load_rows(c - 1);
+            load_scales(c - 1);
+            load_tri(c - 1, a.ptf, pt);
+        }
+        lds_barrier();
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+            f32x4 Z = splat4(0.f);
+            bf16x8 b[3];
+            if (w < 2) {
+                shared_frag<3, NC>(dbuf, 0, nc, lane, b);
+                Z = mm(tt[0], b, Z);
+            }
+            shared_frag<3, NC>(dbuf, 1, nc, lane, b);
+            Z = mm(tt[1], b, Z);
+            const int n = sp.len - c * kDeltaChunk;
+            float* to = a.z + ((vslot0 + (size_t)c * a.hv) * kDeltaChunk + row) * a.dv_width + col + 16 * nc;
+            raw* dv = (raw*)a.dv + ((size_t)(sp.begin + c * kDeltaChunk + row) * a.hv + hv) * a.dv_width + col + 16 * nc;
+            f32x4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                to[r * a.dv_width] = Z[r];
+                const float d = step[r] * Z[r];
+                if (row + r < n) dv[(size_t)r * a.hv * a.dv_width] = In::from_f32(d);
+                x[r] = -head[r] * d;
+            }
+            share_tile<3, NC>(zbuf, w, nc, lane, x);
+        }
+        if (c > 0) load_tri(c - 1, a.ttf, tt);
+        lds_barrier();
+#pragma unroll
+        for (int i = 0; i < MW; ++i)
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[i][nc][r] *= hold;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc) {
+                bf16x8 b[3], e[3];
+                shared_frag<3, NC>(zbuf, ks, nc, lane, b);
+                shared_frag<3, NC>(wbuf, ks, nc, lane, e);
+#pragma unroll
+                for (int i = 0; i < MW; ++i) {
+                    S[i][nc] = mm(kt[i][ks], b, S[i][nc]);
+                    S[i][nc] = mm(qt[i][ks], e, S[i][nc]);
+                }
+            }
+        if (c > 0) {
+            load_columns(c - 1);
+            share(c - 1);
+        }
+        lds_barrier();
     }
     if (a.ds0) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int i = 0; i < MW; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) a.ds0[st + (size_t)(16 * m + 4 * q + r) * a.dv_width + col] = S[m][r];
+            for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) a.ds0[st + (size_t)(16 * i + r) * a.dv_width + 16 * nc] = S[i][nc][r];
     }
 }
 

@@ -65,8 +65,8 @@ int describe(const HelenDeltaRule* op, Check level, DeltaArgs* a) {
     if (!op->offsets && op->tokens % op->sequences)
         return fail(HELEN_EINVAL, "delta rule: %d tokens are no %d sequences of one length", op->tokens, op->sequences);
     const int64_t slots = (int64_t)op->tokens / kDeltaChunk + op->sequences + 1;
-    const int64_t chains = (int64_t)op->sequences * op->heads_v * ((op->width_v + 63) / 64);
-    if (slots > INT32_MAX || !grid_fits(slots * op->heads_k) || !grid_fits(chains * 8))
+    const int64_t chains = (int64_t)op->sequences * op->heads_v * (op->width_v / 16);
+    if (slots > INT32_MAX || !grid_fits(slots * op->heads_k) || !grid_fits(chains + 8))
         return fail(HELEN_EINVAL, "delta rule: %d tokens x %d heads in %d sequences are more than one call takes", op->tokens,
                     op->heads_v, op->sequences);
     const int size = type_size(op->dtype);
@@ -99,15 +99,17 @@ int describe(const HelenDeltaRule* op, Check level, DeltaArgs* a) {
     return HELEN_OK;
 }
 
+template <typename In, int DK, int PT, bool KEEP>
+void launch_forward(const DeltaArgs& a, hipStream_t s) {
+    if (a.tokens > 0) hipLaunchKernelGGL((delta_prep_kernel<In, DK, PT, KEEP>), dim3((unsigned)a.slots * a.hk), dim3(256), 0, s, a);
+    const int tiles = chain_tiles(a);
+    const dim3 grid(chain_grid(a, tiles));
+    if (tiles == 1) hipLaunchKernelGGL((delta_forward_kernel<In, DK, PT, KEEP, 1>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((delta_forward_kernel<In, DK, PT, KEEP, 2>), grid, dim3(256), 0, s, a);
+}
 template <typename In, int DK, int PT>
 void launch_forward(const DeltaArgs& a, int keep, hipStream_t s) {
-    const dim3 prep((unsigned)a.slots * a.hk), chain((unsigned)a.nseq * a.hv * ((a.dv_width + 63) / 64));
-    if (a.tokens > 0) {
-        if (keep) hipLaunchKernelGGL((delta_prep_kernel<In, DK, PT, true>), prep, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((delta_prep_kernel<In, DK, PT, false>), prep, dim3(256), 0, s, a);
-    }
-    if (keep) hipLaunchKernelGGL((delta_forward_kernel<In, DK, PT, true>), chain, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((delta_forward_kernel<In, DK, PT, false>), chain, dim3(256), 0, s, a);
+    keep ? launch_forward<In, DK, PT, true>(a, s) : launch_forward<In, DK, PT, false>(a, s);
 }
 
 }  // namespace

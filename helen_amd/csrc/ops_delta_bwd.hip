@@ -8,7 +8,10 @@ namespace {
 
 template <typename In, int DK>
 void launch(const DeltaArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL((delta_backward_kernel<In, DK>), dim3((unsigned)a.nseq * a.hv * ((a.dv_width + 63) / 64)), dim3(256), 0, s, a);
+    const int tiles = chain_tiles(a);
+    const dim3 grid(chain_grid(a, tiles));
+    if (tiles == 1) hipLaunchKernelGGL((delta_backward_kernel<In, DK, 1>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((delta_backward_kernel<In, DK, 2>), grid, dim3(256), 0, s, a);
     if (a.tokens > 0) hipLaunchKernelGGL((delta_grads_kernel<In, DK>), dim3((unsigned)a.slots * a.hk), dim3(256), 0, s, a);
 }
 
