@@ -4,8 +4,11 @@
 //     u_t = beta_t (v_t - e^{g_t} S_{t-1}^T k_t),   S_t = e^{g_t} S_{t-1} + k_t u_t^T,   o_t = scale S_t^T q_t
 // In a chunk of C = 64 tokens, with D_ij = sum of g over (j, i], b_i the sum from the chunk's start and c_i the sum after i
 // to its end, all C tokens are products (S0 = the state before the chunk):
-//     A_ij = beta_i (k_i . k_j) e^{D_ij} (j < i),  T = (I + A)^-1,   R = V - e^{b} K S0,   U = T beta R,
+//     A_ij = (k_i . k_j) e^{D_ij} beta_j (j < i),  T = (I + A)^-1,   R = V - e^{b} K S0,   E = T R,   U = beta E,
 //     O = scale (e^{b} Q S0 + P U),  P_ij = (q_i . k_j) e^{D_ij} (j <= i),   S1 = e^{b_C} S0 + K^T (e^{c} U)
+// (E_t = v_t - e^{g_t} S_{t-1}^T k_t, what the state got wrong.  With beta on the columns of A the backward pass needs E alone:
+// d beta = Z . E / beta, see kernels_delta_bwd.h.  A beta below 2^-64 counts as 2^-64 in A, far below a rounding, so that this
+// quotient exists where beta is zero; U takes beta as it is.)
 // A, T and P do not depend on the state: delta_prep_kernel makes them for every chunk at once.  What is left, one chunk after
 // another, is delta_forward_kernel: a column of S needs no other column, so a chain is split over its columns.
 //
@@ -117,8 +120,9 @@ struct DeltaArgs {
     // workspace: fragments per (slot, key head) and per (slot, value head)
     bf16x8 *kf, *ktf, *qf, *qtf;
     bf16x8 *tf, *ttf, *pf, *ptf;
+    f32x4* dots;                // kept: [slot, hk][10 tiles][K K^T | Q K^T][lane]
     float* sc;                  // [slot, hv][4][64]: beta, e^b, e^c, -
-    float *states, *u, *r;      // kept for the backward pass: [slot, hv, Dk, Dv], [slot, hv, 64, Dv] twice
+    float *states, *e;          // kept for the backward pass: [slot, hv, Dk, Dv], [slot, hv, 64, Dv]
     float *dstates, *z;         // backward: [slot, hv, Dk, Dv], [slot, hv, 64, Dv]
 };
 
@@ -166,6 +170,8 @@ __device__ __forceinline__ constexpr int tri_index(int mt, int ks) { return mt <
 __device__ __forceinline__ int trt_row(int f) { return f < 4 ? f >> 1 : f - 2; }
 __device__ __forceinline__ int trt_step(int f) { return f < 4 ? f & 1 : 1; }
 __device__ __forceinline__ constexpr int trt_index(int mt, int ks) { return mt < 2 ? 2 * mt + ks : mt + 2; }
+
+__device__ __forceinline__ float beta_of(float beta) { return fabsf(beta) < 0x1p-64f ? 0x1p-64f : beta; }
 
 // sums of the chunk's g (64 values in LDS) over its four blocks of 16
 __device__ __forceinline__ void block_sums(const float* gs, float (&block)[4]) {
@@ -218,6 +224,27 @@ __device__ __forceinline__ void decays(const float* gs, const float (&block)[4],
 #pragma unroll
         for (int r = 0; r < 4; ++r) out[nt][r] = expf(nt < w ? tail + head[r] : within[r]);
     }
+}
+// the same of one tile (mt, nt)
+__device__ __forceinline__ f32x4 tile_decay(const float* gs, const float (&block)[4], int mt, int nt, int j, int q) {
+    f32x4 sum = splat4(0.f);
+    float tail = 0.f;
+    if (nt < mt) {
+#pragma unroll
+        for (int m = 0; m < 16; ++m) tail += m > j ? gs[16 * nt + m] : 0.f;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) tail += (m > nt && m < mt) ? block[m] : 0.f;
+    }
+    const int from = nt < mt ? -1 : j;
+#pragma unroll
+    for (int m = 0; m < 16; ++m) {
+        const float gm = gs[16 * mt + m];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[r] += (m > from && m <= 4 * q + r) ? gm : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sum[r] = expf(tail + sum[r]);
+    return sum;
 }
 
 constexpr int kTriStride = 68;    // floats per row of a 64 x 64 matrix in LDS: rows 16-byte aligned, four banks apart
@@ -296,6 +323,15 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a) {
             }
         }
     }
+    if constexpr (BWD) {
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+            if (nt <= w) {
+                f32x4* to = a.dots + (((size_t)slot * a.hk + h) * 10 + w * (w + 1) / 2 + nt) * 128 + lane;
+                to[0] = kk[nt];
+                to[64] = qk[nt];
+            }
+    }
     // K^T (and Q^T): rows dk, k = tokens.  Element (token t, d) lies in fragment (t / 16, d / 32) at lane t % 16 + 16 ((d % 16) / 4)
     auto transposed = [&](bf16x8* to) {
         const unsigned short* src = (const unsigned short*)kfr;
@@ -357,7 +393,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = 16 * w + 4 * q + r, col = 16 * nt + j;
-                amat[i * kTriStride + col] = col < i ? bs[i] * (kk[nt][r] * decay[nt][r]) : 0.f;
+                amat[i * kTriStride + col] = col < i ? beta_of(bs[col]) * (kk[nt][r] * decay[nt][r]) : 0.f;
                 pmat[i * kTriStride + col] = col <= i ? qk[nt][r] * decay[nt][r] : 0.f;
             }
         }
@@ -492,11 +528,11 @@ __device__ __forceinline__ unsigned xcd_order(unsigned block, unsigned grid) { r
 // ------------------------------------------------------------------------------------------------
 // The chain: a workgroup per (sequence, value head, 16 NC columns of the state).  Each of its four waves owns a quarter of
 // the ROWS of everything: token tile w of R, U and O, the dk tiles of S from w DK/64 on.  The other waves' rows of a right-hand
-// operand (S, X = beta R, U) come through LDS as bf16 terms, three barriers a chunk; every left-hand fragment is read by
+// operand (S, R, U) come through LDS as bf16 terms, three barriers a chunk; every left-hand fragment is read by
 // one wave only, straight into registers, and the next chunk's are loaded into the registers the present chunk is done with.
 // ------------------------------------------------------------------------------------------------
 template <typename In, int DK, int PT, bool KEEP, int NC>
-__global__ __launch_bounds__(256) void delta_forward_kernel(const DeltaArgs a) {
+__global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_kernel(const DeltaArgs a) {
     constexpr int NI = In::kTerms, KS = DK / 32, MW = DK / 64;
     typedef typename In::raw raw;
     __shared__ bf16x8 sbuf[KS * 3 * NC * 64], xbuf[2 * 3 * NC * 64], ubuf[2 * PT * NC * 64], cbuf[2 * 3 * NC * 64];
@@ -621,23 +657,16 @@ __global__ __launch_bounds__(256) void delta_forward_kernel(const DeltaArgs a) {
                 R[nc] = mm(kf[ks], b, R[nc]);
                 O[nc] = mm(qf[ks], b, O[nc]);
             }
-        const f32x4 after = ec;
+        const f32x4 after = ec, step = beta;
         const float hold = whole;
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
-            f32x4 x;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 R[nc][r] = In::to_f32(v[nc][r]) - eb[r] * R[nc][r];
                 O[nc][r] *= eb[r];
-                x[r] = beta[r] * R[nc][r];
             }
-            share_tile<3, NC>(xbuf, w, nc, lane, x);
-            if constexpr (KEEP) {
-                float* to = a.r + ((vslot0 + (size_t)c * a.hv) * kDeltaChunk + row) * a.dv_width + col + 16 * nc;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) to[r * a.dv_width] = R[nc][r];
-            }
+            share_tile<3, NC>(xbuf, w, nc, lane, R[nc]);
         }
         if (more) {
             load_rows(c + 1);
@@ -658,10 +687,12 @@ __global__ __launch_bounds__(256) void delta_forward_kernel(const DeltaArgs a) {
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
             if constexpr (KEEP) {
-                float* to = a.u + ((vslot0 + (size_t)c * a.hv) * kDeltaChunk + row) * a.dv_width + col + 16 * nc;
+                float* to = a.e + ((vslot0 + (size_t)c * a.hv) * kDeltaChunk + row) * a.dv_width + col + 16 * nc;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) to[r * a.dv_width] = U[nc][r];
             }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) U[nc][r] *= step[r];
             share_tile<PT, NC>(ubuf, w, nc, lane, U[nc]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) U[nc][r] *= after[r];

@@ -1,11 +1,11 @@
 // kernels_delta_bwd.h -- backward pass of the gated delta rule (kernels_delta.h has the forward formulas and the layouts)
 //
 // With dO, dS1 the gradients of a chunk's outputs and of the state behind it:
-//     dU = scale P^T dO + e^{c} K dS1,   Z = T^T dU,   dV = beta Z,
-//     dS0 = e^{b_C} dS1 + Q^T (scale e^{b} dO) - K^T (e^{b} beta Z)                        (the reverse chain)
-//     dA = -tril(Z U^T, -1),  dP = scale tril(dO U^T),  G = beta dA e^{D},  H = dP e^{D}
-//     dQ = scale e^{b} dO S0^T + H K,   dK = -e^{b} beta Z S0^T + e^{c} U dS1^T + (G + G^T) K + H^T Q
-//     dbeta_i = Z_i . R_i + sum_j dA_ij (k_i . k_j) e^{D_ij}
+//     dU = scale P^T dO + e^{c} K dS1,   Z = T^T (beta dU) = dV,
+//     dS0 = e^{b_C} dS1 + Q^T (scale e^{b} dO) - K^T (e^{b} Z)                                (the reverse chain)
+//     dA = -tril(Z E^T, -1),  dP = scale tril(dO U^T),  G = dA e^{D} beta (of the column),  H = dP e^{D}
+//     dQ = scale e^{b} dO S0^T + H K,   dK = -e^{b} Z S0^T + e^{c} U dS1^T + (G + G^T) K + H^T Q
+//     dbeta_j = dU_j . E_j + sum_i dA_ij (k_i . k_j) e^{D_ij} = Z_j . E_j / beta_j      (since Z + A^T Z = beta dU)
 //     dg_m = sum_{j < m <= i} (dA A + dP P)_ij + sum_{i >= m} (q_i . dQ1_i + k_i . dK1_i) + sum_{i < m} k_i . dK2_i
 //            + e^{b_C} <S0, dS1>,   dQ1, dK1 = the S0 terms of dQ, dK;  dK2 = the dS1 term of dK
 // The reverse chain is the forward one with other operands; everything else of all chunks follows at once.  dg is summed over the positions it reaches, not as a difference of running sums.
@@ -16,7 +16,7 @@ namespace helen {
 
 // The reverse chain, built like delta_forward_kernel: wave w owns token tile w of dO, dU and Z and its quarter of dS's rows.
 template <typename In, int DK, int NC>
-__global__ __launch_bounds__(256) void delta_backward_kernel(const DeltaArgs a) {
+__global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_kernel(const DeltaArgs a) {
     constexpr int NI = In::kTerms, KS = DK / 32, MW = DK / 64;
     typedef typename In::raw raw;
     __shared__ bf16x8 sbuf[KS * 3 * NC * 64], ybuf[2 * NI * NC * 64], wbuf[2 * 3 * NC * 64], dbuf[2 * 3 * NC * 64], zbuf[2 * 3 * NC * 64];
@@ -146,14 +146,14 @@ __global__ __launch_bounds__(256) void delta_backward_kernel(const DeltaArgs a) 
             shared_frag<NI, NC>(ybuf, 1, nc, lane, b);
             P[nc] = mm(pt[1], b, P[nc]);
         }
-        const f32x4 step = beta, head = eb;
+        const f32x4 head = eb;
         const float hold = whole;
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
             f32x4 x;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                E[nc][r] = ec[r] * E[nc][r] + a.scale * P[nc][r];
+                E[nc][r] = beta_of(beta[r]) * (ec[r] * E[nc][r] + a.scale * P[nc][r]);
                 x[r] = a.scale * eb[r] * In::to_f32(y[nc][r]);
             }
             share_tile<3, NC>(dbuf, w, nc, lane, E[nc]);
@@ -183,9 +183,8 @@ __global__ __launch_bounds__(256) void delta_backward_kernel(const DeltaArgs a) 
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 to[r * a.dv_width] = Z[r];
-                const float d = step[r] * Z[r];
-                if (row + r < n) dv[(size_t)r * a.hv * a.dv_width] = In::from_f32(d);
-                x[r] = -head[r] * d;
+                if (row + r < n) dv[(size_t)r * a.hv * a.dv_width] = In::from_f32(Z[r]);
+                x[r] = -head[r] * Z[r];
             }
             share_tile<3, NC>(zbuf, w, nc, lane, x);
         }
@@ -226,32 +225,59 @@ __global__ __launch_bounds__(256) void delta_backward_kernel(const DeltaArgs a) 
     }
 }
 
-// sum over the 16 lanes of a quarter
-__device__ __forceinline__ float sum16(float x) {
+// sum over the 16 lanes of a quarter (rotations within a row of 16 lanes, on the VALU), over a wave, and running sums
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+    return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float sum16(float x) { return dpp_add<0x121>(dpp_add<0x122>(dpp_add<0x124>(dpp_add<0x128>(x)))); }
+__device__ __forceinline__ float sum64(float x) {
+    x = sum16(x);
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+__device__ __forceinline__ float sum_before(float x, int lane) {      // over the lanes below
+    float sum = x;
 #pragma unroll
-    for (int m = 1; m < 16; m <<= 1) x += __shfl_xor(x, m);
+    for (int m = 1; m < 64; m <<= 1) {
+        const float y = __shfl_up(sum, m);
+        sum += lane >= m ? y : 0.f;
+    }
+    const float y = __shfl_up(sum, 1);
+    return lane ? y : 0.f;
+}
+__device__ __forceinline__ float sum_from(float x, int lane) {        // over this lane and those above
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const float y = __shfl_down(x, m);
+        x += lane + m < 64 ? y : 0.f;
+    }
     return x;
 }
 
 // ------------------------------------------------------------------------------------------------
-// dQ, dK, dbeta and dg of one chunk: a workgroup per (slot, key head).  The value heads of the key head follow one another
-// and are summed in registers: no atomics, one order.  Wave w: token tile w of everything that is 64 x 64 and of the staging,
-// columns dk = w DK/4 .. of everything that is 64 x DK.
+// dQ, dK, dbeta and dg of one chunk: a workgroup of DK / 16 waves per (slot, key head).  The value heads of the key head follow
+// one another and are summed in registers: no atomics, one order.
+//   64 x DK results: wave w has dk tiles 2 p, 2 p + 1 (p = w % (DK / 32)) of token tiles 2 mh, 2 mh + 1 (mh = w / (DK / 32))
+//   64 x 64 results: the ten tiles on and below the diagonal go round the waves
+// dv is walked 32 columns a step: Z, E and dO of the step as fragments in LDS (two buffers, one barrier a step), the states
+// straight into registers; both are loaded a step ahead.
 // ------------------------------------------------------------------------------------------------
-template <typename In, int DK>
-__global__ __launch_bounds__(256) void delta_grads_kernel(const DeltaArgs a) {
-    constexpr int NI = In::kTerms, KS = DK / 32, NT = DK / 64;
+template <typename In, int DK, bool SHARED>
+__global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) {
+    constexpr int NI = In::kTerms, KS = DK / 32, W = DK / 16, NP = DK / 32, TPW = (10 + W - 1) / W, RB = 64 / W;
     typedef typename In::raw raw;
-    constexpr int kStage = 4 * (6 + NI), kTail = 3 * (8 + 2 * kTriFrags), kKeys = 4 * KS * NI;
-    constexpr int kFrags = kTail > kKeys ? (kTail > kStage ? kTail : kStage) : (kKeys > kStage ? kKeys : kStage);
-    __shared__ bf16x8 fr[kFrags * 64];
-    __shared__ f32x4 gmat4[64 * kTriStride / 4], hmat4[64 * kTriStride / 4], dmat4[64 * kTriStride / 4];
-    __shared__ float gs[64], bs[64], sums[2][4][64], zr[64], da_row[64], gamma[4], part[4][64];
-    float* const gmat = (float*)gmat4;
-    float* const hmat = (float*)hmat4;
-    float* const dmat = (float*)dmat4;
+    constexpr int kStage = 4 * (6 + NI);
+    __shared__ bf16x8 stage[2 * kStage * 64];
+    __shared__ bf16x8 fr[3 * (8 + 2 * kTriFrags) * 64];
+    __shared__ float gs[64], bs[64], scl[192], sums[2][NP][64], dbeta[64], gamma[NP], part[W][64];
+    static_assert(sizeof(stage) >= 3 * 64 * kTriStride * 4, "the 64 x 64 gradients take the stage's place");
+    float* const gmat = (float*)stage;
+    float* const hmat = gmat + 64 * kTriStride;
+    float* const dmat = hmat + 64 * kTriStride;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int j = lane & 15, q = lane >> 4;
+    const int p = w % NP, mh = w / NP;
     const int slot = blockIdx.x / a.hk, h = blockIdx.x % a.hk;
     const int s = sequence_of(a, slot, lane);
     const Span sp = span_of(a, s);
@@ -263,10 +289,10 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(const DeltaArgs a) {
             const int end = sp.begin + sp.len;
             const int lo = max(end, (slot - a.nseq) * kDeltaChunk), hi = min(a.tokens, (slot - a.nseq + 1) * kDeltaChunk);
             for (int t = lo; t < hi; ++t) {
-                for (int d = threadIdx.x; d < DK; d += 256)
+                for (int d = threadIdx.x; d < DK; d += DK * 4)
                     ((raw*)a.dq)[((size_t)t * a.hk + h) * DK + d] = ((raw*)a.dk)[((size_t)t * a.hk + h) * DK + d] = raw(0);
                 for (int hv = h * a.group; hv < (h + 1) * a.group; ++hv) {
-                    for (int d = threadIdx.x; d < a.dv_width; d += 256)
+                    for (int d = threadIdx.x; d < a.dv_width; d += DK * 4)
                         ((raw*)a.dv)[((size_t)t * a.hv + hv) * a.dv_width + d] = raw(0);
                     if (threadIdx.x == 0) a.dg[(size_t)t * a.hv + hv] = a.dbeta[(size_t)t * a.hv + hv] = 0.f;
                 }
@@ -275,200 +301,223 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(const DeltaArgs a) {
         return;
     }
     const size_t kslot = (size_t)slot * a.hk + h;
-
-    // K K^T and Q K^T, row tile w
-    f32x4 kk[4], qk[4];
-    for (int f = w; f < kKeys; f += 4) fr[f * 64 + lane] = a.kf[(kslot * kKeys + f) * 64 + lane];
-    __syncthreads();
-    {
-        bf16x8 qf[KS][NI];
+    int tm[TPW], tn[TPW];          // this wave's 64 x 64 tiles; a wave that has fewer repeats its first and drops the result
+    bool own[TPW];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int t = 0; t < NI; ++t) qf[ks][t] = a.qf[(((kslot * 4 + w) * KS + ks) * NI + t) * 64 + lane];
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-            kk[nt] = qk[nt] = splat4(0.f);
-            if (nt <= w) {
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    bf16x8 b[NI], kf[NI];
-#pragma unroll
-                    for (int t = 0; t < NI; ++t) {
-                        b[t] = fr[((nt * KS + ks) * NI + t) * 64 + lane];
-                        kf[t] = fr[((w * KS + ks) * NI + t) * 64 + lane];
-                    }
-                    kk[nt] = mm(kf, b, kk[nt]);
-                    qk[nt] = mm(qf[ks], b, qk[nt]);
-                }
-            }
-        }
+    for (int t = 0; t < TPW; ++t) {
+        own[t] = w + W * t < 10;
+        const int id = own[t] ? w + W * t : w;
+        tm[t] = id < 1 ? 0 : (id < 3 ? 1 : (id < 6 ? 2 : 3));
+        tn[t] = id - tm[t] * (tm[t] + 1) / 2;
     }
-
-    f32x4 dQ[NT][4], dK[NT][4];
+    f32x4 dQ[2][2], dK[2][2];      // [dk tile][token tile], summed over the value heads
+    if constexpr (SHARED) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) dQ[i][mt] = dK[i][mt] = splat4(0.f);
-
+            for (int m = 0; m < 2; ++m) dQ[i][m] = dK[i][m] = splat4(0.f);
+    }
+    const bool has_z = W == 4 || w < 4;     // who stages Z and dO, and who E, of token tile w & 3
+    const int srow = 16 * (w & 3) + j;
     for (int hv = h * a.group; hv < (h + 1) * a.group; ++hv) {
         const size_t vslot = (size_t)slot * a.hv + hv;
-        const float* sc = a.sc + vslot * 256;
         __syncthreads();
         if (w == 0) {
             const bool in = lane < n;
             gs[lane] = in ? a.g[(start + lane) * a.g_t + hv * a.g_h] : 0.f;
             bs[lane] = in ? a.beta[(start + lane) * a.b_t + hv * a.b_h] : 0.f;
+        } else if (w < 4) {
+            scl[threadIdx.x - 64] = a.sc[vslot * 256 + threadIdx.x - 64];
         }
-        // products over dv, 32 columns a step
-        f32x4 q1[NT][4], k1[NT][4], k2[NT][4], da[4], dp[4];
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int mt = 0; mt < 4; ++mt) q1[i][mt] = k1[i][mt] = k2[i][mt] = splat4(0.f);
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt) da[nt] = dp[nt] = splat4(0.f);
-        float dots = 0.f, zrow = 0.f;
-        for (int d0 = 0; d0 < a.dv_width; d0 += 32) {
-            const int row = 16 * w + j;
-            const size_t at = (vslot * kDeltaChunk + row) * a.dv_width + d0 + 4 * q;
-            const f32x4 z0 = *(const f32x4*)(a.z + at), z1 = *(const f32x4*)(a.z + at + 16);
-            const f32x4 u0 = *(const f32x4*)(a.u + at), u1 = *(const f32x4*)(a.u + at + 16);
-            const f32x4 r0 = *(const f32x4*)(a.r + at), r1 = *(const f32x4*)(a.r + at + 16);
-            f32x4 y0 = splat4(0.f), y1 = splat4(0.f);
-            if (row < n) {
-                const raw* yp = (const raw*)a.dout + (start + row) * a.do_t + hv * a.do_h + d0 + 4 * q;
-                y0 = load4<In>(yp);
-                y1 = load4<In>(yp + 16);
+        f32x4 x0, x1, e0, e1, y0, y1, sa[2][2], sd[2][2];   // (eight waves: x is Z or E)
+        auto load = [&](int d0) {
+            const size_t at = (vslot * kDeltaChunk + srow) * a.dv_width + d0 + 4 * q;
+            const float* xp = (has_z ? a.z : a.e) + at;
+            x0 = *(const f32x4*)xp;
+            x1 = *(const f32x4*)(xp + 16);
+            if (has_z) {
+                y0 = y1 = splat4(0.f);
+                if (srow < n) {
+                    const raw* yp = (const raw*)a.dout + (start + srow) * a.do_t + hv * a.do_h + d0 + 4 * q;
+                    y0 = load4<In>(yp);
+                    y1 = load4<In>(yp + 16);
+                }
+            }
+            if constexpr (W == 4) {
+                e0 = *(const f32x4*)(a.e + at);
+                e1 = *(const f32x4*)(a.e + at + 16);
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) zrow += z0[r] * r0[r] + z1[r] * r1[r];
-            bf16x8 zt[3], ut[3], yt[NI];
-            split8<3>(z0, z1, zt);
-            split8<3>(u0, u1, ut);
-            split8<NI>(y0, y1, yt);
-            __syncthreads();
-#pragma unroll
-            for (int t = 0; t < 3; ++t) {
-                fr[(w * 3 + t) * 64 + lane] = zt[t];
-                fr[(12 + w * 3 + t) * 64 + lane] = ut[t];
+            for (int i = 0; i < 2; ++i) {
+                const size_t sat = (vslot * DK + 16 * (2 * p + i) + j) * a.dv_width + d0 + 4 * q;
+                sa[i][0] = *(const f32x4*)(a.states + sat);
+                sa[i][1] = *(const f32x4*)(a.states + sat + 16);
+                sd[i][0] = *(const f32x4*)(a.dstates + sat);
+                sd[i][1] = *(const f32x4*)(a.dstates + sat + 16);
             }
+        };
+        auto put = [&](bf16x8* to) {
+            bf16x8 t[3];
+            split8<3>(x0, x1, t);
 #pragma unroll
-            for (int t = 0; t < NI; ++t) fr[(24 + w * NI + t) * 64 + lane] = yt[t];
-            __syncthreads();
+            for (int k = 0; k < 3; ++k) to[((has_z ? 0 : 12) + (w & 3) * 3 + k) * 64 + lane] = t[k];
+            if (has_z) {
+                bf16x8 y[NI];
+                split8<NI>(y0, y1, y);
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const size_t sat = (vslot * DK + 16 * (w * NT + i) + j) * a.dv_width + d0 + 4 * q;
-                const f32x4 a0 = *(const f32x4*)(a.states + sat), a1 = *(const f32x4*)(a.states + sat + 16);
-                const f32x4 b0 = *(const f32x4*)(a.dstates + sat), b1 = *(const f32x4*)(a.dstates + sat + 16);
+                for (int k = 0; k < NI; ++k) to[(24 + (w & 3) * NI + k) * 64 + lane] = y[k];
+            }
+            if constexpr (W == 4) {
+                split8<3>(e0, e1, t);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) dots += a0[r] * b0[r] + a1[r] * b1[r];
-                bf16x8 st[3], dt[3];
-                split8<3>(a0, a1, st);
-                split8<3>(b0, b1, dt);
+                for (int k = 0; k < 3; ++k) to[(12 + (w & 3) * 3 + k) * 64 + lane] = t[k];
+            }
+        };
+        f32x4 q1[2][2], k1[2][2], k2[2][2], da[TPW], dp[TPW];
 #pragma unroll
-                for (int mt = 0; mt < 4; ++mt) {
-                    bf16x8 zf[3], uf[3], yf[NI];
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int t = 0; t < 3; ++t) {
-                        zf[t] = fr[(mt * 3 + t) * 64 + lane];
-                        uf[t] = fr[(12 + mt * 3 + t) * 64 + lane];
-                    }
+            for (int m = 0; m < 2; ++m) q1[i][m] = k1[i][m] = k2[i][m] = splat4(0.f);
 #pragma unroll
-                    for (int t = 0; t < NI; ++t) yf[t] = fr[(24 + mt * NI + t) * 64 + lane];
-                    q1[i][mt] = mm(yf, st, q1[i][mt]);
-                    k1[i][mt] = mm(zf, st, k1[i][mt]);
-                    k2[i][mt] = mm(uf, dt, k2[i][mt]);
+        for (int t = 0; t < TPW; ++t) da[t] = dp[t] = splat4(0.f);
+        float dots = 0.f;
+        load(0);
+        put(stage);
+        for (int d0 = 0, buf = 0; d0 < a.dv_width; d0 += 32, buf ^= 1) {
+            const bf16x8* const from = stage + buf * kStage * 64;
+            bf16x8 st[2][3], dt[2][3];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) dots += sa[i][0][r] * sd[i][0][r] + sa[i][1][r] * sd[i][1][r];
+                split8<3>(sa[i][0], sa[i][1], st[i]);
+                split8<3>(sd[i][0], sd[i][1], dt[i]);
+            }
+            const bool more = d0 + 32 < a.dv_width;
+            if (more) load(d0 + 32);
+            lds_barrier();
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                bf16x8 zf[3], ef[3], yf[NI];
+#pragma unroll
+                for (int t = 0; t < 3; ++t) {
+                    zf[t] = from[((2 * mh + m) * 3 + t) * 64 + lane];
+                    ef[t] = from[(12 + (2 * mh + m) * 3 + t) * 64 + lane];
+                }
+#pragma unroll
+                for (int t = 0; t < NI; ++t) yf[t] = from[(24 + (2 * mh + m) * NI + t) * 64 + lane];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    q1[i][m] = mm(yf, st[i], q1[i][m]);
+                    k1[i][m] = mm(zf, st[i], k1[i][m]);
+                    k2[i][m] = mm(ef, dt[i], k2[i][m]);
                 }
             }
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt)
-                if (nt <= w) {
-                    bf16x8 uf[3];
+            for (int t = 0; t < TPW; ++t) {
+                if (!own[t]) continue;
+                bf16x8 zf[3], ef[3], yf[NI];
 #pragma unroll
-                    for (int t = 0; t < 3; ++t) uf[t] = fr[(12 + nt * 3 + t) * 64 + lane];
-                    da[nt] = mm(zt, uf, da[nt]);
-                    dp[nt] = mm(yt, uf, dp[nt]);
+                for (int k = 0; k < 3; ++k) {
+                    zf[k] = from[(tm[t] * 3 + k) * 64 + lane];
+                    ef[k] = from[(12 + tn[t] * 3 + k) * 64 + lane];
                 }
+#pragma unroll
+                for (int k = 0; k < NI; ++k) yf[k] = from[(24 + tm[t] * NI + k) * 64 + lane];
+                da[t] = mm(zf, ef, da[t]);
+                dp[t] = mm(yf, ef, dp[t]);
+            }
+            if (more) put(stage + (buf ^ 1) * kStage * 64);
         }
-        // Z_i . R_i, <S0, dS1>
-        zrow += __shfl_xor(zrow, 16);
-        zrow += __shfl_xor(zrow, 32);
-        if (q == 0) zr[16 * w + j] = zrow;
-        dots = sum16(dots);
-        dots += __shfl_xor(dots, 16);
-        dots += __shfl_xor(dots, 32);
-        if (lane == 0) gamma[w] = dots;
+        // K^T and Q^T of this wave's dk tiles: B operands below, and -- element r of half m of step ks -- the values of token
+        // 16 (2 ks + m) + 4 q + r that the dots need
+        bf16x8 kt[2][2][NI], qt[2][2][NI];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int t = 0; t < NI; ++t) {
+                    const size_t at = ((kslot * (DK / 16) * 2 + 2 * (2 * p + i) + ks) * NI + t) * 64 + lane;
+                    kt[i][ks][t] = a.ktf[at];
+                    qt[i][ks][t] = a.qtf[at];
+                }
+        f32x4 kk[TPW], qk[TPW];
+#pragma unroll
+        for (int t = 0; t < TPW; ++t) {
+            const f32x4* at = a.dots + (kslot * 10 + tm[t] * (tm[t] + 1) / 2 + tn[t]) * 128 + lane;
+            kk[t] = at[0];
+            qk[t] = at[64];
+        }
+        if (mh == 0) {
+            dots = sum64(dots);
+            if (lane == 0) gamma[p] = dots;
+        }
+        // the 64 x 64 gradients, in the stage's place
+        __syncthreads();
+        {
+            float block[4];
+            block_sums(gs, block);
+#pragma unroll
+            for (int t = 0; t < TPW; ++t) {
+                if (!own[t]) continue;
+                const f32x4 decay = tile_decay(gs, block, tm[t], tn[t], j, q);
+                const int col = 16 * tn[t] + j;
+                const float beta = bs[col], beta1 = beta_of(beta);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = 16 * tm[t] + 4 * q + r;
+                    if (col == i) dbeta[i] = da[t][r] / beta1;
+                    const float e = col <= i ? decay[r] : 0.f;
+                    const float A = col < i ? -da[t][r] * (beta1 * e) : 0.f, P = col <= i ? a.scale * beta * dp[t][r] : 0.f;
+                    if (col <= i) gmat[i * kTriStride + col] = gmat[col * kTriStride + i] = A;
+                    hmat[i * kTriStride + col] = P * e;
+                    dmat[i * kTriStride + col] = col < i ? A * kk[t][r] + P * (qk[t][r] * e) : 0.f;
+                }
+            }
+        }
         // rows' scales, and the dots with q and k that dg needs
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-            const f32x4 beta = *(const f32x4*)(sc + 16 * mt + 4 * q), eb = *(const f32x4*)(sc + 64 + 16 * mt + 4 * q),
-                        ec = *(const f32x4*)(sc + 128 + 16 * mt + 4 * q);
+        for (int m = 0; m < 2; ++m) {
+            const int t0 = 16 * (2 * mh + m) + 4 * q;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int t = 16 * mt + 4 * q + r;
+                const float beta = scl[t0 + r], eb = scl[64 + t0 + r], ec = scl[128 + t0 + r];
                 float from = 0.f, to = 0.f;
 #pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    const int d = 16 * (w * NT + i) + j;
-                    q1[i][mt][r] *= a.scale * eb[r];
-                    k1[i][mt][r] *= -(eb[r] * beta[r]);
-                    k2[i][mt][r] *= ec[r];
-                    if (t < n) {
-                        const float qv = In::to_f32(((const raw*)a.q)[(start + t) * a.q_t + h * a.q_h + d]);
-                        const float kv = In::to_f32(((const raw*)a.k)[(start + t) * a.k_t + h * a.k_h + d]);
-                        from += qv * q1[i][mt][r] + kv * k1[i][mt][r];
-                        to += kv * k2[i][mt][r];
+                for (int i = 0; i < 2; ++i) {
+                    float kv = 0.f, qv = 0.f;
+#pragma unroll
+                    for (int t = NI - 1; t >= 0; --t) {
+                        kv += (float)(mh ? kt[i][1][t] : kt[i][0][t])[4 * m + r];
+                        qv += (float)(mh ? qt[i][1][t] : qt[i][0][t])[4 * m + r];
                     }
-                    dQ[i][mt][r] += q1[i][mt][r];
-                    dK[i][mt][r] += k1[i][mt][r] + k2[i][mt][r];
+                    q1[i][m][r] *= a.scale * eb;
+                    k1[i][m][r] *= -eb;
+                    k2[i][m][r] *= ec * beta;
+                    from += qv * q1[i][m][r] + kv * k1[i][m][r];
+                    to += kv * k2[i][m][r];
+                    k1[i][m][r] += k2[i][m][r];
                 }
                 from = sum16(from);
                 to = sum16(to);
                 if (j == 0) {
-                    sums[0][w][t] = from;
-                    sums[1][w][t] = to;
+                    sums[0][p][t0 + r] = from;
+                    sums[1][p][t0 + r] = to;
                 }
             }
         }
-        // the 64 x 64 gradients
-        float block[4];
-        f32x4 decay[4];
-        block_sums(gs, block);
-        decays(gs, block, w, j, q, decay);
-        f32x4 row_sum = splat4(0.f);
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-            if (nt > w) continue;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * w + 4 * q + r, col = 16 * nt + j;
-                const float e = col <= i ? decay[nt][r] : 0.f;
-                const float A = col < i ? -da[nt][r] : 0.f, P = col <= i ? a.scale * dp[nt][r] : 0.f;
-                const float ke = col < i ? kk[nt][r] * e : 0.f;
-                row_sum[r] += A * ke;
-                const float g = A * (bs[i] * e);
-                if (col <= i) gmat[i * kTriStride + col] = gmat[col * kTriStride + i] = g;
-                hmat[i * kTriStride + col] = P * e;
-                dmat[i * kTriStride + col] = A * (bs[i] * ke) + (col < i ? P * (qk[nt][r] * e) : 0.f);
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float x = sum16(row_sum[r]);
-            if (j == 0) da_row[16 * w + 4 * q + r] = x;
-        }
         __syncthreads();
         // A operands of the products with K and Q: G + G^T (8 fragments), H, H^T
-        for (int f = w; f < 8 + 2 * kTriFrags; f += 4) {
+        for (int f = w; f < 8 + 2 * kTriFrags; f += W) {
             f32x4 lo, hi;
             if (f < 8) {
-                const f32x4* m4 = gmat4 + ((16 * (f >> 1) + j) * kTriStride + 32 * (f & 1) + 4 * q) / 4;
+                const f32x4* m4 = (const f32x4*)(gmat + (16 * (f >> 1) + j) * kTriStride + 32 * (f & 1) + 4 * q);
                 lo = m4[0];
                 hi = m4[4];
             } else if (f < 8 + kTriFrags) {
                 const int mt = tri_row(f - 8), ks = tri_step(f - 8);
-                const f32x4* m4 = hmat4 + ((16 * mt + j) * kTriStride + 32 * ks + 4 * q) / 4;
+                const f32x4* m4 = (const f32x4*)(hmat + (16 * mt + j) * kTriStride + 32 * ks + 4 * q);
                 lo = m4[0];
                 hi = (mt & 1) || ks < (mt >> 1) ? m4[4] : splat4(0.f);
             } else {
@@ -485,85 +534,90 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(const DeltaArgs a) {
 #pragma unroll
             for (int k = 0; k < 3; ++k) fr[(f * 3 + k) * 64 + lane] = t[k];
         }
-        // dg, first half: sums of column `lane` over rows i >= m, for m in this wave's 16 rows (in place, below)
+        // dg: sums of column `lane` over rows i >= m, for m in this wave's rows; what the rows below this wave's give follows
+        float run[RB];
         {
             float below = 0.f;
-            for (int i = 16 * (w + 1); i < 64; ++i) below += lane < i ? dmat[i * kTriStride + lane] : 0.f;
-            float run[16];
 #pragma unroll
-            for (int m = 15; m >= 0; --m) {
-                const int i = 16 * w + m;
+            for (int m = RB - 1; m >= 0; --m) {
+                const int i = RB * w + m;
                 below += lane < i ? dmat[i * kTriStride + lane] : 0.f;
                 run[m] = below;
             }
-            __syncthreads();
-#pragma unroll
-            for (int m = 0; m < 16; ++m)
-                if (lane < 16 * w + m) dmat[(16 * w + m) * kTriStride + lane] = run[m];
+            part[w][lane] = below;
         }
         __syncthreads();
-        {
-            float x = 0.f;
-#pragma unroll
-            for (int m = 0; m < 16; ++m) x += 16 * w + m < lane ? dmat[lane * kTriStride + 16 * w + m] : 0.f;
-            part[w][lane] = x;
-        }
-        __syncthreads();
-        if (w == 0) {
-            float x = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
-            float from = 0.f, to = 0.f;
-            for (int i = 0; i < 64; ++i) {
-                from += i >= lane ? (sums[0][0][i] + sums[0][1][i]) + (sums[0][2][i] + sums[0][3][i]) : 0.f;
-                to += i < lane ? (sums[1][0][i] + sums[1][1][i]) + (sums[1][2][i] + sums[1][3][i]) : 0.f;
-            }
-            x += from + to + sc[64 + 63] * ((gamma[0] + gamma[1]) + (gamma[2] + gamma[3]));
-            if (lane < n) {
-                a.dg[(size_t)(start + lane) * a.hv + hv] = x;
-                a.dbeta[(size_t)(start + lane) * a.hv + hv] = zr[lane] + da_row[lane];
-            }
-        }
         // dQ += H K,  dK += (G + G^T) K + H^T Q
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+        for (int m = 0; m < 2; ++m) {
+            const int mt = 2 * mh + m;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                bf16x8 kt[NI], qt[NI];
+                bf16x8 x[3];
 #pragma unroll
-                for (int t = 0; t < NI; ++t) {
-                    const size_t at = ((kslot * (DK / 16) * 2 + 2 * (w * NT + i) + ks) * NI + t) * 64 + lane;
-                    kt[t] = a.ktf[at];
-                    qt[t] = a.qtf[at];
+                for (int t = 0; t < 3; ++t) x[t] = fr[((2 * mt + ks) * 3 + t) * 64 + lane];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) k1[i][m] = mm(x, kt[i][ks], k1[i][m]);
+                if (ks <= mh) {
+#pragma unroll
+                    for (int t = 0; t < 3; ++t) x[t] = fr[((8 + tri_index(mt, ks)) * 3 + t) * 64 + lane];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) q1[i][m] = mm(x, kt[i][ks], q1[i][m]);
                 }
+                if (ks >= mh) {
 #pragma unroll
-                for (int mt = 0; mt < 4; ++mt) {
-                    bf16x8 m[3];
+                    for (int t = 0; t < 3; ++t) x[t] = fr[((8 + kTriFrags + trt_index(mt, ks)) * 3 + t) * 64 + lane];
 #pragma unroll
-                    for (int t = 0; t < 3; ++t) m[t] = fr[((2 * mt + ks) * 3 + t) * 64 + lane];
-                    dK[i][mt] = mm(m, kt, dK[i][mt]);
-                    if (ks <= mt / 2) {
+                    for (int i = 0; i < 2; ++i) k1[i][m] = mm(x, qt[i][ks], k1[i][m]);
+                }
+            }
+        }
+        // dg_m of this wave's rows: the rectangle, what leaves before m and arrives from m on, what the state carries over
+        {
+            float below = 0.f, f = 0.f, g = 0.f, hold = 0.f;
 #pragma unroll
-                        for (int t = 0; t < 3; ++t) m[t] = fr[((8 + tri_index(mt, ks)) * 3 + t) * 64 + lane];
-                        dQ[i][mt] = mm(m, kt, dQ[i][mt]);
-                    }
-                    if (ks >= mt / 2) {
+            for (int k = 1; k < W; ++k) below += k > w ? part[k][lane] : 0.f;
 #pragma unroll
-                        for (int t = 0; t < 3; ++t) m[t] = fr[((8 + kTriFrags + trt_index(mt, ks)) * 3 + t) * 64 + lane];
-                        dK[i][mt] = mm(m, qt, dK[i][mt]);
-                    }
+            for (int k = 0; k < NP; ++k) {
+                f += sums[0][k][lane];
+                g += sums[1][k][lane];
+                hold += gamma[k];
+            }
+            float mine = sum_from(f, lane) + sum_before(g, lane) + scl[64 + 63] * hold;
+#pragma unroll
+            for (int m = 0; m < RB; ++m) {
+                const float x = sum64(lane < RB * w + m ? run[m] + below : 0.f);
+                mine += lane == RB * w + m ? x : 0.f;
+            }
+            if (lane / RB == w && lane < n) {
+                a.dg[(size_t)(start + lane) * a.hv + hv] = mine;
+                a.dbeta[(size_t)(start + lane) * a.hv + hv] = dbeta[lane];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                if constexpr (SHARED) {
+                    dQ[i][m] += q1[i][m];
+                    dK[i][m] += k1[i][m];
+                } else {
+                    dQ[i][m] = q1[i][m];
+                    dK[i][m] = k1[i][m];
                 }
             }
     }
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt)
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int t = 16 * mt + 4 * q + r;
+                const int t = 16 * (2 * mh + m) + 4 * q + r;
                 if (t >= n) continue;
-                const size_t at = ((size_t)(start + t) * a.hk + h) * DK + 16 * (w * NT + i) + j;
-                ((raw*)a.dq)[at] = In::from_f32(dQ[i][mt][r]);
-                ((raw*)a.dk)[at] = In::from_f32(dK[i][mt][r]);
+                const size_t at = ((size_t)(start + t) * a.hk + h) * DK + 16 * (2 * p + i) + j;
+                ((raw*)a.dq)[at] = In::from_f32(dQ[i][m][r]);
+                ((raw*)a.dk)[at] = In::from_f32(dK[i][m][r]);
             }
 }
 

@@ -31,11 +31,11 @@ size_t carve(const HelenDeltaRule& op, int keep, void* base, DeltaArgs* a) {
     a->sc = c.take<float>(vs * 256);
     if (keep) {
         a->qtf = c.take<bf16x8>(rows);
+        a->dots = c.take<f32x4>(ks * 10 * 128);
         a->ttf = c.take<bf16x8>(tri * 3);
         a->ptf = c.take<bf16x8>(tri * 3);
         a->states = c.take<float>(vs * op.width_k * op.width_v);
-        a->u = c.take<float>(vs * kDeltaChunk * op.width_v);
-        a->r = c.take<float>(vs * kDeltaChunk * op.width_v);
+        a->e = c.take<float>(vs * kDeltaChunk * op.width_v);
     }
     return c.at;
 }

@@ -12,7 +12,10 @@ void launch(const DeltaArgs& a, hipStream_t s) {
     const dim3 grid(chain_grid(a, tiles));
     if (tiles == 1) hipLaunchKernelGGL((delta_backward_kernel<In, DK, 1>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((delta_backward_kernel<In, DK, 2>), grid, dim3(256), 0, s, a);
-    if (a.tokens > 0) hipLaunchKernelGGL((delta_grads_kernel<In, DK>), dim3((unsigned)a.slots * a.hk), dim3(256), 0, s, a);
+    if (a.tokens == 0) return;
+    const dim3 chunks((unsigned)a.slots * a.hk), block(DK * 4);
+    if (a.group == 1) hipLaunchKernelGGL((delta_grads_kernel<In, DK, false>), chunks, block, 0, s, a);
+    else hipLaunchKernelGGL((delta_grads_kernel<In, DK, true>), chunks, block, 0, s, a);
 }
 
 }  // namespace
