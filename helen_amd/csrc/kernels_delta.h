@@ -173,79 +173,72 @@ __device__ __forceinline__ constexpr int trt_index(int mt, int ks) { return mt <
 
 __device__ __forceinline__ float beta_of(float beta) { return fabsf(beta) < 0x1p-64f ? 0x1p-64f : beta; }
 
-// sums of the chunk's g (64 values in LDS) over its four blocks of 16
-__device__ __forceinline__ void block_sums(const float* gs, float (&block)[4]) {
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        block[b] = 0.f;
-#pragma unroll
-        for (int m = 0; m < 16; ++m) block[b] += gs[16 * b + m];
-    }
+// e^x of a decay: 2^(x log2 e) with the product's rounding error put back (v_exp_f32 alone would be off by |x| 2^-24); 0 from
+// -150 down, -inf included; a NaN stays one
+__device__ __forceinline__ float exp_decay(float x) {
+    x = x < -150.f ? -150.f : x;
+    const float t = x * 1.44269504f;
+    const float low = __builtin_fmaf(x, 1.44269504f, -t) + x * 1.9259630e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(e, low * 0.693147181f, e);
 }
-// sums of g from the chunk's start up to and with token `lane`, and of those after it
-__device__ __forceinline__ void head_tail(const float* gs, const float (&block)[4], int lane, float* head_out, float* tail_out) {
-    const int j = lane & 15, b = lane >> 4;
-    float head = 0.f, tail = 0.f;
-#pragma unroll
-    for (int m = 0; m < 16; ++m) {
-        head += m <= j ? gs[16 * b + m] : 0.f;
-        tail += m > j ? gs[16 * b + m] : 0.f;
-    }
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-        head += m < b ? block[m] : 0.f;
-        tail += m > b ? block[m] : 0.f;
-    }
-    *head_out = head;
-    *tail_out = tail;
+
+// the lane's own value plus others of its row of 16 lanes (rotations and shifts on the VALU; shifts bring in zeros)
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+    return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
-// e^{D_ij} of rows i = 16 w + 4 q + r, columns 16 nt + j, nt <= w (on and below the diagonal; what lies above is not used)
-__device__ __forceinline__ void decays(const float* gs, const float (&block)[4], int w, int j, int q, f32x4 (&out)[4]) {
-    f32x4 head = splat4(0.f), within = splat4(0.f);
+// sums of the chunk's g (lane = token) within its block of 16: up to and with the token, and after it
+__device__ __forceinline__ void block_scans(float g, float* head, float* tail) {
+    *head = dpp_add<0x118>(dpp_add<0x114>(dpp_add<0x112>(dpp_add<0x111>(g))));
+    const float next = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, g), 0x101, 0xf, 0xf, true));
+    *tail = dpp_add<0x108>(dpp_add<0x104>(dpp_add<0x102>(dpp_add<0x101>(next))));
+}
+// What a chunk's decays are made of, in LDS: g, the scans within blocks of 16.  Written by the 64 lanes of one wave.
+struct Decays {
+    float g[64], head[64], tail[64];
+    __device__ __forceinline__ void set(int lane, float x) {
+        g[lane] = x;
+        block_scans(x, &head[lane], &tail[lane]);
+    }
+    __device__ __forceinline__ float block(int b) const { return head[16 * b + 15]; }
+    // sums from the chunk's start up to and with token `lane`, and after it to the chunk's end
+    __device__ __forceinline__ void ends(int lane, float* from_start, float* to_end) const {
+        float a = head[lane], b = tail[lane];
 #pragma unroll
-    for (int m = 0; m < 16; ++m) {
-        const float gm = gs[16 * w + m];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            head[r] += m <= 4 * q + r ? gm : 0.f;
-            within[r] += (m > j && m <= 4 * q + r) ? gm : 0.f;
+        for (int m = 0; m < 4; ++m) {
+            const float x = block(m);
+            a += m < (lane >> 4) ? x : 0.f;
+            b += m > (lane >> 4) ? x : 0.f;
         }
+        *from_start = a;
+        *to_end = b;
     }
+    // e^{D_ij} of tile (mt, nt <= mt): rows i = 16 mt + 4 q + r, column 16 nt + j; what lies above the diagonal is not used
+    __device__ __forceinline__ f32x4 tile(int mt, int nt, int j, int q) const {
+        f32x4 d = splat4(0.f);
+        if (nt < mt) {
+            float t = tail[16 * nt + j];
+            if (nt + 1 < mt) t += block(nt + 1);
+            if (nt + 2 < mt) t += block(nt + 2);
+            d = *(const f32x4*)&head[16 * mt + 4 * q];
 #pragma unroll
-    for (int nt = 0; nt < 4; ++nt) {
-        if (nt > w) continue;
-        float tail = 0.f;
-        if (nt < w) {
+            for (int r = 0; r < 4; ++r) d[r] += t;
+        } else {
 #pragma unroll
-            for (int m = 0; m < 16; ++m) tail += m > j ? gs[16 * nt + m] : 0.f;
+            for (int m4 = 0; m4 < 4; ++m4) {
+                const f32x4 x = *(const f32x4*)&g[16 * mt + 4 * m4];
 #pragma unroll
-            for (int m = 0; m < 4; ++m) tail += (m > nt && m < w) ? block[m] : 0.f;
+                for (int m = 0; m < 4; ++m)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) d[r] += (4 * m4 + m > j && 4 * m4 + m <= 4 * q + r) ? x[m] : 0.f;
+            }
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) out[nt][r] = expf(nt < w ? tail + head[r] : within[r]);
+        for (int r = 0; r < 4; ++r) d[r] = exp_decay(d[r]);
+        return d;
     }
-}
-// the same of one tile (mt, nt)
-__device__ __forceinline__ f32x4 tile_decay(const float* gs, const float (&block)[4], int mt, int nt, int j, int q) {
-    f32x4 sum = splat4(0.f);
-    float tail = 0.f;
-    if (nt < mt) {
-#pragma unroll
-        for (int m = 0; m < 16; ++m) tail += m > j ? gs[16 * nt + m] : 0.f;
-#pragma unroll
-        for (int m = 0; m < 4; ++m) tail += (m > nt && m < mt) ? block[m] : 0.f;
-    }
-    const int from = nt < mt ? -1 : j;
-#pragma unroll
-    for (int m = 0; m < 16; ++m) {
-        const float gm = gs[16 * mt + m];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sum[r] += (m > from && m <= 4 * q + r) ? gm : 0.f;
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) sum[r] = expf(tail + sum[r]);
-    return sum;
-}
+};
 
 constexpr int kTriStride = 68;    // floats per row of a 64 x 64 matrix in LDS: rows 16-byte aligned, four banks apart
 
@@ -259,7 +252,8 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a) {
     typedef typename In::raw raw;
     __shared__ bf16x8 kfr[4 * KS * NI * 64];
     __shared__ f32x4 amat4[64 * kTriStride / 4], pmat4[64 * kTriStride / 4], tmat4[64 * kTriStride / 4];
-    __shared__ float gs[64], bs[64];
+    __shared__ __attribute__((aligned(16))) Decays dec;
+    __shared__ float bs[64];
     float* const amat = (float*)amat4;
     float* const pmat = (float*)pmat4;
     float* const tmat = (float*)tmat4;
@@ -367,34 +361,33 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a) {
         transposed(a.qtf);
     }
 
+    const int lane0 = lane;
     for (int hv = h * a.group; hv < (h + 1) * a.group; ++hv) {
+        const int lane = in_block(lane0), j = lane & 15, q = lane >> 4;     // (nothing of a head's addresses is kept over the loop)
         __syncthreads();
         if (w == 0) {
             const bool in = lane < n;
-            gs[lane] = in ? a.g[(start + lane) * a.g_t + hv * a.g_h] : 0.f;
+            dec.set(lane, in ? a.g[(start + lane) * a.g_t + hv * a.g_h] : 0.f);
             bs[lane] = in ? a.beta[(start + lane) * a.b_t + hv * a.b_h] : 0.f;
         }
         __syncthreads();
-        float block[4];
-        block_sums(gs, block);
         if (w == 0) {
-            float head, tail;
-            head_tail(gs, block, lane, &head, &tail);
+            float from_start, to_end;
+            dec.ends(lane, &from_start, &to_end);
             float* sc = a.sc + (size_t)(slot * (size_t)a.hv + hv) * 256;
             sc[lane] = bs[lane];
-            sc[64 + lane] = expf(head);
-            sc[128 + lane] = expf(tail);
+            sc[64 + lane] = exp_decay(from_start);
+            sc[128 + lane] = exp_decay(to_end);
         }
-        f32x4 decay[4];
-        decays(gs, block, w, j, q, decay);
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt) {
             if (nt > w) continue;
+            const f32x4 decay = dec.tile(w, nt, j, q);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = 16 * w + 4 * q + r, col = 16 * nt + j;
-                amat[i * kTriStride + col] = col < i ? beta_of(bs[col]) * (kk[nt][r] * decay[nt][r]) : 0.f;
-                pmat[i * kTriStride + col] = col <= i ? qk[nt][r] * decay[nt][r] : 0.f;
+                amat[i * kTriStride + col] = col < i ? beta_of(bs[col]) * (kk[nt][r] * decay[r]) : 0.f;
+                pmat[i * kTriStride + col] = col <= i ? qk[nt][r] * decay[r] : 0.f;
             }
         }
         __syncthreads();

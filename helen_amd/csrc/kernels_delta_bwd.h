@@ -225,11 +225,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
     }
 }
 
-// sum over the 16 lanes of a quarter (rotations within a row of 16 lanes, on the VALU), over a wave, and running sums
-template <int CTRL>
-__device__ __forceinline__ float dpp_add(float x) {
-    return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
-}
+// sum over the 16 lanes of a quarter, over a wave, and running sums
 __device__ __forceinline__ float sum16(float x) { return dpp_add<0x121>(dpp_add<0x122>(dpp_add<0x124>(dpp_add<0x128>(x)))); }
 __device__ __forceinline__ float sum64(float x) {
     x = sum16(x);
@@ -270,7 +266,8 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
     constexpr int kStage = 4 * (6 + NI);
     __shared__ bf16x8 stage[2 * kStage * 64];
     __shared__ bf16x8 fr[3 * (8 + 2 * kTriFrags) * 64];
-    __shared__ float gs[64], bs[64], scl[192], sums[2][NP][64], dbeta[64], gamma[NP], part[W][64];
+    __shared__ __attribute__((aligned(16))) Decays dec;
+    __shared__ float bs[64], scl[192], sums[2][NP][64], dbeta[64], gamma[NP], part[W][64];
     static_assert(sizeof(stage) >= 3 * 64 * kTriStride * 4, "the 64 x 64 gradients take the stage's place");
     float* const gmat = (float*)stage;
     float* const hmat = gmat + 64 * kTriStride;
@@ -318,13 +315,15 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
             for (int m = 0; m < 2; ++m) dQ[i][m] = dK[i][m] = splat4(0.f);
     }
     const bool has_z = W == 4 || w < 4;     // who stages Z and dO, and who E, of token tile w & 3
-    const int srow = 16 * (w & 3) + j;
+    const int lane0 = lane;
     for (int hv = h * a.group; hv < (h + 1) * a.group; ++hv) {
+        const int lane = in_block(lane0), j = lane & 15, q = lane >> 4;     // (nothing of a head's addresses is kept over the loop)
+        const int srow = 16 * (w & 3) + j;
         const size_t vslot = (size_t)slot * a.hv + hv;
         __syncthreads();
         if (w == 0) {
             const bool in = lane < n;
-            gs[lane] = in ? a.g[(start + lane) * a.g_t + hv * a.g_h] : 0.f;
+            dec.set(lane, in ? a.g[(start + lane) * a.g_t + hv * a.g_h] : 0.f);
             bs[lane] = in ? a.beta[(start + lane) * a.b_t + hv * a.b_h] : 0.f;
         } else if (w < 4) {
             scl[threadIdx.x - 64] = a.sc[vslot * 256 + threadIdx.x - 64];
@@ -456,12 +455,10 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
         // the 64 x 64 gradients, in the stage's place
         __syncthreads();
         {
-            float block[4];
-            block_sums(gs, block);
 #pragma unroll
             for (int t = 0; t < TPW; ++t) {
                 if (!own[t]) continue;
-                const f32x4 decay = tile_decay(gs, block, tm[t], tn[t], j, q);
+                const f32x4 decay = dec.tile(tm[t], tn[t], j, q);
                 const int col = 16 * tn[t] + j;
                 const float beta = bs[col], beta1 = beta_of(beta);
 #pragma unroll
