@@ -116,12 +116,14 @@ struct DeltaArgs {
     long q_t, q_h, k_t, k_h, v_t, v_h, o_t, o_h, do_t, do_h, g_t, g_h, b_t, b_h;   // strides in elements: token, head
     int tokens, nseq, seq_len, hk, hv, group, dv_width, slots;
     float scale;
+    void* sink;                 // where rows behind a sequence's end are stored
+    bf16x8* zeros;              // three fragments of zeros: the k step of a triangle's row tile that lies above the diagonal
     int zero_tail;              // rows behind the last sequence: 1 = zero them, 0 = leave them
     // workspace: fragments per (slot, key head) and per (slot, value head)
     bf16x8 *kf, *ktf, *qf, *qtf;
     bf16x8 *tf, *ttf, *pf, *ptf;
     f32x4* dots;                // kept: [slot, hk][10 tiles][K K^T | Q K^T][lane]
-    float* sc;                  // [slot, hv][4][64]: beta, e^b, e^c, -
+    float* sc;                  // [slot, hv][4][64]: beta, e^b, e^c, e^{b_C} in every place
     float *states, *e;          // kept for the backward pass: [slot, hv, Dk, Dv], [slot, hv, 64, Dv]
     float *dstates, *z;         // backward: [slot, hv, Dk, Dv], [slot, hv, 64, Dv]
 };
@@ -260,6 +262,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a) {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int j = lane & 15, q = lane >> 4;
     const int slot = blockIdx.x / a.hk, h = blockIdx.x % a.hk;
+    if (blockIdx.x == 0 && threadIdx.x < 192) ((u32x4*)a.zeros)[threadIdx.x] = (u32x4){0, 0, 0, 0};
     const int s = sequence_of(a, slot, lane);
     const Span sp = span_of(a, s);
     const int c = slot - sp.slot;
@@ -378,6 +381,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a) {
             sc[lane] = bs[lane];
             sc[64 + lane] = exp_decay(from_start);
             sc[128 + lane] = exp_decay(to_end);
+            sc[192 + lane] = exp_decay((dec.block(0) + dec.block(1)) + (dec.block(2) + dec.block(3)));
         }
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt) {
@@ -514,9 +518,28 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
+// loads stay above this (they are issued here, and not where their values are first needed)
+__device__ __forceinline__ void issue_loads() { asm volatile("" ::: "memory"); }
 // workgroups go round the eight XCDs: neighbours in `logical` order (the column groups of one head, which read the same
 // fragments) stay on one of them.  The grid is padded to a multiple of eight.
 __device__ __forceinline__ unsigned xcd_order(unsigned block, unsigned grid) { return (block & 7) * (grid >> 3) + (block >> 3); }
+
+// A wave's rows of a state [DK, dv]: MW row tiles, 16 rows of stride `dv` apart; zero where there is no state.  The loads are not
+// conditional (they read some zeros then): behind a skipped load the compiler waits for everything that is in flight.
+template <int MW, int NC>
+__device__ __forceinline__ void load_state(const float* state, const void* zeros, size_t at, int dv, f32x4 (&S)[MW][NC]) {
+    const float* const from = state ? state + at : (const float*)zeros;
+    const size_t stride = state ? dv : 0;
+#pragma unroll
+    for (int i = 0; i < MW; ++i)
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float x = from[(16 * i + r) * stride + 16 * nc];
+                S[i][nc][r] = state ? x : 0.f;
+            }
+}
 
 // ------------------------------------------------------------------------------------------------
 // The chain: a workgroup per (sequence, value head, 16 NC columns of the state).  Each of its four waves owns a quarter of
@@ -541,59 +564,57 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
     const size_t st = (((size_t)s * a.hv + hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col;
 
     f32x4 S[MW][NC];
-#pragma unroll
-    for (int i = 0; i < MW; ++i)
-#pragma unroll
-        for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) S[i][nc][r] = a.s0 ? a.s0[st + (size_t)(16 * i + r) * a.dv_width + 16 * nc] : 0.f;
+    load_state<MW, NC>(a.s0, a.zeros, st, a.dv_width, S);
 
     bf16x8 kf[KS][NI], qf[KS][NI], kt[MW][2][NI], tf[2][3], pf[2][PT];
-    f32x4 beta, eb, ec;
-    float whole;
+    f32x4 beta, eb, ec, whole;
     raw v[NC][4];
     const bf16x8* const kf0 = a.kf + (size_t)sp.slot * a.hk * (DK / 8 * NI * 64) + (size_t)h * (DK / 8 * NI * 64) + lane;
     const bf16x8* const qf0 = a.qf + (kf0 - a.kf);
     const bf16x8* const kt0 = a.ktf + (kf0 - a.kf);
     const size_t vslot0 = (size_t)sp.slot * a.hv + hv;
     const int row = 16 * w + 4 * q;                 // this lane's tokens: row .. row + 3
-    auto load_rows = [&](int c) {
+    const auto load_rows = [&](const bf16x8* from, int c, bf16x8 (&to)[KS][NI]) {
         const size_t at = (size_t)c * a.hk * (DK / 8 * NI * 64) + w * KS * NI * 64;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-            for (int t = 0; t < NI; ++t) {
-                kf[ks][t] = kf0[at + (ks * NI + t) * 64];
-                qf[ks][t] = qf0[at + (ks * NI + t) * 64];
-            }
+            for (int t = 0; t < NI; ++t) to[ks][t] = from[at + (ks * NI + t) * 64];
     };
+    auto load_k = [&](int c) { load_rows(kf0, c, kf); };
+    auto load_q = [&](int c) { load_rows(qf0, c, qf); };
+    // (No load or store of the loop is conditional: the compiler counts what is in flight, and a skipped access would make it
+    // wait for everything.  Rows behind the sequence's end read its last row and are stored to the sink.)
     auto load_tokens = [&](int c) {
         const float* sc = a.sc + (vslot0 + (size_t)c * a.hv) * 256;
         beta = *(const f32x4*)(sc + row);
         eb = *(const f32x4*)(sc + 64 + row);
         ec = *(const f32x4*)(sc + 128 + row);
-        whole = sc[64 + 63];
-        const int n = sp.len - c * kDeltaChunk;
-        const raw* p = (const raw*)a.v + (sp.begin + c * kDeltaChunk + row) * a.v_t + hv * a.v_h + col;
+        whole = *(const f32x4*)(sc + 192 + row);
+        const int last = sp.len - 1;
+        const raw* p = (const raw*)a.v + sp.begin * a.v_t + hv * a.v_h + col;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int nc = 0; nc < NC; ++nc) v[nc][r] = row + r < n ? p[r * a.v_t + 16 * nc] : raw(0);
+            for (int nc = 0; nc < NC; ++nc) v[nc][r] = p[min(c * kDeltaChunk + row + r, last) * a.v_t + 16 * nc];
     };
+    // token tiles 0 and 1 have one k step of T and P, the other one is zeros
     auto load_t = [&](int c) {
-        const size_t at = ((vslot0 + (size_t)c * a.hv) * kTriFrags + tri_index(w, 0)) * 3 * 64 + lane;
+        const bf16x8* const at = a.tf + ((vslot0 + (size_t)c * a.hv) * kTriFrags + tri_index(w, 0)) * 3 * 64;
+        const bf16x8* const at1 = w < 2 ? a.zeros : at + 3 * 64;
 #pragma unroll
         for (int t = 0; t < 3; ++t) {
-            tf[0][t] = a.tf[at + t * 64];
-            if (w >= 2) tf[1][t] = a.tf[at + (3 + t) * 64];
+            tf[0][t] = at[t * 64 + lane];
+            tf[1][t] = at1[t * 64 + lane];
         }
     };
     auto load_p = [&](int c) {
-        const size_t at = ((vslot0 + (size_t)c * a.hv) * kTriFrags + tri_index(w, 0)) * PT * 64 + lane;
+        const bf16x8* const at = a.pf + ((vslot0 + (size_t)c * a.hv) * kTriFrags + tri_index(w, 0)) * PT * 64;
+        const bf16x8* const at1 = w < 2 ? a.zeros : at + PT * 64;
 #pragma unroll
         for (int t = 0; t < PT; ++t) {
-            pf[0][t] = a.pf[at + t * 64];
-            if (w >= 2) pf[1][t] = a.pf[at + (PT + t) * 64];
+            pf[0][t] = at[t * 64 + lane];
+            pf[1][t] = at1[t * 64 + lane];
         }
     };
     auto load_kt = [&](int c) {
@@ -628,8 +649,9 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
         }
     };
     if (chunks > 0) {
-        load_rows(0);
+        load_k(0);
         load_tokens(0);
+        load_q(0);
         load_t(0);
         load_p(0);
         load_kt(0);
@@ -637,46 +659,55 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
     }
     lds_barrier();
     for (int c = 0; c < chunks; ++c) {
-        const bool more = c + 1 < chunks;
-        f32x4 R[NC], O[NC], U[NC];
+        const int next = min(c + 1, chunks - 1), n = sp.len - c * kDeltaChunk;
+        // Two sums each where there is one column tile: a product waits for the one before it in the same sum
+        constexpr int NS = NC == 1 ? 2 : 1;
+        f32x4 R[NC], O[NC], U[NC], sums[NS][NC], osum[NS][NC];
+        bf16x8 b[KS][NC][3];
 #pragma unroll
-        for (int nc = 0; nc < NC; ++nc) R[nc] = O[nc] = U[nc] = splat4(0.f);
+        for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+            for (int k = 0; k < NS; ++k) sums[k][nc] = osum[k][nc] = splat4(0.f);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc) {
-                bf16x8 b[3];
-                shared_frag<3, NC>(sbuf, ks, nc, lane, b);
-                R[nc] = mm(kf[ks], b, R[nc]);
-                O[nc] = mm(qf[ks], b, O[nc]);
+                shared_frag<3, NC>(sbuf, ks, nc, lane, b[ks][nc]);
+                sums[ks % NS][nc] = mm(kf[ks], b[ks][nc], sums[ks % NS][nc]);
+                if constexpr (NC > 1) osum[0][nc] = mm(qf[ks], b[ks][nc], osum[0][nc]);
             }
-        const f32x4 after = ec, step = beta;
-        const float hold = whole;
+        const f32x4 after = ec, step = beta, head = eb;
+        const f32x4 hold = whole;
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                R[nc][r] = In::to_f32(v[nc][r]) - eb[r] * R[nc][r];
-                O[nc][r] *= eb[r];
+                const float x = NS == 2 ? sums[0][nc][r] + sums[NS - 1][nc][r] : sums[0][nc][r];
+                R[nc][r] = (row + r < n ? In::to_f32(v[nc][r]) : 0.f) - eb[r] * x;
             }
             share_tile<3, NC>(xbuf, w, nc, lane, R[nc]);
         }
-        if (more) {
-            load_rows(c + 1);
-            load_tokens(c + 1);
-        }
+        load_k(next);
+        load_tokens(next);
+        issue_loads();
         lds_barrier();
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
-            bf16x8 b[3];
-            shared_frag<3, NC>(xbuf, 0, nc, lane, b);
-            U[nc] = mm(tf[0], b, U[nc]);
-            if (w >= 2) {
-                shared_frag<3, NC>(xbuf, 1, nc, lane, b);
-                U[nc] = mm(tf[1], b, U[nc]);
-            }
+            bf16x8 x[2][3];
+            shared_frag<3, NC>(xbuf, 0, nc, lane, x[0]);
+            shared_frag<3, NC>(xbuf, 1, nc, lane, x[1]);
+            f32x4 u0 = splat4(0.f), u1 = splat4(0.f);
+            u0 = mm(tf[0], x[0], u0);
+            u1 = mm(tf[1], x[1], u1);
+            U[nc] = u0 + u1;
         }
-        if (more) load_t(c + 1);
+        // one column tile: Q S0 fills the wait for U
+        if constexpr (NC == 1) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) osum[ks % NS][0] = mm(qf[ks], b[ks][0], osum[ks % NS][0]);
+        }
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) O[nc] = NS == 2 ? osum[0][nc] + osum[NS - 1][nc] : osum[0][nc];
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
             if constexpr (KEEP) {
@@ -691,45 +722,50 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
             for (int r = 0; r < 4; ++r) U[nc][r] *= after[r];
             share_tile<3, NC>(cbuf, w, nc, lane, U[nc]);
         }
+        load_q(next);
+        load_t(next);
+        issue_loads();
         lds_barrier();
 #pragma unroll
         for (int i = 0; i < MW; ++i)
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) S[i][nc][r] *= hold;
+                for (int r = 0; r < 4; ++r) S[i][nc][r] *= hold[r];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc) {
-                bf16x8 b[3];
-                shared_frag<3, NC>(cbuf, ks, nc, lane, b);
+                bf16x8 x[3];
+                shared_frag<3, NC>(cbuf, ks, nc, lane, x);
 #pragma unroll
-                for (int i = 0; i < MW; ++i) S[i][nc] = mm(kt[i][ks], b, S[i][nc]);
+                for (int i = 0; i < MW; ++i) S[i][nc] = mm(kt[i][ks], x, S[i][nc]);
             }
+        bf16x8 x[2][NC][PT];
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
-            bf16x8 b[PT];
-            shared_frag<PT, NC>(ubuf, 0, nc, lane, b);
-            O[nc] = mm<PT, PT, PT - 1>(pf[0], b, O[nc]);
-            if (w >= 2) {
-                shared_frag<PT, NC>(ubuf, 1, nc, lane, b);
-                O[nc] = mm<PT, PT, PT - 1>(pf[1], b, O[nc]);
-            }
+            shared_frag<PT, NC>(ubuf, 0, nc, lane, x[0][nc]);
+            shared_frag<PT, NC>(ubuf, 1, nc, lane, x[1][nc]);
         }
-        if (more) {
-            share_state(c + 1);
-            load_kt(c + 1);
-            load_p(c + 1);
+        load_kt(next);
+        issue_loads();
+        if (c + 1 < chunks) share_state(next);
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+            f32x4 p0 = splat4(0.f);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) O[nc][r] *= head[r];
+            p0 = mm<PT, PT, PT - 1>(pf[0], x[0][nc], p0);
+            O[nc] = mm<PT, PT, PT - 1>(pf[1], x[1][nc], O[nc]) + p0;
         }
-        if (a.o) {
-            const int n = sp.len - c * kDeltaChunk;
-            raw* to = (raw*)a.o + (sp.begin + c * kDeltaChunk + row) * a.o_t + hv * a.o_h + col;
+        load_p(next);
+        issue_loads();
+        raw* const to = (raw*)a.o + (sp.begin + c * kDeltaChunk) * a.o_t + hv * a.o_h + col;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r) {
+            raw* const at = row + r < n ? to + (row + r) * a.o_t : (raw*)a.sink + col;
 #pragma unroll
-                for (int nc = 0; nc < NC; ++nc)
-                    if (row + r < n) to[r * a.o_t + 16 * nc] = In::from_f32(a.scale * O[nc][r]);
+            for (int nc = 0; nc < NC; ++nc) at[16 * nc] = In::from_f32(a.scale * O[nc][r]);
         }
         lds_barrier();
     }

@@ -32,16 +32,10 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
     const size_t st = (((size_t)s * a.hv + hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col;
 
     f32x4 S[MW][NC];
-#pragma unroll
-    for (int i = 0; i < MW; ++i)
-#pragma unroll
-        for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) S[i][nc][r] = a.ds1 ? a.ds1[st + (size_t)(16 * i + r) * a.dv_width + 16 * nc] : 0.f;
+    load_state<MW, NC>(a.ds1, a.zeros, st, a.dv_width, S);
 
     bf16x8 kf[KS][NI], kt[MW][2][NI], qt[MW][2][NI], tt[2][3], pt[2][3];
-    f32x4 beta, eb, ec;
-    float whole;
+    f32x4 beta, eb, ec, whole;
     raw y[NC][4];
     const bf16x8* const kf0 = a.kf + (size_t)sp.slot * a.hk * (DK / 8 * NI * 64) + (size_t)h * (DK / 8 * NI * 64) + lane;
     const bf16x8* const kt0 = a.ktf + (kf0 - a.kf);
@@ -60,22 +54,29 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
         beta = *(const f32x4*)(sc + row);
         eb = *(const f32x4*)(sc + 64 + row);
         ec = *(const f32x4*)(sc + 128 + row);
-        whole = sc[64 + 63];
+        whole = *(const f32x4*)(sc + 192 + row);
     };
+    // (no conditional loads or stores: see delta_forward_kernel)
     auto load_dout = [&](int c) {
-        const int n = sp.len - c * kDeltaChunk;
-        const raw* p = (const raw*)a.dout + (sp.begin + c * kDeltaChunk + row) * a.do_t + hv * a.do_h + col;
+        const int last = sp.len - 1;
+        const raw* p = (const raw*)a.dout + sp.begin * a.do_t + hv * a.do_h + col;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int nc = 0; nc < NC; ++nc) y[nc][r] = row + r < n ? p[r * a.do_t + 16 * nc] : raw(0);
+            for (int nc = 0; nc < NC; ++nc) {
+                const int t = c * kDeltaChunk + row + r;
+                y[nc][r] = p[min(t, last) * a.do_t + 16 * nc];
+            }
     };
+    auto dout = [&](int c, int nc, int r) { return c * kDeltaChunk + row + r < sp.len ? In::to_f32(y[nc][r]) : 0.f; };
+    // token tiles 2 and 3 have only the second k step of T^T and P^T
     auto load_tri = [&](int c, const bf16x8* from, bf16x8 (&to)[2][3]) {
-        const size_t at = (vslot0 + (size_t)c * a.hv) * kTriFrags * 3 * 64 + lane;
+        const bf16x8* const at = from + ((vslot0 + (size_t)c * a.hv) * kTriFrags + trt_index(w, 1)) * 3 * 64;
+        const bf16x8* const at0 = w < 2 ? at - 3 * 64 : a.zeros;
 #pragma unroll
         for (int t = 0; t < 3; ++t) {
-            if (w < 2) to[0][t] = from[at + (trt_index(w, 0) * 3 + t) * 64];
-            to[1][t] = from[at + (trt_index(w, 1) * 3 + t) * 64];
+            to[0][t] = at0[t * 64 + lane];
+            to[1][t] = at[t * 64 + lane];
         }
     };
     auto load_columns = [&](int c) {
@@ -103,7 +104,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
                 share_tile<3, NC>(sbuf, w, nc, lane, S[0][nc]);
             }
             share_tile<NI, NC>(ybuf, w, nc, lane,
-                               (f32x4){In::to_f32(y[nc][0]), In::to_f32(y[nc][1]), In::to_f32(y[nc][2]), In::to_f32(y[nc][3])});
+                               (f32x4){dout(c, nc, 0), dout(c, nc, 1), dout(c, nc, 2), dout(c, nc, 3)});
         }
         float* to = a.dstates + ((vslot0 + (size_t)c * a.hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col;
 #pragma unroll
@@ -125,77 +126,80 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
     }
     lds_barrier();
     for (int c = chunks - 1; c >= 0; --c) {
-        f32x4 E[NC], P[NC];
+        const int next = max(c - 1, 0), n = sp.len - c * kDeltaChunk;
+        constexpr int NS = NC == 1 ? 2 : 1;
+        f32x4 E[NS][NC], P[2][NC];
 #pragma unroll
-        for (int nc = 0; nc < NC; ++nc) E[nc] = P[nc] = splat4(0.f);
+        for (int nc = 0; nc < NC; ++nc) {
+            P[0][nc] = P[1][nc] = splat4(0.f);
+#pragma unroll
+            for (int k = 0; k < NS; ++k) E[k][nc] = splat4(0.f);
+        }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc) {
                 bf16x8 b[3];
                 shared_frag<3, NC>(sbuf, ks, nc, lane, b);
-                E[nc] = mm(kf[ks], b, E[nc]);
+                E[ks % NS][nc] = mm(kf[ks], b, E[ks % NS][nc]);
             }
 #pragma unroll
-        for (int nc = 0; nc < NC; ++nc) {
-            bf16x8 b[NI];
-            if (w < 2) {
-                shared_frag<NI, NC>(ybuf, 0, nc, lane, b);
-                P[nc] = mm(pt[0], b, P[nc]);
+        for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                bf16x8 b[NI];
+                shared_frag<NI, NC>(ybuf, ks, nc, lane, b);
+                P[ks][nc] = mm(pt[ks], b, P[ks][nc]);
             }
-            shared_frag<NI, NC>(ybuf, 1, nc, lane, b);
-            P[nc] = mm(pt[1], b, P[nc]);
-        }
         const f32x4 head = eb;
-        const float hold = whole;
+        const f32x4 hold = whole;
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
             f32x4 x;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                E[nc][r] = beta_of(beta[r]) * (ec[r] * E[nc][r] + a.scale * P[nc][r]);
-                x[r] = a.scale * eb[r] * In::to_f32(y[nc][r]);
+                const float e = NS == 2 ? E[0][nc][r] + E[NS - 1][nc][r] : E[0][nc][r];
+                E[0][nc][r] = beta_of(beta[r]) * (ec[r] * e + a.scale * (P[0][nc][r] + P[1][nc][r]));
+                x[r] = a.scale * eb[r] * dout(c, nc, r);
             }
-            share_tile<3, NC>(dbuf, w, nc, lane, E[nc]);
+            share_tile<3, NC>(dbuf, w, nc, lane, E[0][nc]);
             share_tile<3, NC>(wbuf, w, nc, lane, x);
         }
-        if (c > 0) {
-            load_dout(c - 1);
-            load_rows(c - 1);
-            load_scales(c - 1);
-            load_tri(c - 1, a.ptf, pt);
-        }
+        load_rows(next);
+        load_scales(next);
+        load_dout(next);
+        load_tri(next, a.ptf, pt);
+        issue_loads();
         lds_barrier();
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
-            f32x4 Z = splat4(0.f);
-            bf16x8 b[3];
-            if (w < 2) {
-                shared_frag<3, NC>(dbuf, 0, nc, lane, b);
-                Z = mm(tt[0], b, Z);
-            }
-            shared_frag<3, NC>(dbuf, 1, nc, lane, b);
-            Z = mm(tt[1], b, Z);
-            const int n = sp.len - c * kDeltaChunk;
+            f32x4 z0 = splat4(0.f), z1 = splat4(0.f);
+            bf16x8 b[2][3];
+            shared_frag<3, NC>(dbuf, 0, nc, lane, b[0]);
+            shared_frag<3, NC>(dbuf, 1, nc, lane, b[1]);
+            z0 = mm(tt[0], b[0], z0);
+            z1 = mm(tt[1], b[1], z1);
+            const f32x4 Z = z0 + z1;
             float* to = a.z + ((vslot0 + (size_t)c * a.hv) * kDeltaChunk + row) * a.dv_width + col + 16 * nc;
             raw* dv = (raw*)a.dv + ((size_t)(sp.begin + c * kDeltaChunk + row) * a.hv + hv) * a.dv_width + col + 16 * nc;
             f32x4 x;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 to[r * a.dv_width] = Z[r];
-                if (row + r < n) dv[(size_t)r * a.hv * a.dv_width] = In::from_f32(Z[r]);
+                *(row + r < n ? dv + (size_t)r * a.hv * a.dv_width : (raw*)a.sink + col) = In::from_f32(Z[r]);
                 x[r] = -head[r] * Z[r];
             }
             share_tile<3, NC>(zbuf, w, nc, lane, x);
         }
-        if (c > 0) load_tri(c - 1, a.ttf, tt);
+        load_tri(next, a.ttf, tt);
+        issue_loads();
         lds_barrier();
 #pragma unroll
         for (int i = 0; i < MW; ++i)
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) S[i][nc][r] *= hold;
+                for (int r = 0; r < 4; ++r) S[i][nc][r] *= hold[r];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -209,10 +213,9 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
                     S[i][nc] = mm(qt[i][ks], e, S[i][nc]);
                 }
             }
-        if (c > 0) {
-            load_columns(c - 1);
-            share(c - 1);
-        }
+        load_columns(next);
+        issue_loads();
+        if (c > 0) share(next);
         lds_barrier();
     }
     if (a.ds0) {

@@ -23,6 +23,8 @@ size_t carve(const HelenDeltaRule& op, int keep, void* base, DeltaArgs* a) {
     const int ni = op.dtype == HELEN_TYPE_BF16 ? 1 : (op.dtype == HELEN_TYPE_FP16 ? 2 : 3);
     const int pt = op.dtype == HELEN_TYPE_FP32 ? 3 : 2;
     const size_t rows = ks * (op.width_k / 8) * ni * 64, tri = vs * kTriFrags * 64;
+    a->sink = c.take<float>(256);
+    a->zeros = c.take<bf16x8>(3 * 64);
     a->kf = c.take<bf16x8>(rows);
     a->ktf = c.take<bf16x8>(rows);
     a->qf = c.take<bf16x8>(rows);
@@ -135,6 +137,10 @@ int helen_delta_rule_forward(const HelenDeltaRule* op, int keep, void* workspace
     const size_t need = carve(*op, keep != 0, workspace, &a);
     if (workspace_bytes < need || !workspace || (uintptr_t)workspace % 256)
         return fail(HELEN_EINVAL, "delta rule: workspace of %zu bytes, %zu are needed, 256-byte aligned", workspace_bytes, need);
+    if (!a.o) {          // the chain stores its rows all the same: into the sink
+        a.o = a.sink;
+        a.o_t = a.o_h = a.zero_tail = 0;
+    }
     OnDevice on(op->device);
     if (on.status() != hipSuccess) return fail(HELEN_ENODEV, "delta rule: device %d: %s", op->device, hipGetErrorString(on.status()));
     hipStream_t s = (hipStream_t)stream;
