@@ -524,6 +524,74 @@ __device__ __forceinline__ void issue_loads() { asm volatile("" ::: "memory"); }
 // fragments) stay on one of them.  The grid is padded to a multiple of eight.
 __device__ __forceinline__ unsigned xcd_order(unsigned block, unsigned grid) { return (block & 7) * (grid >> 3) + (block >> 3); }
 
+// Where a wave of a chain finds its left-hand fragments: uniform bases plus the lane
+template <typename In, int DK>
+struct ChainAddress {
+    static constexpr int NI = In::kTerms, kSlot = DK / 8 * NI * 64;    // fragments of a (slot, key head), times 64 lanes
+    const bf16x8* zeros;
+    size_t kslot, vslot;
+    int hk, hv, w;
+    unsigned lane;
+    __device__ __forceinline__ ChainAddress(const DeltaArgs& a, const Span& sp, int h, int head, int wave, int l)
+        : zeros(a.zeros), kslot((size_t)sp.slot * a.hk + h), vslot((size_t)sp.slot * a.hv + head), hk(a.hk), hv(a.hv), w(wave), lane(l) {}
+    // row tile w of K or Q
+    __device__ __forceinline__ void rows(const bf16x8* from, int c, bf16x8 (&to)[DK / 32][NI]) const {
+        from += (kslot + (size_t)c * hk) * kSlot + w * (DK / 32) * NI * 64;
+#pragma unroll
+        for (int ks = 0; ks < DK / 32; ++ks)
+#pragma unroll
+            for (int t = 0; t < NI; ++t) to[ks][t] = (from + (ks * NI + t) * 64)[lane];
+    }
+    // the wave's dk tiles of K^T or Q^T
+    __device__ __forceinline__ void columns(const bf16x8* from, int c, bf16x8 (&to)[DK / 64][2][NI]) const {
+        from += (kslot + (size_t)c * hk) * kSlot + w * (DK / 64) * 2 * NI * 64;
+#pragma unroll
+        for (int i = 0; i < DK / 64; ++i)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int t = 0; t < NI; ++t) to[i][ks][t] = (from + ((2 * i + ks) * NI + t) * 64)[lane];
+    }
+    // row tile w of T or P; row tiles 0 and 1 have one k step, their other one is zeros
+    template <int N>
+    __device__ __forceinline__ void triangle(const bf16x8* from, int c, bf16x8 (&to)[2][N]) const {
+        from += ((vslot + (size_t)c * hv) * kTriFrags + tri_index(w, 0)) * N * 64;
+        const bf16x8* const second = w < 2 ? zeros : from + N * 64;
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            to[0][t] = (from + t * 64)[lane];
+            to[1][t] = (second + t * 64)[lane];
+        }
+    }
+    // row tile w of T^T or P^T; row tiles 2 and 3 have only the second k step
+    __device__ __forceinline__ void transposed(const bf16x8* from, int c, bf16x8 (&to)[2][3]) const {
+        from += ((vslot + (size_t)c * hv) * kTriFrags + trt_index(w, 1)) * 3 * 64;
+        const bf16x8* const first = w < 2 ? from - 3 * 64 : zeros;
+#pragma unroll
+        for (int t = 0; t < 3; ++t) {
+            to[0][t] = (first + t * 64)[lane];
+            to[1][t] = (from + t * 64)[lane];
+        }
+    }
+};
+// Element offsets of a lane's four rows of a chunk in a [tokens, ..] tensor (the host has checked that they fit 32 bits); rows
+// from n on stand for row n - 1.
+struct RowOffsets {
+    unsigned at[4], stride;
+    int row, col, full;
+    __device__ __forceinline__ RowOffsets(long stride_, int row_, int col0, int j) : stride((unsigned)stride_), row(row_), col(col0 + j), full(1) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) at[r] = (row + r) * stride + col;
+    }
+    __device__ __forceinline__ void clamp(int n) {
+        if (n < kDeltaChunk || !full) {
+            full = n >= kDeltaChunk;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) at[r] = min(row + r, n - 1) * stride + col;
+        }
+    }
+};
+
 // A wave's rows of a state [DK, dv]: MW row tiles, 16 rows of stride `dv` apart; zero where there is no state.  The loads are not
 // conditional (they read some zeros then): behind a skipped load the compiler waits for everything that is in flight.
 template <int MW, int NC>
@@ -569,63 +637,32 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
     bf16x8 kf[KS][NI], qf[KS][NI], kt[MW][2][NI], tf[2][3], pf[2][PT];
     f32x4 beta, eb, ec, whole;
     raw v[NC][4];
-    const bf16x8* const kf0 = a.kf + (size_t)sp.slot * a.hk * (DK / 8 * NI * 64) + (size_t)h * (DK / 8 * NI * 64) + lane;
-    const bf16x8* const qf0 = a.qf + (kf0 - a.kf);
-    const bf16x8* const kt0 = a.ktf + (kf0 - a.kf);
-    const size_t vslot0 = (size_t)sp.slot * a.hv + hv;
     const int row = 16 * w + 4 * q;                 // this lane's tokens: row .. row + 3
-    const auto load_rows = [&](const bf16x8* from, int c, bf16x8 (&to)[KS][NI]) {
-        const size_t at = (size_t)c * a.hk * (DK / 8 * NI * 64) + w * KS * NI * 64;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int t = 0; t < NI; ++t) to[ks][t] = from[at + (ks * NI + t) * 64];
-    };
-    auto load_k = [&](int c) { load_rows(kf0, c, kf); };
-    auto load_q = [&](int c) { load_rows(qf0, c, qf); };
-    // (No load or store of the loop is conditional: the compiler counts what is in flight, and a skipped access would make it
-    // wait for everything.  Rows behind the sequence's end read its last row and are stored to the sink.)
+    const ChainAddress<In, DK> at(a, sp, h, hv, w, lane);
+    // (No load of the loop is conditional: the compiler counts what is in flight, and a skipped load would make it wait for
+    // everything.  Rows behind the sequence's end read its last row: their k and beta are zero.)
+    RowOffsets vrow(a.v_t, row, col - j, j), orow(a.o_t, row, col - j, j);
     auto load_tokens = [&](int c) {
-        const float* sc = a.sc + (vslot0 + (size_t)c * a.hv) * 256;
+        const float* sc = a.sc + (at.vslot + (size_t)c * a.hv) * 256;
         beta = *(const f32x4*)(sc + row);
         eb = *(const f32x4*)(sc + 64 + row);
         ec = *(const f32x4*)(sc + 128 + row);
         whole = *(const f32x4*)(sc + 192 + row);
-        const int last = sp.len - 1;
-        const raw* p = (const raw*)a.v + sp.begin * a.v_t + hv * a.v_h + col;
+        vrow.clamp(sp.len - c * kDeltaChunk);
+        const raw* p = (const raw*)a.v + (sp.begin + c * kDeltaChunk) * a.v_t + hv * a.v_h;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int nc = 0; nc < NC; ++nc) v[nc][r] = p[min(c * kDeltaChunk + row + r, last) * a.v_t + 16 * nc];
+            for (int nc = 0; nc < NC; ++nc) v[nc][r] = (p + 16 * nc)[vrow.at[r]];
     };
-    // token tiles 0 and 1 have one k step of T and P, the other one is zeros
-    auto load_t = [&](int c) {
-        const bf16x8* const at = a.tf + ((vslot0 + (size_t)c * a.hv) * kTriFrags + tri_index(w, 0)) * 3 * 64;
-        const bf16x8* const at1 = w < 2 ? a.zeros : at + 3 * 64;
+    auto load_k = [&](int c) { at.rows(a.kf, c, kf); };
+    auto load_q = [&](int c) { at.rows(a.qf, c, qf); };
+    auto load_kt = [&](int c) { at.columns(a.ktf, c, kt); };
+    auto load_t = [&](int c) { at.template triangle<3>(a.tf, c, tf); };
+    auto load_p = [&](int c) { at.template triangle<PT>(a.pf, c, pf); };
+    unsigned tile_at[4];                            // D tile of a [.., dv] matrix: this lane's four elements
 #pragma unroll
-        for (int t = 0; t < 3; ++t) {
-            tf[0][t] = at[t * 64 + lane];
-            tf[1][t] = at1[t * 64 + lane];
-        }
-    };
-    auto load_p = [&](int c) {
-        const bf16x8* const at = a.pf + ((vslot0 + (size_t)c * a.hv) * kTriFrags + tri_index(w, 0)) * PT * 64;
-        const bf16x8* const at1 = w < 2 ? a.zeros : at + PT * 64;
-#pragma unroll
-        for (int t = 0; t < PT; ++t) {
-            pf[0][t] = at[t * 64 + lane];
-            pf[1][t] = at1[t * 64 + lane];
-        }
-    };
-    auto load_kt = [&](int c) {
-        const size_t at = (size_t)c * a.hk * (DK / 8 * NI * 64) + w * MW * 2 * NI * 64;
-#pragma unroll
-        for (int i = 0; i < MW; ++i)
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                for (int t = 0; t < NI; ++t) kt[i][ks][t] = kt0[at + ((2 * i + ks) * NI + t) * 64];
-    };
+    for (int r = 0; r < 4; ++r) tile_at[r] = (4 * q + r) * a.dv_width + col;
     auto share_state = [&](int c) {
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
@@ -639,13 +676,13 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
             }
         }
         if constexpr (KEEP) {
-            float* to = a.states + ((vslot0 + (size_t)c * a.hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col;
+            float* to = a.states + ((at.vslot + (size_t)c * a.hv) * DK + 16 * MW * w) * a.dv_width;
 #pragma unroll
             for (int i = 0; i < MW; ++i)
 #pragma unroll
                 for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) to[(size_t)(16 * i + r) * a.dv_width + 16 * nc] = S[i][nc][r];
+                    for (int r = 0; r < 4; ++r) (to + (size_t)16 * i * a.dv_width + 16 * nc)[tile_at[r]] = S[i][nc][r];
         }
     };
     if (chunks > 0) {
@@ -683,7 +720,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float x = NS == 2 ? sums[0][nc][r] + sums[NS - 1][nc][r] : sums[0][nc][r];
-                R[nc][r] = (row + r < n ? In::to_f32(v[nc][r]) : 0.f) - eb[r] * x;
+                R[nc][r] = In::to_f32(v[nc][r]) - eb[r] * x;
             }
             share_tile<3, NC>(xbuf, w, nc, lane, R[nc]);
         }
@@ -711,9 +748,9 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
             if constexpr (KEEP) {
-                float* to = a.e + ((vslot0 + (size_t)c * a.hv) * kDeltaChunk + row) * a.dv_width + col + 16 * nc;
+                float* to = a.e + ((at.vslot + (size_t)c * a.hv) * kDeltaChunk + 16 * w) * a.dv_width + 16 * nc;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) to[r * a.dv_width] = U[nc][r];
+                for (int r = 0; r < 4; ++r) to[tile_at[r]] = U[nc][r];
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) U[nc][r] *= step[r];
@@ -760,13 +797,12 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
         }
         load_p(next);
         issue_loads();
-        raw* const to = (raw*)a.o + (sp.begin + c * kDeltaChunk) * a.o_t + hv * a.o_h + col;
+        raw* const to = (raw*)a.o + (sp.begin + c * kDeltaChunk) * a.o_t + hv * a.o_h;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            raw* const at = row + r < n ? to + (row + r) * a.o_t : (raw*)a.sink + col;
+        for (int r = 0; r < 4; ++r)
+            if (row + r < n)
 #pragma unroll
-            for (int nc = 0; nc < NC; ++nc) at[16 * nc] = In::from_f32(a.scale * O[nc][r]);
-        }
+                for (int nc = 0; nc < NC; ++nc) (to + 16 * nc)[orow.at[r]] = In::from_f32(a.scale * O[nc][r]);
         lds_barrier();
     }
     if (a.s1) {

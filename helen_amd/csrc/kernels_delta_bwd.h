@@ -37,60 +37,38 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
     bf16x8 kf[KS][NI], kt[MW][2][NI], qt[MW][2][NI], tt[2][3], pt[2][3];
     f32x4 beta, eb, ec, whole;
     raw y[NC][4];
-    const bf16x8* const kf0 = a.kf + (size_t)sp.slot * a.hk * (DK / 8 * NI * 64) + (size_t)h * (DK / 8 * NI * 64) + lane;
-    const bf16x8* const kt0 = a.ktf + (kf0 - a.kf);
-    const bf16x8* const qt0 = a.qtf + (kf0 - a.kf);
-    const size_t vslot0 = (size_t)sp.slot * a.hv + hv;
     const int row = 16 * w + 4 * q;
-    auto load_rows = [&](int c) {
-        const size_t at = (size_t)c * a.hk * (DK / 8 * NI * 64) + w * KS * NI * 64;
+    const ChainAddress<In, DK> at(a, sp, h, hv, w, lane);
+    RowOffsets yrow(a.do_t, row, col - j, j);
+    unsigned tile_at[4], dv_at[4];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int t = 0; t < NI; ++t) kf[ks][t] = kf0[at + (ks * NI + t) * 64];
+    for (int r = 0; r < 4; ++r) {
+        tile_at[r] = (4 * q + r) * a.dv_width + col;
+        dv_at[r] = (row + r) * a.hv * a.dv_width + col;
+    }
+    auto load_rows = [&](int c) { at.rows(a.kf, c, kf); };
+    auto load_columns = [&](int c) {
+        at.columns(a.ktf, c, kt);
+        at.columns(a.qtf, c, qt);
     };
+    auto load_tri = [&](int c, const bf16x8* from, bf16x8 (&to)[2][3]) { at.transposed(from, c, to); };
     auto load_scales = [&](int c) {
-        const float* sc = a.sc + (vslot0 + (size_t)c * a.hv) * 256;
+        const float* sc = a.sc + (at.vslot + (size_t)c * a.hv) * 256;
         beta = *(const f32x4*)(sc + row);
         eb = *(const f32x4*)(sc + 64 + row);
         ec = *(const f32x4*)(sc + 128 + row);
         whole = *(const f32x4*)(sc + 192 + row);
     };
-    // (no conditional loads or stores: see delta_forward_kernel)
+    // (no conditional loads, see delta_forward_kernel; rows behind the end meet q = k = 0)
     auto load_dout = [&](int c) {
-        const int last = sp.len - 1;
-        const raw* p = (const raw*)a.dout + sp.begin * a.do_t + hv * a.do_h + col;
+        yrow.clamp(sp.len - c * kDeltaChunk);
+        const raw* p = (const raw*)a.dout + (sp.begin + c * kDeltaChunk) * a.do_t + hv * a.do_h;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int nc = 0; nc < NC; ++nc) {
-                const int t = c * kDeltaChunk + row + r;
-                y[nc][r] = p[min(t, last) * a.do_t + 16 * nc];
-            }
+            for (int nc = 0; nc < NC; ++nc) y[nc][r] = (p + 16 * nc)[yrow.at[r]];
     };
-    auto dout = [&](int c, int nc, int r) { return c * kDeltaChunk + row + r < sp.len ? In::to_f32(y[nc][r]) : 0.f; };
-    // token tiles 2 and 3 have only the second k step of T^T and P^T
-    auto load_tri = [&](int c, const bf16x8* from, bf16x8 (&to)[2][3]) {
-        const bf16x8* const at = from + ((vslot0 + (size_t)c * a.hv) * kTriFrags + trt_index(w, 1)) * 3 * 64;
-        const bf16x8* const at0 = w < 2 ? at - 3 * 64 : a.zeros;
-#pragma unroll
-        for (int t = 0; t < 3; ++t) {
-            to[0][t] = at0[t * 64 + lane];
-            to[1][t] = at[t * 64 + lane];
-        }
-    };
-    auto load_columns = [&](int c) {
-        const size_t at = (size_t)c * a.hk * (DK / 8 * NI * 64) + w * MW * 2 * NI * 64;
-#pragma unroll
-        for (int i = 0; i < MW; ++i)
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                for (int t = 0; t < NI; ++t) {
-                    kt[i][ks][t] = kt0[at + ((2 * i + ks) * NI + t) * 64];
-                    qt[i][ks][t] = qt0[at + ((2 * i + ks) * NI + t) * 64];
-                }
-    };
+    auto dout = [&](int nc, int r) { return In::to_f32(y[nc][r]); };
     // dS (behind chunk c) and dO (of chunk c) for all waves
     auto share = [&](int c) {
 #pragma unroll
@@ -104,15 +82,15 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
                 share_tile<3, NC>(sbuf, w, nc, lane, S[0][nc]);
             }
             share_tile<NI, NC>(ybuf, w, nc, lane,
-                               (f32x4){dout(c, nc, 0), dout(c, nc, 1), dout(c, nc, 2), dout(c, nc, 3)});
+                               (f32x4){dout(nc, 0), dout(nc, 1), dout(nc, 2), dout(nc, 3)});
         }
-        float* to = a.dstates + ((vslot0 + (size_t)c * a.hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col;
+        float* to = a.dstates + ((at.vslot + (size_t)c * a.hv) * DK + 16 * MW * w) * a.dv_width;
 #pragma unroll
         for (int i = 0; i < MW; ++i)
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) to[(size_t)(16 * i + r) * a.dv_width + 16 * nc] = S[i][nc][r];
+                for (int r = 0; r < 4; ++r) (to + (size_t)16 * i * a.dv_width + 16 * nc)[tile_at[r]] = S[i][nc][r];
     };
     if (chunks > 0) {
         const int c = chunks - 1;
@@ -160,7 +138,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
             for (int r = 0; r < 4; ++r) {
                 const float e = NS == 2 ? E[0][nc][r] + E[NS - 1][nc][r] : E[0][nc][r];
                 E[0][nc][r] = beta_of(beta[r]) * (ec[r] * e + a.scale * (P[0][nc][r] + P[1][nc][r]));
-                x[r] = a.scale * eb[r] * dout(c, nc, r);
+                x[r] = a.scale * eb[r] * dout(nc, r);
             }
             share_tile<3, NC>(dbuf, w, nc, lane, E[0][nc]);
             share_tile<3, NC>(wbuf, w, nc, lane, x);
@@ -180,13 +158,13 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
             z0 = mm(tt[0], b[0], z0);
             z1 = mm(tt[1], b[1], z1);
             const f32x4 Z = z0 + z1;
-            float* to = a.z + ((vslot0 + (size_t)c * a.hv) * kDeltaChunk + row) * a.dv_width + col + 16 * nc;
-            raw* dv = (raw*)a.dv + ((size_t)(sp.begin + c * kDeltaChunk + row) * a.hv + hv) * a.dv_width + col + 16 * nc;
+            float* to = a.z + ((at.vslot + (size_t)c * a.hv) * kDeltaChunk + 16 * w) * a.dv_width + 16 * nc;
+            raw* dv = (raw*)a.dv + ((size_t)(sp.begin + c * kDeltaChunk) * a.hv + hv) * a.dv_width + 16 * nc;
             f32x4 x;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                to[r * a.dv_width] = Z[r];
-                *(row + r < n ? dv + (size_t)r * a.hv * a.dv_width : (raw*)a.sink + col) = In::from_f32(Z[r]);
+                to[tile_at[r]] = Z[r];
+                if (row + r < n) dv[dv_at[r]] = In::from_f32(Z[r]);
                 x[r] = -head[r] * Z[r];
             }
             share_tile<3, NC>(zbuf, w, nc, lane, x);

@@ -1,6 +1,8 @@
 // ops_delta.hip -- C entries of the gated delta rule (include/helen_hip.h): checks, workspace layout, forward launches
 #include "ops_delta.h"
 
+#include <initializer_list>
+
 namespace helen {
 
 namespace {
@@ -77,6 +79,10 @@ int describe(const HelenDeltaRule* op, Check level, DeltaArgs* a) {
         if (!aligned(op->q, op->q_stride, size, 16) || !aligned(op->k, op->k_stride, size, 16) ||
             !aligned(op->v, op->v_stride, size, 16))
             return fail(HELEN_EINVAL, "delta rule: q, k, v and their strides must be multiples of 16 bytes");
+        const int64_t most = int64_t(1) << 24;      // 64 rows fit 32 bits of elements
+        for (const int64_t t : {op->q_stride[0], op->k_stride[0], op->v_stride[0], op->o ? op->o_stride[0] : 0, backward ? op->d_o_stride[0] : 0,
+                                (int64_t)op->heads_v * op->width_v})
+            if (t < 0 || t > most) return fail(HELEN_EINVAL, "delta rule: a stride of %lld elements between tokens", (long long)t);
         if (backward) {
             if (!op->d_o || !op->grad_q || !op->grad_k || !op->grad_v || !op->grad_g || !op->grad_beta)
                 return fail(HELEN_EINVAL, "delta rule: null gradient");

@@ -38,7 +38,7 @@ def _inner(t, bytes_=0):
     it has to be one."""
     if t.numel() and t.stride(-1) != 1 and t.shape[-1] != 1:
         return t.contiguous()
-    if bytes_ and (t.data_ptr() % bytes_ or any(s * t.element_size() % bytes_ for s in t.stride()[:-1])):
+    if bytes_ and (t.data_ptr() % bytes_ or any(s * t.element_size() % bytes_ for s in t.stride()[:-1]) or t.stride(0) > 1 << 24):
         return t.clone(memory_format=torch.contiguous_format) if t.is_contiguous() else t.contiguous()
     return t
 
