@@ -57,25 +57,40 @@ struct InF32 {
     static __device__ __forceinline__ raw from_f32(float f) { return f; }
 };
 
-// N bf16 terms of eight fp32 values (x = t[0] + t[1] + t[2] exactly: 3 x 8 significand bits)
-template <int N>
-__device__ __forceinline__ void split8(const f32x4 lo, const f32x4 hi, bf16x8 (&t)[N]) {
-    u32x4 out[N];
+// VALU instructions stay on their side of this, all others may cross
+__device__ __forceinline__ void valu_fence() { __builtin_amdgcn_sched_barrier(0x4 | 0x8 | 0x10 | 0x80); }
+
+// N bf16 terms of 2 P fp32 values: x = t[0] + t[1] + t[2] exactly (3 x 8 significand bits).  One level of all values after the
+// other: a VALU instruction that needs the result of the one right before it costs 9 cycles here instead of 4 to 5, and left
+// alone the compiler puts each value's chain in one piece.
+template <int N, int P>
+__device__ __forceinline__ void split_pairs(f32x2 (&x)[P], unsigned (&t)[N][P]) {
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-        f32x2 x = p < 2 ? (f32x2){lo[2 * p], lo[2 * p + 1]} : (f32x2){hi[2 * p - 4], hi[2 * p - 3]};
+    for (int n = 0; n < N; ++n) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const unsigned b = __builtin_bit_cast(unsigned, __builtin_convertvector(x, bf16x2_t));
-            out[n][p] = b;
-            if (n + 1 < N) {
-                x.x -= __builtin_bit_cast(float, b << 16);
-                x.y -= __builtin_bit_cast(float, b & 0xffff0000u);
+        for (int p = 0; p < P; ++p) t[n][p] = __builtin_bit_cast(unsigned, __builtin_convertvector(x[p], bf16x2_t));
+        if (n + 1 < N) {
+            f32x2 hi[P];
+            valu_fence();
+#pragma unroll
+            for (int p = 0; p < P; ++p) hi[p] = (f32x2){__builtin_bit_cast(float, t[n][p] << 16), __builtin_bit_cast(float, t[n][p] & 0xffff0000u)};
+            valu_fence();
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                x[p].x -= hi[p].x;
+                x[p].y -= hi[p].y;
             }
+            valu_fence();
         }
     }
+}
+template <int N>
+__device__ __forceinline__ void split8(const f32x4 lo, const f32x4 hi, bf16x8 (&t)[N]) {
+    f32x2 x[4] = {{lo[0], lo[1]}, {lo[2], lo[3]}, {hi[0], hi[1]}, {hi[2], hi[3]}};
+    unsigned w[N][4];
+    split_pairs<N, 4>(x, w);
 #pragma unroll
-    for (int n = 0; n < N; ++n) t[n] = __builtin_bit_cast(bf16x8, out[n]);
+    for (int n = 0; n < N; ++n) t[n] = __builtin_bit_cast(bf16x8, (u32x4){w[n][0], w[n][1], w[n][2], w[n][3]});
 }
 
 // c += A B over 32 k, of operands in NA and NB terms: the products of terms whose orders add up to 2 at most, small ones first
@@ -484,19 +499,11 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a) {
 // four values in N terms: the half of a fragment that one row tile is
 template <int N>
 __device__ __forceinline__ void split4(const f32x4 v, u32x2 (&t)[N]) {
+    f32x2 x[2] = {{v[0], v[1]}, {v[2], v[3]}};
+    unsigned w[N][2];
+    split_pairs<N, 2>(x, w);
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-        f32x2 x = {v[2 * p], v[2 * p + 1]};
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const unsigned b = __builtin_bit_cast(unsigned, __builtin_convertvector(x, bf16x2_t));
-            t[n][p] = b;
-            if (n + 1 < N) {
-                x.x -= __builtin_bit_cast(float, b << 16);
-                x.y -= __builtin_bit_cast(float, b & 0xffff0000u);
-            }
-        }
-    }
+    for (int n = 0; n < N; ++n) t[n] = (u32x2){w[n][0], w[n][1]};
 }
 // row tile mt of a [64 or DK x 16 NC] operand that the workgroup shares: fragments [k step][term][column tile][lane]
 template <int N, int NC>
@@ -798,11 +805,18 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
         load_p(next);
         issue_loads();
         raw* const to = (raw*)a.o + (sp.begin + c * kDeltaChunk) * a.o_t + hv * a.o_h;
+        if (n >= kDeltaChunk) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (row + r < n)
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
                 for (int nc = 0; nc < NC; ++nc) (to + 16 * nc)[orow.at[r]] = In::from_f32(a.scale * O[nc][r]);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (row + r < n)
+#pragma unroll
+                    for (int nc = 0; nc < NC; ++nc) (to + 16 * nc)[orow.at[r]] = In::from_f32(a.scale * O[nc][r]);
+        }
         lds_barrier();
     }
     if (a.s1) {

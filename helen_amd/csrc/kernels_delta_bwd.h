@@ -162,10 +162,16 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
             raw* dv = (raw*)a.dv + ((size_t)(sp.begin + c * kDeltaChunk) * a.hv + hv) * a.dv_width + 16 * nc;
             f32x4 x;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                to[tile_at[r]] = Z[r];
-                if (row + r < n) dv[dv_at[r]] = In::from_f32(Z[r]);
-                x[r] = -head[r] * Z[r];
+            for (int r = 0; r < 4; ++r) x[r] = -head[r] * Z[r];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) to[tile_at[r]] = Z[r];
+            if (n >= kDeltaChunk) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) dv[dv_at[r]] = In::from_f32(Z[r]);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (row + r < n) dv[dv_at[r]] = In::from_f32(Z[r]);
             }
             share_tile<3, NC>(zbuf, w, nc, lane, x);
         }
