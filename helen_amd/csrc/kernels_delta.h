@@ -116,6 +116,34 @@ __device__ __forceinline__ f32x4 load4(const typename In::raw* p) {
     }
 }
 
+// NC neighbouring elements of a row
+template <typename In, int NC>
+struct Columns {
+    typedef typename In::raw raw;
+    typedef raw vec __attribute__((ext_vector_type(NC), aligned(sizeof(raw))));
+    vec v;
+    static __device__ __forceinline__ Columns load(const raw* p) { return {*(const vec*)p}; }
+    __device__ __forceinline__ float get(int nc) const { return In::to_f32(v[nc]); }
+    static __device__ __forceinline__ void store(raw* p, const float (&x)[NC]) {
+        vec t;
+        if constexpr (In::kTerms == 1 && NC == 2) {      // (one conversion for both)
+            t = __builtin_bit_cast(vec, __builtin_convertvector((f32x2){x[0], x[1]}, bf16x2_t));
+        } else {
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc) t[nc] = In::from_f32(x[nc]);
+        }
+        *(vec*)p = t;
+    }
+};
+template <typename In>
+struct Columns<In, 1> {
+    typedef typename In::raw raw;
+    raw v;
+    static __device__ __forceinline__ Columns load(const raw* p) { return {*p}; }
+    __device__ __forceinline__ float get(int) const { return In::to_f32(v); }
+    static __device__ __forceinline__ void store(raw* p, const float (&x)[1]) { *p = In::from_f32(x[0]); }
+};
+
 // ---- arguments of the launches (built by ops_delta.hip) ----
 struct DeltaArgs {
     const void *q, *k, *v, *dout;
@@ -586,7 +614,7 @@ struct ChainAddress {
 struct RowOffsets {
     unsigned at[4], stride;
     int row, col, full;
-    __device__ __forceinline__ RowOffsets(long stride_, int row_, int col0, int j) : stride((unsigned)stride_), row(row_), col(col0 + j), full(1) {
+    __device__ __forceinline__ RowOffsets(long stride_, int row_, int col_) : stride((unsigned)stride_), row(row_), col(col_), full(1) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) at[r] = (row + r) * stride + col;
     }
@@ -599,21 +627,33 @@ struct RowOffsets {
     }
 };
 
+// NC neighbouring D tiles to a [.., dv] fp32 matrix; at[r]: the lane's offset in row r of its four
+template <int NC>
+__device__ __forceinline__ void store_tile(float* to, const unsigned (&at)[4], const f32x4 (&x)[NC]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        float row[NC];
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) row[nc] = x[nc][r];
+        Columns<InF32, NC>::store(to + at[r], row);
+    }
+}
+
 // A wave's rows of a state [DK, dv]: MW row tiles, 16 rows of stride `dv` apart; zero where there is no state.  The loads are not
 // conditional (they read some zeros then): behind a skipped load the compiler waits for everything that is in flight.
 template <int MW, int NC>
 __device__ __forceinline__ void load_state(const float* state, const void* zeros, size_t at, int dv, f32x4 (&S)[MW][NC]) {
+    typedef Columns<InF32, NC> Cols;
     const float* const from = state ? state + at : (const float*)zeros;
     const size_t stride = state ? dv : 0;
 #pragma unroll
     for (int i = 0; i < MW; ++i)
 #pragma unroll
-        for (int nc = 0; nc < NC; ++nc)
+        for (int r = 0; r < 4; ++r) {
+            const Cols x = Cols::load(from + (16 * i + r) * stride);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float x = from[(16 * i + r) * stride + 16 * nc];
-                S[i][nc][r] = state ? x : 0.f;
-            }
+            for (int nc = 0; nc < NC; ++nc) S[i][nc][r] = state ? x.get(nc) : 0.f;
+        }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -633,7 +673,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
     const unsigned item = xcd_order(blockIdx.x, gridDim.x);
     if (item >= (unsigned)a.nseq * a.hv * groups) return;
     const int hv = item / groups % a.hv, s = item / groups / a.hv, h = hv / a.group;
-    const int col = 16 * NC * (item % groups) + j;
+    const int col = NC * (16 * (item % groups) + j);    // column tile nc has columns 16 NC g + NC j + nc: a lane's are neighbours
     const Span sp = span_of(a, s);
     const int chunks = (sp.len + kDeltaChunk - 1) / kDeltaChunk;
     const size_t st = (((size_t)s * a.hv + hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col;
@@ -643,12 +683,12 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
 
     bf16x8 kf[KS][NI], qf[KS][NI], kt[MW][2][NI], tf[2][3], pf[2][PT];
     f32x4 beta, eb, ec, whole;
-    raw v[NC][4];
+    Columns<In, NC> v[4];
     const int row = 16 * w + 4 * q;                 // this lane's tokens: row .. row + 3
     const ChainAddress<In, DK> at(a, sp, h, hv, w, lane);
     // (No load of the loop is conditional: the compiler counts what is in flight, and a skipped load would make it wait for
     // everything.  Rows behind the sequence's end read its last row: their k and beta are zero.)
-    RowOffsets vrow(a.v_t, row, col - j, j), orow(a.o_t, row, col - j, j);
+    RowOffsets vrow(a.v_t, row, col), orow(a.o_t, row, col);
     auto load_tokens = [&](int c) {
         const float* sc = a.sc + (at.vslot + (size_t)c * a.hv) * 256;
         beta = *(const f32x4*)(sc + row);
@@ -658,9 +698,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
         vrow.clamp(sp.len - c * kDeltaChunk);
         const raw* p = (const raw*)a.v + (sp.begin + c * kDeltaChunk) * a.v_t + hv * a.v_h;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int nc = 0; nc < NC; ++nc) v[nc][r] = (p + 16 * nc)[vrow.at[r]];
+        for (int r = 0; r < 4; ++r) v[r] = Columns<In, NC>::load(p + vrow.at[r]);
     };
     auto load_k = [&](int c) { at.rows(a.kf, c, kf); };
     auto load_q = [&](int c) { at.rows(a.qf, c, qf); };
@@ -685,11 +723,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
         if constexpr (KEEP) {
             float* to = a.states + ((at.vslot + (size_t)c * a.hv) * DK + 16 * MW * w) * a.dv_width;
 #pragma unroll
-            for (int i = 0; i < MW; ++i)
-#pragma unroll
-                for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) (to + (size_t)16 * i * a.dv_width + 16 * nc)[tile_at[r]] = S[i][nc][r];
+            for (int i = 0; i < MW; ++i) store_tile<NC>(to + (size_t)16 * i * a.dv_width, tile_at, S[i]);
         }
     };
     if (chunks > 0) {
@@ -727,7 +761,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float x = NS == 2 ? sums[0][nc][r] + sums[NS - 1][nc][r] : sums[0][nc][r];
-                R[nc][r] = In::to_f32(v[nc][r]) - eb[r] * x;
+                R[nc][r] = v[r].get(nc) - eb[r] * x;
             }
             share_tile<3, NC>(xbuf, w, nc, lane, R[nc]);
         }
@@ -752,13 +786,9 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
         }
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) O[nc] = NS == 2 ? osum[0][nc] + osum[NS - 1][nc] : osum[0][nc];
+        if constexpr (KEEP) store_tile<NC>(a.e + ((at.vslot + (size_t)c * a.hv) * kDeltaChunk + 16 * w) * a.dv_width, tile_at, U);
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
-            if constexpr (KEEP) {
-                float* to = a.e + ((at.vslot + (size_t)c * a.hv) * kDeltaChunk + 16 * w) * a.dv_width + 16 * nc;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) to[tile_at[r]] = U[nc][r];
-            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) U[nc][r] *= step[r];
             share_tile<PT, NC>(ubuf, w, nc, lane, U[nc]);
@@ -805,27 +835,26 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
         load_p(next);
         issue_loads();
         raw* const to = (raw*)a.o + (sp.begin + c * kDeltaChunk) * a.o_t + hv * a.o_h;
+        auto put = [&](int r) {
+            float x[NC];
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc) x[nc] = a.scale * O[nc][r];
+            Columns<In, NC>::store(to + orow.at[r], x);
+        };
         if (n >= kDeltaChunk) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int nc = 0; nc < NC; ++nc) (to + 16 * nc)[orow.at[r]] = In::from_f32(a.scale * O[nc][r]);
+            for (int r = 0; r < 4; ++r) put(r);
         } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (row + r < n)
-#pragma unroll
-                    for (int nc = 0; nc < NC; ++nc) (to + 16 * nc)[orow.at[r]] = In::from_f32(a.scale * O[nc][r]);
+                if (row + r < n) put(r);
         }
         lds_barrier();
     }
     if (a.s1) {
+        float* const to = a.s1 + (((size_t)s * a.hv + hv) * DK + 16 * MW * w) * a.dv_width;
 #pragma unroll
-        for (int i = 0; i < MW; ++i)
-#pragma unroll
-            for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) a.s1[st + (size_t)(16 * i + r) * a.dv_width + 16 * nc] = S[i][nc][r];
+        for (int i = 0; i < MW; ++i) store_tile<NC>(to + (size_t)16 * i * a.dv_width, tile_at, S[i]);
     }
 }
 

@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
     const unsigned item = xcd_order(blockIdx.x, gridDim.x);
     if (item >= (unsigned)a.nseq * a.hv * groups) return;
     const int hv = item / groups % a.hv, s = item / groups / a.hv, h = hv / a.group;
-    const int col = 16 * NC * (item % groups) + j;
+    const int col = NC * (16 * (item % groups) + j);
     const Span sp = span_of(a, s);
     const int chunks = (sp.len + kDeltaChunk - 1) / kDeltaChunk;
     const size_t st = (((size_t)s * a.hv + hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col;
@@ -36,10 +36,10 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
 
     bf16x8 kf[KS][NI], kt[MW][2][NI], qt[MW][2][NI], tt[2][3], pt[2][3];
     f32x4 beta, eb, ec, whole;
-    raw y[NC][4];
+    Columns<In, NC> y[4];
     const int row = 16 * w + 4 * q;
     const ChainAddress<In, DK> at(a, sp, h, hv, w, lane);
-    RowOffsets yrow(a.do_t, row, col - j, j);
+    RowOffsets yrow(a.do_t, row, col);
     unsigned tile_at[4], dv_at[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -64,11 +64,9 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
         yrow.clamp(sp.len - c * kDeltaChunk);
         const raw* p = (const raw*)a.dout + (sp.begin + c * kDeltaChunk) * a.do_t + hv * a.do_h;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int nc = 0; nc < NC; ++nc) y[nc][r] = (p + 16 * nc)[yrow.at[r]];
+        for (int r = 0; r < 4; ++r) y[r] = Columns<In, NC>::load(p + yrow.at[r]);
     };
-    auto dout = [&](int nc, int r) { return In::to_f32(y[nc][r]); };
+    auto dout = [&](int nc, int r) { return y[r].get(nc); };
     // dS (behind chunk c) and dO (of chunk c) for all waves
     auto share = [&](int c) {
 #pragma unroll
@@ -86,11 +84,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
         }
         float* to = a.dstates + ((at.vslot + (size_t)c * a.hv) * DK + 16 * MW * w) * a.dv_width;
 #pragma unroll
-        for (int i = 0; i < MW; ++i)
-#pragma unroll
-            for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) (to + (size_t)16 * i * a.dv_width + 16 * nc)[tile_at[r]] = S[i][nc][r];
+        for (int i = 0; i < MW; ++i) store_tile<NC>(to + (size_t)16 * i * a.dv_width, tile_at, S[i]);
     };
     if (chunks > 0) {
         const int c = chunks - 1;
@@ -149,6 +143,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
         load_tri(next, a.ptf, pt);
         issue_loads();
         lds_barrier();
+        f32x4 Z[NC];
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
             f32x4 z0 = splat4(0.f), z1 = splat4(0.f);
@@ -157,23 +152,30 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
             shared_frag<3, NC>(dbuf, 1, nc, lane, b[1]);
             z0 = mm(tt[0], b[0], z0);
             z1 = mm(tt[1], b[1], z1);
-            const f32x4 Z = z0 + z1;
-            float* to = a.z + ((at.vslot + (size_t)c * a.hv) * kDeltaChunk + 16 * w) * a.dv_width + 16 * nc;
-            raw* dv = (raw*)a.dv + ((size_t)(sp.begin + c * kDeltaChunk) * a.hv + hv) * a.dv_width + 16 * nc;
+            Z[nc] = z0 + z1;
+        }
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
             f32x4 x;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = -head[r] * Z[r];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) to[tile_at[r]] = Z[r];
-            if (n >= kDeltaChunk) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) dv[dv_at[r]] = In::from_f32(Z[r]);
-            } else {
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (row + r < n) dv[dv_at[r]] = In::from_f32(Z[r]);
-            }
+            for (int r = 0; r < 4; ++r) x[r] = -head[r] * Z[nc][r];
             share_tile<3, NC>(zbuf, w, nc, lane, x);
+        }
+        store_tile<NC>(a.z + ((at.vslot + (size_t)c * a.hv) * kDeltaChunk + 16 * w) * a.dv_width, tile_at, Z);
+        raw* const dv = (raw*)a.dv + ((size_t)(sp.begin + c * kDeltaChunk) * a.hv + hv) * a.dv_width;
+        auto put = [&](int r) {
+            float x[NC];
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc) x[nc] = Z[nc][r];
+            Columns<In, NC>::store(dv + dv_at[r], x);
+        };
+        if (n >= kDeltaChunk) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) put(r);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (row + r < n) put(r);
         }
         load_tri(next, a.ttf, tt);
         issue_loads();
@@ -203,12 +205,9 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
         lds_barrier();
     }
     if (a.ds0) {
+        float* const to = a.ds0 + (((size_t)s * a.hv + hv) * DK + 16 * MW * w) * a.dv_width;
 #pragma unroll
-        for (int i = 0; i < MW; ++i)
-#pragma unroll
-            for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) a.ds0[st + (size_t)(16 * i + r) * a.dv_width + 16 * nc] = S[i][nc][r];
+        for (int i = 0; i < MW; ++i) store_tile<NC>(to + (size_t)16 * i * a.dv_width, tile_at, S[i]);
     }
 }
 
