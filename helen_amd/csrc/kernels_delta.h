@@ -144,6 +144,12 @@ struct Columns<In, 1> {
     static __device__ __forceinline__ void store(raw* p, const float (&x)[1]) { *p = In::from_f32(x[0]); }
 };
 
+// LDS writes of every wave are visible behind this; loads and stores to memory stay in flight over it
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 // ---- arguments of the launches (built by ops_delta.hip) ----
 struct DeltaArgs {
     const void *q, *k, *v, *dout;
@@ -188,23 +194,32 @@ __device__ __forceinline__ Span span_of(const DeltaArgs& a, int s) {
     }
     return {b, e - b, b / kDeltaChunk + s};
 }
-// The sequence that holds a slot: 64 probes a round.
-__device__ __forceinline__ int sequence_of(const DeltaArgs& a, int slot, int lane) {
+// The sequence that holds a slot, 64 probes a round, and its span (read in the last round: one trip to memory less)
+__device__ __forceinline__ int sequence_of(const DeltaArgs& a, int slot, int lane, Span* span) {
     int lo = 0, n = a.nseq;
-    while (n > 1) {
+    while (true) {
         const int step = (n + 63) >> 6;
-        const int s = lo + lane * step;
-        bool below = false;
-        if (lane * step < n) {
-            const int b = a.offsets ? min(max(a.offsets[s], 0), a.tokens) : s * a.seq_len;
-            below = b / kDeltaChunk + s <= slot;
+        const int s = min(lo + lane * step, a.nseq - 1);
+        int b, e;
+        if (a.offsets) {
+            b = min(max(a.offsets[s], 0), a.tokens);
+            e = min(max(a.offsets[s + 1], b), a.tokens);
+        } else {
+            b = s * a.seq_len;
+            e = b + a.seq_len;
         }
-        const int hits = __popcll(__ballot(below));
-        const int at = max(hits - 1, 0) * step;
-        lo += at;
-        n = min(step, n - at);
+        const int hits = __popcll(__ballot(lane * step < n && b / kDeltaChunk + s <= slot));
+        const int at = max(hits - 1, 0);
+        if (step == 1) {
+            b = __builtin_amdgcn_readlane(b, at);
+            e = __builtin_amdgcn_readlane(e, at);
+            lo += at;
+            *span = {b, e - b, b / kDeltaChunk + lo};
+            return lo;
+        }
+        lo += at * step;
+        n = min(step, n - at * step);
     }
-    return lo;
 }
 
 // lower triangle (tf, pf): fragment f = row tile mt, k step ks of mt's; the last step of an even row tile ends in a zero half
@@ -233,54 +248,101 @@ template <int CTRL>
 __device__ __forceinline__ float dpp_add(float x) {
     return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
-// sums of the chunk's g (lane = token) within its block of 16: up to and with the token, and after it
-__device__ __forceinline__ void block_scans(float g, float* head, float* tail) {
-    *head = dpp_add<0x118>(dpp_add<0x114>(dpp_add<0x112>(dpp_add<0x111>(g))));
-    const float next = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, g), 0x101, 0xf, 0xf, true));
-    *tail = dpp_add<0x108>(dpp_add<0x104>(dpp_add<0x102>(dpp_add<0x101>(next))));
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
-// What a chunk's decays are made of, in LDS: g, the scans within blocks of 16.  Written by the 64 lanes of one wave.
+// What a chunk's decays are made of, in LDS.  e^{D_ij} is a product: from j to the end of its block of 16 tokens, over the blocks
+// between, from the start of i's block to i -- and inside a block the same over groups of four.  Each factor is e to a sum of
+// the g it covers.  (All are at most one where g <= 0: a product that underflows stands for a decay that does.)
 struct Decays {
-    float g[64], head[64], tail[64];
+    float g[64];
+    float head[64], tail[64];      // e^(sum of g): from the block's start up to and with the token; after it to the block's end
+    float head4[64], tail4[64];    // the same in groups of four
+    // the 64 lanes of one wave
     __device__ __forceinline__ void set(int lane, float x) {
+        const int e = lane & 3;
         g[lane] = x;
-        block_scans(x, &head[lane], &tail[lane]);
+        const float h = dpp_add<0x118>(dpp_add<0x114>(dpp_add<0x112>(dpp_add<0x111>(x))));
+        const float t = dpp_add<0x108>(dpp_add<0x104>(dpp_add<0x102>(dpp_add<0x101>(dpp<0x101>(x)))));
+        // (neighbours are read by all lanes, and then chosen: a lane that is switched off gives nothing)
+        const float b1 = dpp<0x111>(x), n1 = dpp<0x101>(x);
+        float h4 = x + (e >= 1 ? b1 : 0.f), t4 = x + (e <= 2 ? n1 : 0.f);
+        const float b2 = dpp<0x112>(h4), n2 = dpp<0x102>(t4);
+        h4 += e >= 2 ? b2 : 0.f;
+        t4 += e <= 1 ? n2 : 0.f;
+        t4 = dpp<0x101>(t4);
+        head[lane] = exp_decay(h);
+        tail[lane] = exp_decay(t);
+        head4[lane] = exp_decay(h4);
+        tail4[lane] = exp_decay(e <= 2 ? t4 : 0.f);
     }
     __device__ __forceinline__ float block(int b) const { return head[16 * b + 15]; }
-    // sums from the chunk's start up to and with token `lane`, and after it to the chunk's end
-    __device__ __forceinline__ void ends(int lane, float* from_start, float* to_end) const {
-        float a = head[lane], b = tail[lane];
+    // e^b and e^c of token `lane`, and of the whole chunk
+    __device__ __forceinline__ void ends(int lane, float* from_start, float* to_end, float* whole) const {
+        float a = head[lane], b = tail[lane], all = 1.f;
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             const float x = block(m);
-            a += m < (lane >> 4) ? x : 0.f;
-            b += m > (lane >> 4) ? x : 0.f;
+            a *= m < (lane >> 4) ? x : 1.f;
+            b *= m > (lane >> 4) ? x : 1.f;
+            all *= x;
         }
         *from_start = a;
         *to_end = b;
+        *whole = all;
     }
-    // e^{D_ij} of tile (mt, nt <= mt): rows i = 16 mt + 4 q + r, column 16 nt + j; what lies above the diagonal is not used
-    __device__ __forceinline__ f32x4 tile(int mt, int nt, int j, int q) const {
-        f32x4 d = splat4(0.f);
+    __device__ __forceinline__ float between(int mt, int nt) const {
+        float x = 1.f;
+        if (nt + 1 < mt) x *= block(nt + 1);
+        if (nt + 2 < mt) x *= block(nt + 2);
+        return x;
+    }
+    __device__ __forceinline__ float between4(int mt, int iq, int jq) const {      // groups of four jq < k < iq of block mt
+        float x = jq < 1 && iq > 1 ? head4[16 * mt + 7] : 1.f;
+        return jq < 2 && iq > 2 ? x * head4[16 * mt + 11] : x;
+    }
+    // e^{D_ij} of tile (mt, nt <= mt); what lies above the diagonal is not used.
+    // rows: i = 16 mt + 4 q + r, column 16 nt + j (as results lie)
+    __device__ __forceinline__ f32x4 rows(int mt, int nt, int j, int q) const {
+        f32x4 d;
         if (nt < mt) {
-            float t = tail[16 * nt + j];
-            if (nt + 1 < mt) t += block(nt + 1);
-            if (nt + 2 < mt) t += block(nt + 2);
-            d = *(const f32x4*)&head[16 * mt + 4 * q];
+            const float t = tail[16 * nt + j] * between(mt, nt);
+            const f32x4 h = *(const f32x4*)&head[16 * mt + 4 * q];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) d[r] += t;
+            for (int r = 0; r < 4; ++r) d[r] = h[r] * t;
         } else {
-#pragma unroll
-            for (int m4 = 0; m4 < 4; ++m4) {
-                const f32x4 x = *(const f32x4*)&g[16 * mt + 4 * m4];
-#pragma unroll
-                for (int m = 0; m < 4; ++m)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) d[r] += (4 * m4 + m > j && 4 * m4 + m <= 4 * q + r) ? x[m] : 0.f;
-            }
+            const f32x4 x = *(const f32x4*)&g[16 * mt + 4 * q], h = *(const f32x4*)&head4[16 * mt + 4 * q];
+            const int jq = j >> 2, je = j & 3;
+            const float t = tail4[16 * mt + j] * between4(mt, q, jq);
+            const float d1 = je < 1 ? x[1] : 0.f, d2 = d1 + (je < 2 ? x[2] : 0.f), d3 = d2 + (je < 3 ? x[3] : 0.f);
+            const bool same = q == jq;
+            d[0] = same ? 1.f : h[0] * t;
+            d[1] = same ? exp_decay(d1) : h[1] * t;
+            d[2] = same ? exp_decay(d2) : h[2] * t;
+            d[3] = same ? exp_decay(d3) : h[3] * t;
         }
+        return d;
+    }
+    // columns: row 16 mt + j, column 16 nt + 4 q + r (as left-hand operands lie)
+    __device__ __forceinline__ f32x4 columns(int mt, int nt, int j, int q) const {
+        f32x4 d;
+        if (nt < mt) {
+            const float h = head[16 * mt + j] * between(mt, nt);
+            const f32x4 t = *(const f32x4*)&tail[16 * nt + 4 * q];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) d[r] = exp_decay(d[r]);
+            for (int r = 0; r < 4; ++r) d[r] = h * t[r];
+        } else {
+            const f32x4 x = *(const f32x4*)&g[16 * mt + 4 * q], t = *(const f32x4*)&tail4[16 * mt + 4 * q];
+            const int iq = j >> 2, ie = j & 3;
+            const float h = head4[16 * mt + j] * between4(mt, iq, q);
+            const float d2 = ie > 2 ? x[3] : 0.f, d1 = d2 + (ie > 1 ? x[2] : 0.f), d0 = d1 + (ie > 0 ? x[1] : 0.f);
+            const bool same = q == iq;
+            d[0] = same ? exp_decay(d0) : h * t[0];
+            d[1] = same ? exp_decay(d1) : h * t[1];
+            d[2] = same ? exp_decay(d2) : h * t[2];
+            d[3] = same ? 1.f : h * t[3];
+        }
         return d;
     }
 };
@@ -290,24 +352,25 @@ constexpr int kTriStride = 68;    // floats per row of a 64 x 64 matrix in LDS: 
 // ------------------------------------------------------------------------------------------------
 // Everything of a chunk that does not depend on the state.  One workgroup per (slot, key head); the value heads that share
 // the key head follow one another (K K^T and Q K^T are theirs together).
+//
+// What becomes a left-hand operand is computed transposed, (Q K^T)^T = K Q^T: a result tile then already lies as that operand
+// (lane = row, four neighbouring columns), so P goes from the accumulators to memory, and A to LDS and back in whole
+// fragments.  K^T comes from the matrix pipe too: K times a selection of 16 columns is K's tile with lane = dk.
 // ------------------------------------------------------------------------------------------------
 template <typename In, int DK, int PT, bool BWD>
-__global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a) {
+__global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_prep_kernel(const DeltaArgs a) {
     constexpr int NI = In::kTerms, KS = DK / 32;
+    constexpr int kTile = 64 + 4;               // an operand tile in LDS: [column / 4][row] x 4, column groups 17 apart
     typedef typename In::raw raw;
-    __shared__ bf16x8 kfr[4 * KS * NI * 64];
-    __shared__ f32x4 amat4[64 * kTriStride / 4], pmat4[64 * kTriStride / 4], tmat4[64 * kTriStride / 4];
+    __shared__ bf16x8 kfr[4 * KS * NI * 64], qfr[4 * KS * NI * 64];
+    __shared__ f32x4 atile[10 * 64], ttile[10 * kTile];
     __shared__ __attribute__((aligned(16))) Decays dec;
-    __shared__ float bs[64];
-    float* const amat = (float*)amat4;
-    float* const pmat = (float*)pmat4;
-    float* const tmat = (float*)tmat4;
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int j = lane & 15, q = lane >> 4;
+    __shared__ __attribute__((aligned(16))) float bs[64];
+    const int lane0 = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slot = blockIdx.x / a.hk, h = blockIdx.x % a.hk;
     if (blockIdx.x == 0 && threadIdx.x < 192) ((u32x4*)a.zeros)[threadIdx.x] = (u32x4){0, 0, 0, 0};
-    const int s = sequence_of(a, slot, lane);
-    const Span sp = span_of(a, s);
+    Span sp;
+    const int s = sequence_of(a, slot, lane0, &sp);
     const int c = slot - sp.slot;
     const int start = sp.begin + c * kDeltaChunk;
     const int n = min(kDeltaChunk, sp.begin + sp.len - start);
@@ -316,210 +379,279 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a) {
         if (a.zero_tail && s == a.nseq - 1) {
             const int end = sp.begin + sp.len;
             const int lo = max(end, (slot - a.nseq) * kDeltaChunk), hi = min(a.tokens, (slot - a.nseq + 1) * kDeltaChunk);
-            if (a.o)
-                for (int t = lo; t < hi; ++t)
-                    for (int hv = h * a.group; hv < (h + 1) * a.group; ++hv)
-                        for (int d = threadIdx.x; d < a.dv_width; d += 256) ((raw*)a.o)[t * a.o_t + hv * a.o_h + d] = raw(0);
+            for (int t = lo; t < hi; ++t)
+                for (int hv = h * a.group; hv < (h + 1) * a.group; ++hv)
+                    for (int d = threadIdx.x; d < a.dv_width; d += 256) ((raw*)a.o)[t * a.o_t + hv * a.o_h + d] = raw(0);
         }
         return;
     }
-
-    // K and Q rows of this wave's 16 tokens as fragments; rows behind the sequence's end are zero
-    bf16x8 kf[KS][NI], qf[KS][NI];
-    const int row = 16 * w + j;
-    const bool live = row < n;
-    {
-        const raw* kp = (const raw*)a.k + (start + (live ? row : 0)) * a.k_t + h * a.k_h;
-        const raw* qp = (const raw*)a.q + (start + (live ? row : 0)) * a.q_t + h * a.q_h;
-        const size_t at = ((size_t)(slot * (size_t)a.hk + h) * 4 + w) * KS * NI * 64 + lane;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const int d = 32 * ks + 4 * q;
-            const f32x4 zero = splat4(0.f);
-            split8<NI>(live ? load4<In>(kp + d) : zero, live ? load4<In>(kp + d + 16) : zero, kf[ks]);
-            split8<NI>(live ? load4<In>(qp + d) : zero, live ? load4<In>(qp + d + 16) : zero, qf[ks]);
-#pragma unroll
-            for (int t = 0; t < NI; ++t) {
-                a.kf[at + (ks * NI + t) * 64] = kf[ks][t];
-                a.qf[at + (ks * NI + t) * 64] = qf[ks][t];
-                kfr[((w * KS + ks) * NI + t) * 64 + lane] = kf[ks][t];
-            }
-        }
-    }
-    __syncthreads();
-    // K K^T and Q K^T, tiles (w, nt <= w): lane holds rows 16 w + 4 q + r, column 16 nt + j
-    f32x4 kk[4], qk[4];
-#pragma unroll
-    for (int nt = 0; nt < 4; ++nt) {
-        kk[nt] = qk[nt] = splat4(0.f);
-        if (nt <= w) {
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                bf16x8 b[NI];
-#pragma unroll
-                for (int t = 0; t < NI; ++t) b[t] = kfr[((nt * KS + ks) * NI + t) * 64 + lane];
-                kk[nt] = mm(kf[ks], b, kk[nt]);
-                qk[nt] = mm(qf[ks], b, qk[nt]);
-            }
-        }
-    }
-    if constexpr (BWD) {
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
-            if (nt <= w) {
-                f32x4* to = a.dots + (((size_t)slot * a.hk + h) * 10 + w * (w + 1) / 2 + nt) * 128 + lane;
-                to[0] = kk[nt];
-                to[64] = qk[nt];
-            }
-    }
-    // K^T (and Q^T): rows dk, k = tokens.  Element (token t, d) lies in fragment (t / 16, d / 32) at lane t % 16 + 16 ((d % 16) / 4)
-    auto transposed = [&](bf16x8* to) {
-        const unsigned short* src = (const unsigned short*)kfr;
-        for (int f = w; f < (DK / 16) * 2; f += 4) {
-            const int d = 16 * (f >> 1) + j;
-            const int ks = d >> 5, half = (d >> 4) & 1, dq = (d & 15) >> 2, e = d & 3;
-#pragma unroll
-            for (int t = 0; t < NI; ++t) {
-                u32x4 out;
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    unsigned x[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int el = 2 * p + i;
-                        const int tok = 32 * (f & 1) + (el < 4 ? 4 * q + el : 16 + 4 * q + el - 4);
-                        x[i] = src[((((tok >> 4) * KS + ks) * NI + t) * 64 + (tok & 15) + 16 * dq) * 8 + 4 * half + e];
-                    }
-                    out[p] = x[0] | x[1] << 16;
-                }
-                to[(((size_t)(slot * (size_t)a.hk + h) * (DK / 16) * 2 + f) * NI + t) * 64 + lane] = __builtin_bit_cast(bf16x8, out);
-            }
+    // g and beta of the value head that is next, a token a lane of wave 3
+    float gx = 0.f, bx = 0.f;
+    auto load_gates = [&](int hv) {
+        if (w == 3 && lane0 < n) {
+            gx = a.g[(start + lane0) * a.g_t + hv * a.g_h];
+            bx = a.beta[(start + lane0) * a.b_t + hv * a.b_h];
         }
     };
-    transposed(a.ktf);
-    if constexpr (BWD) {
-        __syncthreads();
+    load_gates(h * a.group);
+
+    // tiles (row tile, column tile) of this wave: those of its fragments of T, P ({0,1}, {2,3}, {4}, {5}) ...
+    const int count = w < 2 ? 3 : 2;
+    const int tm[3] = {w == 0 ? 0 : (w == 1 ? 2 : 3), w == 0 ? 1 : (w == 1 ? 2 : 3), w == 0 ? 1 : 2};
+    const int tn[3] = {w == 3 ? 2 : 0, w == 0 ? 0 : (w == 3 ? 3 : 1), w == 0 ? 1 : 2};
+    // ... and of T^T, P^T ({(0,0), (1,0)}, {(1,1), (3,1)}, {(0,1)}, {(2,1)})
+    const int um[3] = {w == 0 ? 0 : 2, w == 0 ? 1 : 3, w == 0 ? 1 : 3};
+    const int un[3] = {w == 0 ? 0 : (w == 1 ? 1 : (w == 2 ? 0 : 2)), w == 0 ? 0 : (w == 1 ? 1 : (w == 2 ? 0 : 2)), w == 0 ? 1 : 3};
+    f32x4 kkt[3], qkt[3], kk[3], qk[3];
+    {
+        const int lane = lane0, j = lane & 15, q = lane >> 4;
+        // K and Q rows of this wave's 16 tokens as fragments; rows behind the sequence's end are zero
+        bf16x8 kf[KS][NI], qf[KS][NI];
+        const int row = 16 * w + j;
+        const bool live = row < n;
+        const raw* kp = (const raw*)a.k + (start + (live ? row : 0)) * a.k_t + h * a.k_h + 4 * q;
+        const raw* qp = (const raw*)a.q + (start + (live ? row : 0)) * a.q_t + h * a.q_h + 4 * q;
+        f32x4 kx[KS][2], qx[KS][2];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-            for (int t = 0; t < NI; ++t) kfr[((w * KS + ks) * NI + t) * 64 + lane] = qf[ks][t];
-        __syncthreads();
-        transposed(a.qtf);
+            for (int i = 0; i < 2; ++i) {
+                kx[ks][i] = load4<In>(kp + 32 * ks + 16 * i);
+                qx[ks][i] = load4<In>(qp + 32 * ks + 16 * i);
+            }
+        bf16x8* const kto = a.kf + (((size_t)slot * a.hk + h) * 4 + w) * KS * NI * 64;
+        bf16x8* const qto = a.qf + (kto - a.kf);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const f32x4 zero = splat4(0.f);
+            split8<NI>(live ? kx[ks][0] : zero, live ? kx[ks][1] : zero, kf[ks]);
+            split8<NI>(live ? qx[ks][0] : zero, live ? qx[ks][1] : zero, qf[ks]);
+#pragma unroll
+            for (int t = 0; t < NI; ++t) {
+                kfr[((w * KS + ks) * NI + t) * 64 + lane] = kf[ks][t];
+                qfr[((w * KS + ks) * NI + t) * 64 + lane] = qf[ks][t];
+                (kto + (ks * NI + t) * 64)[lane] = kf[ks][t];
+                (qto + (ks * NI + t) * 64)[lane] = qf[ks][t];
+            }
+        }
+        // K^T, Q^T: half (w & 1) of the fragments of token step w >> 1, dk tiles 2 ks + i
+        const unsigned one = q == (j >> 2) ? 0x3f80u << (16 * (j & 1)) : 0u;
+        const unsigned lo = j & 2 ? 0u : one, hi = j & 2 ? one : 0u;
+        const bf16x8 pick[2] = {__builtin_bit_cast(bf16x8, (u32x4){lo, hi, 0u, 0u}), __builtin_bit_cast(bf16x8, (u32x4){0u, 0u, lo, hi})};
+        auto turn = [&](const bf16x8 (&from)[KS][NI], bf16x8* to) {
+            to += ((size_t)slot * a.hk + h) * (DK / 8) * NI * 64 + (w >> 1) * NI * 64;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int t = 0; t < NI; ++t) {
+                        const f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(from[ks][t], pick[i], splat4(0.f), 0, 0, 0);
+                        const u32x2 y = {__builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){x[0], x[1]}, bf16x2_t)),
+                                         __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){x[2], x[3]}, bf16x2_t))};
+                        ((u32x2*)(to + ((2 * ks + i) * 2 * NI + t) * 64))[2 * (unsigned)lane + (w & 1)] = y;
+                    }
+        };
+        turn(kf, a.ktf);
+        if constexpr (BWD) turn(qf, a.qtf);
+        lds_barrier();
+        auto product = [&](const bf16x8* x, int xt, const bf16x8* y, int yt) {
+            f32x4 sum = splat4(0.f);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                bf16x8 xf[NI], yf[NI];
+#pragma unroll
+                for (int t = 0; t < NI; ++t) {
+                    xf[t] = x[((xt * KS + ks) * NI + t) * 64 + lane];
+                    yf[t] = y[((yt * KS + ks) * NI + t) * 64 + lane];
+                }
+                sum = mm(xf, yf, sum);
+            }
+            return sum;
+        };
+#pragma unroll
+        for (int t = 0; t < 3; ++t) {
+            if (t >= count) continue;
+            kkt[t] = product(kfr, tn[t], kfr, tm[t]);
+            qkt[t] = product(kfr, tn[t], qfr, tm[t]);
+        }
+        if constexpr (BWD) {
+#pragma unroll
+            for (int t = 0; t < 3; ++t) {
+                if (t >= count) continue;
+                kk[t] = product(kfr, um[t], kfr, un[t]);
+                qk[t] = product(qfr, um[t], kfr, un[t]);
+                f32x4* to = a.dots + (((size_t)slot * a.hk + h) * 10 + um[t] * (um[t] + 1) / 2 + un[t]) * 128 + lane;
+                to[0] = kk[t];
+                to[64] = qk[t];
+            }
+        }
     }
 
-    const int lane0 = lane;
     for (int hv = h * a.group; hv < (h + 1) * a.group; ++hv) {
-        const int lane = in_block(lane0), j = lane & 15, q = lane >> 4;     // (nothing of a head's addresses is kept over the loop)
-        __syncthreads();
-        if (w == 0) {
-            const bool in = lane < n;
-            dec.set(lane, in ? a.g[(start + lane) * a.g_t + hv * a.g_h] : 0.f);
-            bs[lane] = in ? a.beta[(start + lane) * a.b_t + hv * a.b_h] : 0.f;
+        const unsigned lane = in_block(lane0);      // (nothing of a head's addresses is kept over the loop)
+        const int j = lane & 15, q = lane >> 4;
+        const size_t vslot = (size_t)slot * a.hv + hv;
+        if (w == 3) {
+            dec.set(lane, gx);
+            bs[lane] = bx;
+            if (hv + 1 < (h + 1) * a.group) load_gates(hv + 1);
         }
-        __syncthreads();
-        if (w == 0) {
-            float from_start, to_end;
-            dec.ends(lane, &from_start, &to_end);
-            float* sc = a.sc + (size_t)(slot * (size_t)a.hv + hv) * 256;
+        lds_barrier();
+        if (w == 2) {
+            float from_start, to_end, whole;
+            dec.ends(lane, &from_start, &to_end, &whole);
+            float* sc = a.sc + vslot * 256;
             sc[lane] = bs[lane];
-            sc[64 + lane] = exp_decay(from_start);
-            sc[128 + lane] = exp_decay(to_end);
-            sc[192 + lane] = exp_decay((dec.block(0) + dec.block(1)) + (dec.block(2) + dec.block(3)));
+            (sc + 64)[lane] = from_start;
+            (sc + 128)[lane] = to_end;
+            (sc + 192)[lane] = whole;
         }
+        // A to LDS, P to memory: row 16 tm + j, columns 16 tn + 4 q + r
+        f32x4 P[3];
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-            if (nt > w) continue;
-            const f32x4 decay = dec.tile(w, nt, j, q);
+        for (int t = 0; t < 3; ++t) {
+            P[t] = splat4(0.f);
+            if (t >= count) continue;
+            const f32x4 e = dec.columns(tm[t], tn[t], j, q), b = *(const f32x4*)&bs[16 * tn[t] + 4 * q];
+            const bool diagonal = tm[t] == tn[t];
+            f32x4 A;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int i = 16 * w + 4 * q + r, col = 16 * nt + j;
-                amat[i * kTriStride + col] = col < i ? beta_of(bs[col]) * (kk[nt][r] * decay[r]) : 0.f;
-                pmat[i * kTriStride + col] = col <= i ? qk[nt][r] * decay[r] : 0.f;
+                A[r] = diagonal && 4 * q + r >= j ? 0.f : beta_of(b[r]) * (kkt[t][r] * e[r]);
+                P[t][r] = diagonal && 4 * q + r > j ? 0.f : qkt[t][r] * e[r];
+            }
+            atile[(tm[t] * (tm[t] + 1) / 2 + tn[t]) * 64 + lane] = A;
+        }
+        auto put_p = [&](int f, const f32x4 lo, const f32x4 hi) {
+            bf16x8 t[PT];
+            split8<PT>(lo, hi, t);
+            bf16x8* const to = a.pf + (vslot * kTriFrags + f) * PT * 64;
+#pragma unroll
+            for (int k = 0; k < PT; ++k) (to + k * 64)[lane] = t[k];
+        };
+        if (w == 0) {
+            put_p(0, P[0], splat4(0.f));
+            put_p(1, P[1], P[2]);
+        } else if (w == 1) {
+            put_p(2, P[0], P[1]);
+            put_p(3, P[2], splat4(0.f));
+        } else {
+            put_p(w + 2, P[0], P[1]);
+        }
+        if constexpr (BWD) {       // P^T: row = token 16 un + j, elements tokens 16 um + 4 q + r
+#pragma unroll
+            for (int t = 0; t < 3; ++t) {
+                P[t] = splat4(0.f);
+                if (t >= count) continue;
+                const f32x4 e = dec.rows(um[t], un[t], j, q);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) P[t][r] = um[t] == un[t] && j > 4 * q + r ? 0.f : qk[t][r] * e[r];
+            }
+            auto put_pt = [&](int f, const f32x4 lo, const f32x4 hi) {
+                bf16x8 t[3];
+                split8<3>(lo, hi, t);
+                bf16x8* const to = a.ptf + (vslot * kTriFrags + f) * 3 * 64;
+#pragma unroll
+                for (int k = 0; k < 3; ++k) (to + k * 64)[lane] = t[k];
+            };
+            const f32x4 none = splat4(0.f);
+            if (w == 0) {
+                put_pt(trt_index(0, 0), P[0], P[1]);
+                put_pt(trt_index(1, 0), none, P[2]);
+            } else if (w == 1) {
+                put_pt(trt_index(1, 1), P[0], P[1]);
+                put_pt(trt_index(3, 1), none, P[2]);
+            } else {
+                put_pt(w == 2 ? trt_index(0, 1) : trt_index(2, 1), P[0], P[1]);
             }
         }
-        __syncthreads();
-        // T = (I + A)^-1: the 16 x 16 diagonal blocks by forward substitution, column j of block w in every lane quarter
-        float x[16];
+        lds_barrier();
+        // T = (I + A)^-1: the 16 x 16 diagonal blocks by forward substitution, column j of block w in every lane quarter.  Four
+        // rows at a time: solved one after the other, then taken out of all rows below.
+        f32x4 tcol[4];
+        {
+            const f32x4* const from = atile + (w * (w + 1) / 2 + w) * 64;
+            float x[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float v = i == j ? 1.f : 0.f;
+            for (int i = 0; i < 16; ++i) x[i] = i == j ? 1.f : 0.f;
 #pragma unroll
             for (int m4 = 0; m4 < 4; ++m4) {
-                if (4 * m4 < i) {
-                    const f32x4 arow = amat4[((16 * w + i) * kTriStride + 16 * w) / 4 + m4];
+                f32x4 row[16];
 #pragma unroll
-                    for (int m = 0; m < 4; ++m)
-                        if (4 * m4 + m < i) v -= arow[m] * x[4 * m4 + m];
-                }
+                for (int i = 0; i < 16; ++i)
+                    if (i > 4 * m4) row[i] = from[16 * m4 + i];
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (i > 4 * m4 + m) x[i] -= row[i][m] * x[4 * m4 + m];
             }
-            x[i] = v;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float x0 = x[r], x1 = x[4 + r], x2 = x[8 + r], x3 = x[12 + r];
+                asm("" : "+v"(x0), "+v"(x1), "+v"(x2), "+v"(x3));      // (values: a choice of addresses would put x in memory)
+                tcol[0][r] = q < 2 ? (q == 0 ? x0 : x1) : (q == 2 ? x2 : x3);
+            }
         }
+        // a tile of T (lane = column, rows 4 q + r) as a left-hand operand
+        auto put_t = [&](int id, const f32x4 x) {
+            float* const to = (float*)(ttile + id * kTile + (j >> 2) * 17 + 4 * q) + (j & 3);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if ((i >> 2) == q) tmat[(16 * w + i) * kTriStride + 16 * w + j] = x[i];
-        __syncthreads();
+            for (int r = 0; r < 4; ++r) to[4 * r] = x[r];
+        };
+        put_t(w * (w + 1) / 2 + w, tcol[0]);
+        lds_barrier();
         // below the diagonal: T_iw = -T_ii sum_m A_im T_mw, wave w its block column, on the exact fp32 MFMA
-        f32x4 tcol[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) tcol[0][r] = tmat[(16 * w + 4 * q + r) * kTriStride + 16 * w + j];
 #pragma unroll
         for (int di = 1; di < 4; ++di) {
             if (w + di > 3) continue;
-            const int i = w + di;
+            const int i = w + di, row = i * (i + 1) / 2;
             f32x4 acc = splat4(0.f);
 #pragma unroll
             for (int m = 0; m < di; ++m) {
-                const f32x4 arow = amat4[((16 * i + j) * kTriStride + 16 * (w + m) + 4 * q) / 4];
+                const f32x4 arow = atile[(row + w + m) * 64 + lane];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc = mfma4(arow[r], tcol[m][r], acc);
             }
-            const f32x4 trow = tmat4[((16 * i + j) * kTriStride + 16 * i + 4 * q) / 4];
+            const f32x4 trow = ttile[(row + i) * kTile + 17 * q + j];
             f32x4 res = splat4(0.f);
 #pragma unroll
             for (int r = 0; r < 4; ++r) res = mfma4(trow[r], acc[r], res);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                tcol[di][r] = -res[r];
-                tmat[(16 * i + 4 * q + r) * kTriStride + 16 * w + j] = -res[r];
-            }
-        }
-        __syncthreads();
-        // T and P as A operands of the chain
-        const size_t at = (size_t)(slot * (size_t)a.hv + hv) * kTriFrags;
-        for (int f = w; f < 2 * kTriFrags; f += 4) {
-            const bool isp = f >= kTriFrags;
-            const int ff = isp ? f - kTriFrags : f;
-            const int mt = tri_row(ff), ks = tri_step(ff);
-            const f32x4* m4 = (isp ? pmat4 : tmat4) + ((16 * mt + j) * kTriStride + 32 * ks + 4 * q) / 4;
-            const f32x4 lo = m4[0], hi = (mt & 1) || ks < (mt >> 1) ? m4[4] : splat4(0.f);
-            bf16x8 t[3];
-            split8<3>(lo, hi, t);
-            if (isp) {
-#pragma unroll
-                for (int k = 0; k < PT; ++k) a.pf[((at + ff) * PT + k) * 64 + lane] = t[k];
-            } else {
-#pragma unroll
-                for (int k = 0; k < 3; ++k) a.tf[((at + ff) * 3 + k) * 64 + lane] = t[k];
-            }
+            for (int r = 0; r < 4; ++r) tcol[di][r] = -res[r];
+            put_t(row + w, tcol[di]);
         }
         if constexpr (BWD) {
-            for (int f = w; f < 2 * kTriFrags; f += 4) {
-                const bool isp = f >= kTriFrags;
-                const int ff = isp ? f - kTriFrags : f;
-                const int mt = trt_row(ff), ks = trt_step(ff);
-                const float* src = isp ? pmat : tmat;
-                f32x4 lo, hi;
-                const bool half = (mt & 1) && ks == (mt >> 1);      // the first half lies above the diagonal's block
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    lo[e] = half ? 0.f : src[(32 * ks + 4 * q + e) * kTriStride + 16 * mt + j];
-                    hi[e] = src[(32 * ks + 16 + 4 * q + e) * kTriStride + 16 * mt + j];
-                }
+            auto put_tt = [&](int ks, const f32x4 lo, const f32x4 hi) {
                 bf16x8 t[3];
                 split8<3>(lo, hi, t);
+                bf16x8* const to = a.ttf + (vslot * kTriFrags + trt_index(w, ks)) * 3 * 64;
 #pragma unroll
-                for (int k = 0; k < 3; ++k) (isp ? a.ptf : a.ttf)[((at + ff) * 3 + k) * 64 + lane] = t[k];
+                for (int k = 0; k < 3; ++k) (to + k * 64)[lane] = t[k];
+            };
+            const f32x4 none = splat4(0.f);
+            if (w == 0) {
+                put_tt(0, tcol[0], tcol[1]);
+                put_tt(1, tcol[2], tcol[3]);
+            } else if (w == 1) {
+                put_tt(0, none, tcol[0]);
+                put_tt(1, tcol[1], tcol[2]);
+            } else if (w == 2) {
+                put_tt(1, tcol[0], tcol[1]);
+            } else {
+                put_tt(1, none, tcol[0]);
             }
+        }
+        lds_barrier();
+        for (int f = w; f < kTriFrags; f += 4) {
+            const int mt = tri_row(f), nt = 2 * tri_step(f), id = mt * (mt + 1) / 2 + nt;
+            const f32x4 x0 = ttile[id * kTile + 17 * q + j], x1 = nt + 1 <= mt ? ttile[(id + 1) * kTile + 17 * q + j] : splat4(0.f);
+            bf16x8 t[3];
+            split8<3>(x0, x1, t);
+            bf16x8* const to = a.tf + (vslot * kTriFrags + f) * 3 * 64;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) (to + k * 64)[lane] = t[k];
         }
     }
 }
@@ -546,12 +678,6 @@ template <int N, int NC>
 __device__ __forceinline__ void shared_frag(const bf16x8* buf, int ks, int nc, int lane, bf16x8 (&b)[N]) {
 #pragma unroll
     for (int n = 0; n < N; ++n) b[n] = buf[((ks * N + n) * NC + nc) * 64 + lane];
-}
-// LDS writes of every wave are visible behind this; loads from memory stay in flight over it
-__device__ __forceinline__ void lds_barrier() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 // loads stay above this (they are issued here, and not where their values are first needed)
 __device__ __forceinline__ void issue_loads() { asm volatile("" ::: "memory"); }

@@ -262,8 +262,8 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
     const int j = lane & 15, q = lane >> 4;
     const int p = w % NP, mh = w / NP;
     const int slot = blockIdx.x / a.hk, h = blockIdx.x % a.hk;
-    const int s = sequence_of(a, slot, lane);
-    const Span sp = span_of(a, s);
+    Span sp;
+    const int s = sequence_of(a, slot, lane, &sp);
     const int c = slot - sp.slot;
     const int start = sp.begin + c * kDeltaChunk;
     const int n = min(kDeltaChunk, sp.begin + sp.len - start);
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
         const int lane = in_block(lane0), j = lane & 15, q = lane >> 4;     // (nothing of a head's addresses is kept over the loop)
         const int srow = 16 * (w & 3) + j;
         const size_t vslot = (size_t)slot * a.hv + hv;
-        __syncthreads();
+        lds_barrier();
         if (w == 0) {
             const bool in = lane < n;
             dec.set(lane, in ? a.g[(start + lane) * a.g_t + hv * a.g_h] : 0.f);
@@ -439,12 +439,12 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
             if (lane == 0) gamma[p] = dots;
         }
         // the 64 x 64 gradients, in the stage's place
-        __syncthreads();
+        lds_barrier();
         {
 #pragma unroll
             for (int t = 0; t < TPW; ++t) {
                 if (!own[t]) continue;
-                const f32x4 decay = dec.tile(tm[t], tn[t], j, q);
+                const f32x4 decay = dec.rows(tm[t], tn[t], j, q);
                 const int col = 16 * tn[t] + j;
                 const float beta = bs[col], beta1 = beta_of(beta);
 #pragma unroll
@@ -490,7 +490,7 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
                 }
             }
         }
-        __syncthreads();
+        lds_barrier();
         // A operands of the products with K and Q: G + G^T (8 fragments), H, H^T
         for (int f = w; f < 8 + 2 * kTriFrags; f += W) {
             f32x4 lo, hi;
@@ -529,7 +529,7 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
             }
             part[w][lane] = below;
         }
-        __syncthreads();
+        lds_barrier();
         // dQ += H K,  dK += (G + G^T) K + H^T Q
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -566,7 +566,8 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
                 g += sums[1][k][lane];
                 hold += gamma[k];
             }
-            float mine = sum_from(f, lane) + sum_before(g, lane) + scl[64 + 63] * hold;
+            const float whole = dec.block(0) * dec.block(1) * dec.block(2) * dec.block(3);
+            float mine = sum_from(f, lane) + sum_before(g, lane) + whole * hold;
 #pragma unroll
             for (int m = 0; m < RB; ++m) {
                 const float x = sum64(lane < RB * w + m ? run[m] + below : 0.f);
