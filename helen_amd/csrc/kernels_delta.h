@@ -358,12 +358,17 @@ constexpr int kTriStride = 68;    // floats per row of a 64 x 64 matrix in LDS: 
 // fragments.  K^T comes from the matrix pipe too: K times a selection of 16 columns is K's tile with lane = dk.
 // ------------------------------------------------------------------------------------------------
 template <typename In, int DK, int PT, bool BWD>
-__global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_prep_kernel(const DeltaArgs a) {
+__global__ __launch_bounds__(256, In::kTerms == 1 ? (BWD ? 3 : 4) : 1) void delta_prep_kernel(const DeltaArgs a) {
     constexpr int NI = In::kTerms, KS = DK / 32;
     constexpr int kTile = 64 + 4;               // an operand tile in LDS: [column / 4][row] x 4, column groups 17 apart
     typedef typename In::raw raw;
-    __shared__ bf16x8 kfr[4 * KS * NI * 64], qfr[4 * KS * NI * 64];
-    __shared__ f32x4 atile[10 * 64], ttile[10 * kTile];
+    // K and Q of all rows; later, in their place, A and T (three or four workgroups fit a CU)
+    constexpr int kRows = 4 * KS * NI * 64, kTiles = 10 * 64 + 10 * kTile;
+    __shared__ f32x4 pool[2 * kRows > kTiles ? 2 * kRows : kTiles];
+    bf16x8* const kfr = (bf16x8*)pool;
+    bf16x8* const qfr = kfr + kRows;
+    f32x4* const atile = pool;
+    f32x4* const ttile = pool + 10 * 64;
     __shared__ __attribute__((aligned(16))) Decays dec;
     __shared__ __attribute__((aligned(16))) float bs[64];
     const int lane0 = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
