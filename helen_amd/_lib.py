@@ -186,19 +186,20 @@ def load(with_torch=True):
     lib.helen_polish_slot_wait.argtypes = [vp]
     sz = ctypes.POINTER(ctypes.c_size_t)
     lib.helen_delta_rule_bytes.restype = ci
-    lib.helen_delta_rule_bytes.argtypes = [ctypes.POINTER(HelenDeltaRuleC), sz, sz, sz]
+    # (descriptions go as void*: a ctypes structure by reference, or its packed bytes -- helen_amd.sequence_ops)
+    lib.helen_delta_rule_bytes.argtypes = [vp, sz, sz, sz]
     lib.helen_delta_rule_forward.restype = ci
-    lib.helen_delta_rule_forward.argtypes = [ctypes.POINTER(HelenDeltaRuleC), ci, vp, ctypes.c_size_t, vp]
+    lib.helen_delta_rule_forward.argtypes = [vp, ci, vp, ctypes.c_size_t, vp]
     lib.helen_delta_rule_backward.restype = ci
-    lib.helen_delta_rule_backward.argtypes = [ctypes.POINTER(HelenDeltaRuleC), vp, ctypes.c_size_t, vp, ctypes.c_size_t, vp]
+    lib.helen_delta_rule_backward.argtypes = [vp, vp, ctypes.c_size_t, vp, ctypes.c_size_t, vp]
     lib.helen_delta_rule_step.restype = ci
-    lib.helen_delta_rule_step.argtypes = [ctypes.POINTER(HelenDeltaStepC), vp]
+    lib.helen_delta_rule_step.argtypes = [vp, vp]
     lib.helen_layer_norm_forward.restype = ci
-    lib.helen_layer_norm_forward.argtypes = [ctypes.POINTER(HelenLayerNormC), vp]
+    lib.helen_layer_norm_forward.argtypes = [vp, vp]
     lib.helen_layer_norm_bytes.restype = ci
-    lib.helen_layer_norm_bytes.argtypes = [ctypes.POINTER(HelenLayerNormC), sz]
+    lib.helen_layer_norm_bytes.argtypes = [vp, sz]
     lib.helen_layer_norm_backward.restype = ci
-    lib.helen_layer_norm_backward.argtypes = [ctypes.POINTER(HelenLayerNormC), vp, ctypes.c_size_t, vp]
+    lib.helen_layer_norm_backward.argtypes = [vp, vp, ctypes.c_size_t, vp]
     got = lib.helen_abi_version()
     if got != HELEN_ABI_VERSION:
         raise ImportError("libhelen_hip.so ABI %d != binding ABI %d; rebuild" % (got, HELEN_ABI_VERSION))

@@ -120,19 +120,24 @@ __device__ __forceinline__ f32x4 load4(const typename In::raw* p) {
 template <typename In, int NC>
 struct Columns {
     typedef typename In::raw raw;
-    typedef raw vec __attribute__((ext_vector_type(NC), aligned(sizeof(raw))));
+    typedef raw vec __attribute__((ext_vector_type(NC)));
+    typedef vec vec_any __attribute__((aligned(sizeof(raw))));      // rows may begin anywhere
     vec v;
-    static __device__ __forceinline__ Columns load(const raw* p) { return {*(const vec*)p}; }
+    static __device__ __forceinline__ Columns load(const raw* p) { return {*(const vec_any*)p}; }
     __device__ __forceinline__ float get(int nc) const { return In::to_f32(v[nc]); }
     static __device__ __forceinline__ void store(raw* p, const float (&x)[NC]) {
         vec t;
-        if constexpr (In::kTerms == 1 && NC == 2) {      // (one conversion for both)
-            t = __builtin_bit_cast(vec, __builtin_convertvector((f32x2){x[0], x[1]}, bf16x2_t));
+        if constexpr (In::kTerms == 1) {      // (two a conversion)
+            typedef unsigned pairs __attribute__((ext_vector_type(NC / 2)));
+            pairs y;
+#pragma unroll
+            for (int p = 0; p < NC / 2; ++p) y[p] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){x[2 * p], x[2 * p + 1]}, bf16x2_t));
+            t = __builtin_bit_cast(vec, y);
         } else {
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc) t[nc] = In::from_f32(x[nc]);
         }
-        *(vec*)p = t;
+        *(vec_any*)p = t;
     }
 };
 template <typename In>
@@ -708,6 +713,14 @@ struct ChainAddress {
 #pragma unroll
             for (int t = 0; t < NI; ++t) to[ks][t] = (from + (ks * NI + t) * 64)[lane];
     }
+    // the same with the k steps in the order first, first + 1, ..: to[i] is step (first + i) % (DK / 32)
+    __device__ __forceinline__ void rows_from(int first, const bf16x8* from, int c, bf16x8 (&to)[DK / 32][NI]) const {
+        from += (kslot + (size_t)c * hk) * kSlot + w * (DK / 32) * NI * 64;
+#pragma unroll
+        for (int i = 0; i < DK / 32; ++i)
+#pragma unroll
+            for (int t = 0; t < NI; ++t) to[i][t] = (from + (((first + i) & (DK / 32 - 1)) * NI + t) * 64)[lane];
+    }
     // the wave's dk tiles of K^T or Q^T
     __device__ __forceinline__ void columns(const bf16x8* from, int c, bf16x8 (&to)[DK / 64][2][NI]) const {
         from += (kslot + (size_t)c * hk) * kSlot + w * (DK / 64) * 2 * NI * 64;
@@ -989,13 +1002,275 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
     }
 }
 
-// column tiles of 16 a chain's workgroup takes
-inline int chain_tiles(const DeltaArgs& a) {
-    const long one = (long)a.nseq * a.hv * (a.dv_width / 16);
-    return one >= 1024 ? 2 : 1;
+// ------------------------------------------------------------------------------------------------
+// The same for few long chains: 16 columns of the state, and eight waves.  A wave alone on its SIMD issues an instruction
+// every 5 to 9 cycles, and the chain is as long as what its waves have to issue; so waves 0 .. 3 do only what the next chunk
+// waits for (R, E and S), and waves 4 .. 7, one on each SIMD beside them, the output and every store: from S, E and U as they
+// pass by in LDS, a phase later.
+// ------------------------------------------------------------------------------------------------
+// Fetches a chunk's fragments into the XCD's L2 before the workgroups of its head need them.  They all come by at the same time, and
+// loads that miss there run at half the rate of loads that hit (28 - 35 against 16 cycles a KiB and CU).  Each of the head's
+// waves takes another part: one load, a lane a line of 128 bytes.  The value is handed to `settle` a chunk later.
+struct Piece {
+    const bf16x8* at;
+    int kib;
+};
+template <int N>
+__device__ __forceinline__ unsigned fetch(const Piece (&piece)[N], int part, int lane) {
+    int line = part * 64 + lane;
+    const char* from = (const char*)piece[N - 1].at + 1024 * (piece[N - 1].kib - 1);     // (parts behind the end: a line again)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (line >= 0 && line < 8 * piece[i].kib) from = (const char*)piece[i].at + 128 * line;
+        line -= 8 * piece[i].kib;
+    }
+    return *(const unsigned*)from;
 }
-inline unsigned chain_grid(const DeltaArgs& a, int tiles) {
-    return (unsigned)(((long)a.nseq * a.hv * (a.dv_width / (16 * tiles)) + 7) / 8 * 8);
+__device__ __forceinline__ void settle(unsigned x) { asm volatile("" ::"v"(x)); }
+constexpr int kFetchAhead = 3;
+
+// loads and matrix products by turns: a load is issued while the pipe works on the product before it
+template <int N>
+__device__ __forceinline__ void between_products() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
+    }
+}
+
+// Before a loop whose loads are a turn ahead: nothing is in flight here, so that the compiler's counts inside it are those of the
+// loop alone (it waits for what any path into the loop might have left).
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
+template <typename In, int DK, int PT, bool KEEP>
+__global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs a) {
+    constexpr int NI = In::kTerms, KS = DK / 32, MW = DK / 64;
+    constexpr bool OWN = MW == 2;        // a wave's rows of S are a whole k step: it takes that one from its registers
+    typedef typename In::raw raw;
+    __shared__ bf16x8 sbuf[KS * 3 * 64], xbuf[2 * 3 * 64], ubuf[2 * PT * 64], cbuf[2 * 3 * 64];
+    __shared__ f32x4 ebuf[4 * 64], sfull[KEEP ? 4 * MW * 64 : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+    const int j = lane & 15, q = lane >> 4;
+    const int groups = a.dv_width / 16;
+    const unsigned item = xcd_order(blockIdx.x, gridDim.x);
+    if (item >= (unsigned)a.nseq * a.hv * groups) return;
+    const int hv = item / groups % a.hv, s = item / groups / a.hv, h = hv / a.group;
+    const int col = 16 * (item % groups) + j;
+    const Span sp = span_of(a, s);
+    const int chunks = (sp.len + kDeltaChunk - 1) / kDeltaChunk;
+    const int row = 16 * w + 4 * q;
+    const ChainAddress<In, DK> at(a, sp, h, hv, w, lane);
+    unsigned tile_at[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) tile_at[r] = (4 * q + r) * a.dv_width + col;
+
+    if (wave < 4) {
+        f32x4 S[MW][1];
+        load_state<MW, 1>(a.s0, a.zeros, (((size_t)s * a.hv + hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col, a.dv_width, S);
+        struct Operands {        // of one chunk; the next one's are loaded into a second set meanwhile
+            bf16x8 kf[KS][NI], kt[MW][2][NI], tf[2][3];
+            f32x4 beta, eb, ec, whole;
+            Columns<In, 1> v[4];
+        } first, second;
+        bf16x8 own[3];
+        RowOffsets vrow(a.v_t, row, col);
+        auto load_k = [&](int c, Operands& to) { at.rows_from(OWN ? w : 0, a.kf, c, to.kf); };
+        auto load_tokens = [&](int c, Operands& to) {
+            const float* sc = a.sc + (at.vslot + (size_t)c * a.hv) * 256;
+            to.eb = *(const f32x4*)(sc + 64 + row);
+            vrow.clamp(sp.len - c * kDeltaChunk);
+            const raw* p = (const raw*)a.v + (sp.begin + c * kDeltaChunk) * a.v_t + hv * a.v_h;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) to.v[r] = Columns<In, 1>::load(p + vrow.at[r]);
+        };
+        auto load_scales = [&](int c, Operands& to) {
+            const float* sc = a.sc + (at.vslot + (size_t)c * a.hv) * 256;
+            to.beta = *(const f32x4*)(sc + row);
+            to.ec = *(const f32x4*)(sc + 128 + row);
+            to.whole = *(const f32x4*)(sc + 192 + row);
+        };
+        auto share_state = [&]() {
+            if constexpr (OWN) {
+                split8<3>(S[0][0], S[1][0], own);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) sbuf[(w * 3 + k) * 64 + lane] = own[k];
+            } else {
+                share_tile<3, 1>(sbuf, w, 0, lane, S[0][0]);
+            }
+            if constexpr (KEEP) {
+#pragma unroll
+                for (int i = 0; i < MW; ++i) sfull[(MW * w + i) * 64 + lane] = S[i][0];
+            }
+        };
+        auto step = [&](int c, Operands& now, Operands& then) {
+            const int next = min(c + 1, chunks - 1);
+            f32x4 sum[2] = {splat4(0.f), splat4(0.f)}, R;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                bf16x8 b[3];
+                if (OWN && i == 0) {
+#pragma unroll
+                    for (int t = 0; t < 3; ++t) b[t] = own[t];
+                } else {
+                    shared_frag<3, 1>(sbuf, OWN ? (w + i) & 3 : i, 0, lane, b);
+                }
+                sum[i & 1] = mm(now.kf[i], b, sum[i & 1]);
+            }
+            load_k(next, then);
+            load_tokens(next, then);
+            between_products<KS * 3>();
+#pragma unroll
+            for (int r = 0; r < 4; ++r) R[r] = now.v[r].get(0) - now.eb[r] * (sum[0][r] + sum[1][r]);
+            share_tile<3, 1>(xbuf, w, 0, lane, R);
+            issue_loads();
+            lds_barrier();
+            bf16x8 x[2][3];
+            shared_frag<3, 1>(xbuf, 0, 0, lane, x[0]);
+            shared_frag<3, 1>(xbuf, 1, 0, lane, x[1]);
+            f32x4 e0 = splat4(0.f), e1 = splat4(0.f);
+            e0 = mm(now.tf[0], x[0], e0);
+            e1 = mm(now.tf[1], x[1], e1);
+            at.template triangle<3>(a.tf, next, then.tf);
+            load_scales(next, then);
+            between_products<12>();
+            f32x4 E = e0 + e1;
+            ebuf[w * 64 + lane] = E;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) E[r] *= now.beta[r] * now.ec[r];
+            share_tile<3, 1>(cbuf, w, 0, lane, E);
+            issue_loads();
+            lds_barrier();
+            shared_frag<3, 1>(cbuf, 0, 0, lane, x[0]);
+            shared_frag<3, 1>(cbuf, 1, 0, lane, x[1]);
+#pragma unroll
+            for (int i = 0; i < MW; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[i][0][r] *= now.whole[r];
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int i = 0; i < MW; ++i) S[i][0] = mm(now.kt[i][ks], x[ks], S[i][0]);
+            at.columns(a.ktf, next, then.kt);
+            between_products<2 * MW * 3>();
+            share_state();
+            issue_loads();
+            lds_barrier();
+        };
+        if (chunks > 0) {
+            load_k(0, first);
+            load_tokens(0, first);
+            load_scales(0, first);
+            at.template triangle<3>(a.tf, 0, first.tf);
+            at.columns(a.ktf, 0, first.kt);
+            share_state();
+        }
+        lds_barrier();
+        if (chunks & 1) {
+            step(0, first, second);
+            first = second;
+        }
+        loads_done();
+        for (int c = chunks & 1; c < chunks; c += 2) {
+            step(c, first, second);
+            step(c + 1, second, first);
+        }
+        if (a.s1) {
+            float* const to = a.s1 + (((size_t)s * a.hv + hv) * DK + 16 * MW * w) * a.dv_width;
+#pragma unroll
+            for (int i = 0; i < MW; ++i) store_tile<1>(to + (size_t)16 * i * a.dv_width, tile_at, S[i]);
+        }
+    } else {
+        // The output transposed, S^T Q^T and U^T P^T (the operands change places, the fragments are the same): a lane then has
+        // four neighbouring columns of one token, one store of a chunk
+        bf16x8 qf[KS][NI], pf[2][PT];
+        f32x4 beta, O = splat4(0.f);
+        float eb = 0.f;
+        const int token = 16 * w + j;
+        const unsigned o_at = token * (unsigned)a.o_t + col - j + 4 * q;
+        auto load_scales = [&](int c) {
+            const float* sc = a.sc + (at.vslot + (size_t)c * a.hv) * 256;
+            beta = *(const f32x4*)(sc + row);
+            eb = (sc + 64)[token];
+        };
+        // o of chunk c: O + P U, and its store
+        auto finish = [&](int c) {
+            bf16x8 x[2][PT];
+            shared_frag<PT, 1>(ubuf, 0, 0, lane, x[0]);
+            shared_frag<PT, 1>(ubuf, 1, 0, lane, x[1]);
+            f32x4 p0 = splat4(0.f);
+            p0 = mm<PT, PT, PT - 1>(x[0], pf[0], p0);
+            O = mm<PT, PT, PT - 1>(x[1], pf[1], O) + p0;
+            raw* const to = (raw*)a.o + (sp.begin + c * kDeltaChunk) * a.o_t + hv * a.o_h;
+            const float y[4] = {a.scale * O[0], a.scale * O[1], a.scale * O[2], a.scale * O[3]};
+            if (token < sp.len - c * kDeltaChunk) Columns<In, 4>::store(to + o_at, y);
+        };
+        const int part = 4 * (item % groups) + w;
+        auto fetch_chunk = [&](int c) {
+            const bf16x8* const tri = a.tf + (at.vslot + (size_t)c * a.hv) * kTriFrags * 3 * 64;
+            const bf16x8* const pri = a.pf + (at.vslot + (size_t)c * a.hv) * kTriFrags * PT * 64;
+            const size_t k0 = (at.kslot + (size_t)c * a.hk) * at.kSlot;
+            const Piece piece[5] = {{a.kf + k0, DK / 8 * NI}, {tri, kTriFrags * 3}, {a.ktf + k0, DK / 8 * NI}, {a.qf + k0, DK / 8 * NI}, {pri, kTriFrags * PT}};
+            return fetch(piece, part, lane);
+        };
+        unsigned fetched = 0;
+        if (chunks > 0) {
+            at.rows(a.qf, 0, qf);
+            load_scales(0);
+            settle(fetch_chunk(min(1, chunks - 1)));
+            settle(fetch_chunk(min(2, chunks - 1)));
+        }
+        lds_barrier();
+        for (int c = 0; c < chunks; ++c) {
+            const int next = min(c + 1, chunks - 1);
+            settle(fetched);
+            fetched = fetch_chunk(min(c + kFetchAhead, chunks - 1));
+            if (c > 0) finish(c - 1);
+            at.template triangle<PT>(a.pf, c, pf);
+            issue_loads();
+            lds_barrier();
+            // (the terms of S that a product of PT terms an operand takes)
+            f32x4 sum[2] = {splat4(0.f), splat4(0.f)};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                bf16x8 b[PT];
+#pragma unroll
+                for (int t = 0; t < PT; ++t) b[t] = sbuf[(ks * 3 + t) * 64 + lane];
+                sum[ks & 1] = mm(b, qf[ks], sum[ks & 1]);
+            }
+            if constexpr (KEEP) {
+                float* const to = a.states + ((at.vslot + (size_t)c * a.hv) * DK + 16 * MW * w) * a.dv_width;
+#pragma unroll
+                for (int i = 0; i < MW; ++i) {
+                    const f32x4 x[1] = {sfull[(MW * w + i) * 64 + lane]};
+                    store_tile<1>(to + (size_t)16 * i * a.dv_width, tile_at, x);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) O[r] = eb * (sum[0][r] + sum[1][r]);
+            const f32x4 step = beta;
+            at.rows(a.qf, next, qf);
+            load_scales(next);
+            issue_loads();
+            lds_barrier();
+            f32x4 U = ebuf[w * 64 + lane];
+            if constexpr (KEEP) {
+                const f32x4 x[1] = {U};
+                store_tile<1>(a.e + ((at.vslot + (size_t)c * a.hv) * kDeltaChunk + 16 * w) * a.dv_width, tile_at, x);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) U[r] *= step[r];
+            share_tile<PT, 1>(ubuf, w, 0, lane, U);
+            lds_barrier();
+        }
+        if (chunks > 0) finish(chunks - 1);
+    }
+}
+
+// Which of the two: below this number of 16-column chains the eight-wave kernel
+inline bool chains_are_few(const DeltaArgs& a) { return (long)a.nseq * a.hv * (a.dv_width / 16) < 1024; }
+inline unsigned chain_grid(const DeltaArgs& a, int columns) {
+    return (unsigned)(((long)a.nseq * a.hv * (a.dv_width / columns) + 7) / 8 * 8);
 }
 
 }  // namespace helen

@@ -211,6 +211,249 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
     }
 }
 
+// The reverse chain for few long ones, as delta_forward_long_kernel: waves 0 .. 3 do what the next chunk waits for, waves 4 .. 7
+// what comes from dO alone, one chunk ahead (P^T dO and Q^T (scale e^b dO), handed over as fp32 tiles), and the stores.
+template <typename In, int DK>
+__global__ __launch_bounds__(512) void delta_backward_long_kernel(const DeltaArgs a) {
+    constexpr int NI = In::kTerms, KS = DK / 32, MW = DK / 64;
+    constexpr bool OWN = MW == 2;
+    typedef typename In::raw raw;
+    __shared__ bf16x8 sbuf[KS * 3 * 64], ybuf[2 * NI * 64], wbuf[2 * 3 * 64], dbuf[2 * 3 * 64], zbuf[2 * 3 * 64];
+    __shared__ f32x4 pfull[4 * 64], wfull[4 * MW * 64], zfull[4 * 64], sfull[4 * MW * 64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+    const int j = lane & 15, q = lane >> 4;
+    const int groups = a.dv_width / 16;
+    const unsigned item = xcd_order(blockIdx.x, gridDim.x);
+    if (item >= (unsigned)a.nseq * a.hv * groups) return;
+    const int hv = item / groups % a.hv, s = item / groups / a.hv, h = hv / a.group;
+    const int col = 16 * (item % groups) + j;
+    const Span sp = span_of(a, s);
+    const int chunks = (sp.len + kDeltaChunk - 1) / kDeltaChunk;
+    const int row = 16 * w + 4 * q;
+    const ChainAddress<In, DK> at(a, sp, h, hv, w, lane);
+    unsigned tile_at[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) tile_at[r] = (4 * q + r) * a.dv_width + col;
+
+    if (wave < 4) {
+        f32x4 S[MW][1];
+        load_state<MW, 1>(a.ds1, a.zeros, (((size_t)s * a.hv + hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col, a.dv_width, S);
+        struct Operands {
+            bf16x8 kf[KS][NI], kt[MW][2][NI], tt[2][3];
+            f32x4 beta, eb, ec, whole;
+        } first, second;
+        bf16x8 own[3];
+        auto load_k = [&](int c, Operands& to) {
+            const float* sc = a.sc + (at.vslot + (size_t)c * a.hv) * 256;
+            at.rows_from(OWN ? w : 0, a.kf, c, to.kf);
+            to.beta = *(const f32x4*)(sc + row);
+            to.ec = *(const f32x4*)(sc + 128 + row);
+        };
+        auto load_scales = [&](int c, Operands& to) {
+            const float* sc = a.sc + (at.vslot + (size_t)c * a.hv) * 256;
+            to.eb = *(const f32x4*)(sc + 64 + row);
+            to.whole = *(const f32x4*)(sc + 192 + row);
+        };
+        auto share_state = [&]() {
+            if constexpr (OWN) {
+                split8<3>(S[0][0], S[1][0], own);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) sbuf[(w * 3 + k) * 64 + lane] = own[k];
+            } else {
+                share_tile<3, 1>(sbuf, w, 0, lane, S[0][0]);
+            }
+#pragma unroll
+            for (int i = 0; i < MW; ++i) sfull[(MW * w + i) * 64 + lane] = S[i][0];
+        };
+        auto step = [&](int c, Operands& now, Operands& then) {
+            const int next = max(c - 1, 0);
+            f32x4 sum[2] = {splat4(0.f), splat4(0.f)}, D;
+            const f32x4 p = pfull[w * 64 + lane];
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                bf16x8 b[3];
+                if (OWN && i == 0) {
+#pragma unroll
+                    for (int t = 0; t < 3; ++t) b[t] = own[t];
+                } else {
+                    shared_frag<3, 1>(sbuf, OWN ? (w + i) & 3 : i, 0, lane, b);
+                }
+                sum[i & 1] = mm(now.kf[i], b, sum[i & 1]);
+            }
+            load_k(next, then);
+            between_products<KS * 3>();
+#pragma unroll
+            for (int r = 0; r < 4; ++r) D[r] = beta_of(now.beta[r]) * (now.ec[r] * (sum[0][r] + sum[1][r]) + a.scale * p[r]);
+            share_tile<3, 1>(dbuf, w, 0, lane, D);
+            issue_loads();
+            lds_barrier();
+            bf16x8 x[2][3];
+            shared_frag<3, 1>(dbuf, 0, 0, lane, x[0]);
+            shared_frag<3, 1>(dbuf, 1, 0, lane, x[1]);
+            f32x4 z0 = splat4(0.f), z1 = splat4(0.f);
+            z0 = mm(now.tt[0], x[0], z0);
+            z1 = mm(now.tt[1], x[1], z1);
+            at.transposed(a.ttf, next, then.tt);
+            load_scales(next, then);
+            between_products<12>();
+            f32x4 Z = z0 + z1;
+            zfull[w * 64 + lane] = Z;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) Z[r] *= -now.eb[r];
+            share_tile<3, 1>(zbuf, w, 0, lane, Z);
+            issue_loads();
+            lds_barrier();
+            shared_frag<3, 1>(zbuf, 0, 0, lane, x[0]);
+            shared_frag<3, 1>(zbuf, 1, 0, lane, x[1]);
+#pragma unroll
+            for (int i = 0; i < MW; ++i) {
+                const f32x4 y = wfull[(MW * w + i) * 64 + lane];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[i][0][r] = now.whole[r] * S[i][0][r] + y[r];
+            }
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int i = 0; i < MW; ++i) S[i][0] = mm(now.kt[i][ks], x[ks], S[i][0]);
+            at.columns(a.ktf, next, then.kt);
+            between_products<2 * MW * 3>();
+            share_state();
+            issue_loads();
+            lds_barrier();
+        };
+        if (chunks > 0) {
+            load_k(chunks - 1, first);
+            load_scales(chunks - 1, first);
+            at.transposed(a.ttf, chunks - 1, first.tt);
+            at.columns(a.ktf, chunks - 1, first.kt);
+            share_state();
+        }
+        lds_barrier();
+        lds_barrier();
+        if (chunks & 1) {
+            step(chunks - 1, first, second);
+            first = second;
+        }
+        loads_done();
+        for (int c = (chunks & ~1) - 1; c >= 0; c -= 2) {
+            step(c, first, second);
+            step(c - 1, second, first);
+        }
+        if (a.ds0) {
+            float* const to = a.ds0 + (((size_t)s * a.hv + hv) * DK + 16 * MW * w) * a.dv_width;
+#pragma unroll
+            for (int i = 0; i < MW; ++i) store_tile<1>(to + (size_t)16 * i * a.dv_width, tile_at, S[i]);
+        }
+    } else {
+        bf16x8 qt[MW][2][NI], pt[2][3];
+        f32x4 eb, W[MW];
+        Columns<In, 1> y[4];
+        RowOffsets yrow(a.do_t, row, col);
+        unsigned dv_at[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) dv_at[r] = (row + r) * a.hv * a.dv_width + col;
+        auto load = [&](int c) {
+            eb = *(const f32x4*)(a.sc + (at.vslot + (size_t)c * a.hv) * 256 + 64 + row);
+            yrow.clamp(sp.len - c * kDeltaChunk);
+            const raw* p = (const raw*)a.dout + (sp.begin + c * kDeltaChunk) * a.do_t + hv * a.do_h;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = Columns<In, 1>::load(p + yrow.at[r]);
+        };
+        auto share = [&]() {
+            f32x4 x = {y[0].get(0), y[1].get(0), y[2].get(0), y[3].get(0)};
+            share_tile<NI, 1>(ybuf, w, 0, lane, x);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] *= a.scale * eb[r];
+            share_tile<3, 1>(wbuf, w, 0, lane, x);
+        };
+        auto from_p = [&]() {
+            bf16x8 b[2][NI];
+            shared_frag<NI, 1>(ybuf, 0, 0, lane, b[0]);
+            shared_frag<NI, 1>(ybuf, 1, 0, lane, b[1]);
+            f32x4 p0 = splat4(0.f), p1 = splat4(0.f);
+            p0 = mm(pt[0], b[0], p0);
+            p1 = mm(pt[1], b[1], p1);
+            pfull[w * 64 + lane] = p0 + p1;
+        };
+        auto from_q = [&]() {
+            bf16x8 b[2][3];
+            shared_frag<3, 1>(wbuf, 0, 0, lane, b[0]);
+            shared_frag<3, 1>(wbuf, 1, 0, lane, b[1]);
+#pragma unroll
+            for (int i = 0; i < MW; ++i) {
+                W[i] = splat4(0.f);
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) W[i] = mm(qt[i][ks], b[ks], W[i]);
+            }
+        };
+        if (chunks > 0) {
+            load(chunks - 1);
+            at.transposed(a.ptf, chunks - 1, pt);
+            at.columns(a.qtf, chunks - 1, qt);
+            share();
+        }
+        lds_barrier();
+        if (chunks > 0) {
+            const int next = max(chunks - 2, 0);
+            from_p();
+            from_q();
+            load(next);
+            at.transposed(a.ptf, next, pt);
+            at.columns(a.qtf, next, qt);
+        }
+        issue_loads();
+        lds_barrier();
+        const int part = 4 * (item % groups) + w;
+        unsigned fetched = 0;
+        for (int c = chunks - 1; c >= 0; --c) {
+            const int after = max(c - 2, 0);
+            settle(fetched);
+            {
+                const int ahead = max(c - kFetchAhead - 1, 0);
+                const size_t t0 = (at.vslot + (size_t)ahead * a.hv) * kTriFrags * 3 * 64, k0 = (at.kslot + (size_t)ahead * a.hk) * at.kSlot;
+                const Piece piece[5] = {{a.kf + k0, DK / 8 * NI}, {a.ttf + t0, kTriFrags * 3}, {a.ktf + k0, DK / 8 * NI}, {a.qtf + k0, DK / 8 * NI}, {a.ptf + t0, kTriFrags * 3}};
+                fetched = fetch(piece, part, lane);
+            }
+#pragma unroll
+            for (int i = 0; i < MW; ++i) wfull[(MW * w + i) * 64 + lane] = W[i];
+            share();                        // dO of chunk c - 1
+            load(after);
+            issue_loads();
+            lds_barrier();
+            from_p();
+            at.transposed(a.ptf, after, pt);
+            {
+                float* const to = a.dstates + ((at.vslot + (size_t)c * a.hv) * DK + 16 * MW * w) * a.dv_width;
+#pragma unroll
+                for (int i = 0; i < MW; ++i) {
+                    const f32x4 x[1] = {sfull[(MW * w + i) * 64 + lane]};
+                    store_tile<1>(to + (size_t)16 * i * a.dv_width, tile_at, x);
+                }
+            }
+            issue_loads();
+            lds_barrier();
+            from_q();
+            at.columns(a.qtf, after, qt);
+            {
+                const f32x4 Z[1] = {zfull[w * 64 + lane]};
+                store_tile<1>(a.z + ((at.vslot + (size_t)c * a.hv) * kDeltaChunk + 16 * w) * a.dv_width, tile_at, Z);
+                const int n = sp.len - c * kDeltaChunk;
+                raw* const dv = (raw*)a.dv + ((size_t)(sp.begin + c * kDeltaChunk) * a.hv + hv) * a.dv_width;
+                if (n >= kDeltaChunk) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) dv[dv_at[r]] = In::from_f32(Z[0][r]);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (row + r < n) dv[dv_at[r]] = In::from_f32(Z[0][r]);
+                }
+            }
+            issue_loads();
+            lds_barrier();
+        }
+    }
+}
+
 // sum over the 16 lanes of a quarter, over a wave, and running sums
 __device__ __forceinline__ float sum16(float x) { return dpp_add<0x121>(dpp_add<0x122>(dpp_add<0x124>(dpp_add<0x128>(x)))); }
 __device__ __forceinline__ float sum64(float x) {

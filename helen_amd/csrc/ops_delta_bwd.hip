@@ -8,10 +8,8 @@ namespace {
 
 template <typename In, int DK>
 void launch(const DeltaArgs& a, hipStream_t s) {
-    const int tiles = chain_tiles(a);
-    const dim3 grid(chain_grid(a, tiles));
-    if (tiles == 1) hipLaunchKernelGGL((delta_backward_kernel<In, DK, 1>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((delta_backward_kernel<In, DK, 2>), grid, dim3(256), 0, s, a);
+    if (chains_are_few(a)) hipLaunchKernelGGL((delta_backward_long_kernel<In, DK>), dim3(chain_grid(a, 16)), dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((delta_backward_kernel<In, DK, 2>), dim3(chain_grid(a, 32)), dim3(256), 0, s, a);
     if (a.tokens == 0) return;
     const dim3 chunks((unsigned)a.slots * a.hk), block(DK * 4);
     if (a.group == 1) hipLaunchKernelGGL((delta_grads_kernel<In, DK, false>), chunks, block, 0, s, a);

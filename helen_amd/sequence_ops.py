@@ -9,6 +9,8 @@ A call keeps nothing: workspaces come from torch's allocator, so calls on severa
 captured into a graph.  Nothing here waits for the device.
 """
 import ctypes
+import functools
+import struct
 
 import torch
 
@@ -16,138 +18,182 @@ from . import _lib
 
 _TYPES = {torch.float32: _lib.HELEN_TYPE_FP32, torch.bfloat16: _lib.HELEN_TYPE_BF16, torch.float16: _lib.HELEN_TYPE_FP16}
 
+# The descriptions of include/helen_hip.h in native layout: packed in one go, a quarter of the time of setting a ctypes
+# structure's fields one by one (a single-token call is shorter on the GPU than on the host).
+_RULE = struct.Struct("@N2i 4i 2i i f P 3P 2P 10q P P 2q P P 2q P 3P 3P".replace(" ", ""))
+_STEP = struct.Struct("@N2i 4i 2i f P 3P 2P 10q P q P 2q".replace(" ", ""))
+_NORM = struct.Struct("@N2i i i q f P q 2P P q 2P P q P q 2P".replace(" ", ""))
 
-def _need(ok, message):
-    if not ok:
-        raise ValueError(message)
+
+def _fail(message):
+    raise ValueError(message)
 
 
-def _on_gpu(name, t, device=None):
-    _need(isinstance(t, torch.Tensor), "%s must be a torch tensor" % name)
-    if not t.is_cuda:
+def _gpu_index(name, t):
+    """The device of a call's first tensor."""
+    if not isinstance(t, torch.Tensor):
+        _fail("%s must be a torch tensor" % name)
+    device = t.get_device()
+    if device < 0:
         raise RuntimeError("%s is not on a GPU: the sequence operators need one, there is no CPU fallback" % name)
-    _need(device is None or t.device == device, "%s is on %s, the other tensors on %s" % (name, t.device, device))
+    return device
 
 
-def _stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def _same_gpu(name, t, device):
+    if not isinstance(t, torch.Tensor):
+        _fail("%s must be a torch tensor" % name)
+    at = t.get_device()
+    if at != device:
+        if at < 0:
+            raise RuntimeError("%s is not on a GPU: the sequence operators need one, there is no CPU fallback" % name)
+        _fail("%s is on GPU %d, the other tensors on %d" % (name, at, device))
+
+
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _inner(t, bytes_=0):
     """`t` with a contiguous last dimension and, where `bytes_` is given, base and strides that are multiples of it; a copy if
     it has to be one."""
-    if t.numel() and t.stride(-1) != 1 and t.shape[-1] != 1:
+    strides = t.stride()
+    if strides[-1] != 1 and t.numel() and t.shape[-1] != 1:
         return t.contiguous()
-    if bytes_ and (t.data_ptr() % bytes_ or any(s * t.element_size() % bytes_ for s in t.stride()[:-1]) or t.stride(0) > 1 << 24):
-        return t.clone(memory_format=torch.contiguous_format) if t.is_contiguous() else t.contiguous()
+    if bytes_:
+        size = t.element_size()
+        if t.data_ptr() % bytes_ or strides[0] > 1 << 24 or any(s * size % bytes_ for s in strides[:-1]):
+            return t.clone(memory_format=torch.contiguous_format) if t.is_contiguous() else t.contiguous()
     return t
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _pair(t):
-    return (ctypes.c_int64 * 2)(t.stride(0), t.stride(1))
+    return 0 if t is None else t.data_ptr()
 
 
 def _heads(q, k, v, g, beta):
-    """Types, devices and shapes of a call's tokens: -> (tokens, heads_k, heads_v, width_k, width_v)."""
-    _on_gpu("q", q)
-    for name, t in (("k", k), ("v", v), ("g", g), ("beta", beta)):
-        _on_gpu(name, t, q.device)
-    _need(q.dtype in _TYPES, "q is %s: float32, bfloat16 or float16 are supported" % q.dtype)
-    _need(k.dtype == q.dtype and v.dtype == q.dtype, "q, k, v are %s, %s, %s: one type is needed" % (q.dtype, k.dtype, v.dtype))
-    _need(g.dtype == torch.float32 and beta.dtype == torch.float32, "g and beta must be float32")
-    _need(q.dim() == 3 and v.dim() == 3, "q, k, v must be [tokens, heads, width]")
-    _need(k.shape == q.shape, "k is %s, q %s" % (tuple(k.shape), tuple(q.shape)))
-    n, hk, dk = q.shape
-    hv, dv = v.shape[1:]
-    _need(v.shape[0] == n, "v has %d tokens, q %d" % (v.shape[0], n))
-    _need(tuple(g.shape) == (n, hv) and tuple(beta.shape) == (n, hv),
-          "g and beta must be [%d, %d]: they are %s and %s" % (n, hv, tuple(g.shape), tuple(beta.shape)))
-    _need(dk in (64, 128), "width %d of q and k: 64 and 128 are supported" % dk)
-    _need(dv in (64, 128, 192, 256), "width %d of v: 64, 128, 192 and 256 are supported" % dv)
-    _need(hk > 0 and hv > 0 and hv % hk == 0, "%d value heads do not share %d key heads evenly" % (hv, hk))
-    _need(n < 2 ** 31, "%d tokens in one call" % n)
-    return n, hk, hv, dk, dv
+    """Types, devices and shapes of a call's tokens: -> (device, type, tokens, heads_k, heads_v, width_k, width_v)."""
+    device = _gpu_index("q", q)
+    _same_gpu("k", k, device)
+    _same_gpu("v", v, device)
+    _same_gpu("g", g, device)
+    _same_gpu("beta", beta, device)
+    dtype = q.dtype
+    code = _TYPES.get(dtype)
+    if code is None:
+        _fail("q is %s: float32, bfloat16 or float16 are supported" % dtype)
+    if k.dtype != dtype or v.dtype != dtype:
+        _fail("q, k, v are %s, %s, %s: one type is needed" % (dtype, k.dtype, v.dtype))
+    if g.dtype != torch.float32 or beta.dtype != torch.float32:
+        _fail("g and beta must be float32")
+    shape, v_shape = q.shape, v.shape
+    if len(shape) != 3 or len(v_shape) != 3:
+        _fail("q, k, v must be [tokens, heads, width]")
+    if k.shape != shape:
+        _fail("k is %s, q %s" % (tuple(k.shape), tuple(shape)))
+    n, hk, dk = shape
+    nv, hv, dv = v_shape
+    if nv != n:
+        _fail("v has %d tokens, q %d" % (nv, n))
+    if g.shape != v_shape[:2] or beta.shape != v_shape[:2]:
+        _fail("g and beta must be [%d, %d]: they are %s and %s" % (n, hv, tuple(g.shape), tuple(beta.shape)))
+    if dk not in (64, 128):
+        _fail("width %d of q and k: 64 and 128 are supported" % dk)
+    if dv not in (64, 128, 192, 256):
+        _fail("width %d of v: 64, 128, 192 and 256 are supported" % dv)
+    if hk < 1 or hv < 1 or hv % hk:
+        _fail("%d value heads do not share %d key heads evenly" % (hv, hk))
+    if n >= 2 ** 31:
+        _fail("%d tokens in one call" % n)
+    return device, code, n, hk, hv, dk, dv
 
 
 def _state(name, t, shape, device):
     if t is None:
         return None
-    _on_gpu(name, t, device)
-    _need(t.dtype == torch.float32 and tuple(t.shape) == shape, "%s must be float32 %s" % (name, shape))
+    _same_gpu(name, t, device)
+    if t.dtype != torch.float32 or tuple(t.shape) != shape:
+        _fail("%s must be float32 %s" % (name, shape))
     t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
 
 
 def _output(name, t, shape, dtype, device):
-    _on_gpu(name, t, device)
-    _need(t.dtype == dtype and tuple(t.shape) == shape, "%s must be %s %s" % (name, dtype, shape))
-    _need(t.numel() == 0 or t.stride(-1) == 1, "%s must have a contiguous last dimension" % name)
+    _same_gpu(name, t, device)
+    if t.dtype != dtype or tuple(t.shape) != shape:
+        _fail("%s must be %s %s" % (name, dtype, shape))
+    if t.numel() and t.stride(-1) != 1:
+        _fail("%s must have a contiguous last dimension" % name)
     return t
 
 
+@functools.lru_cache(maxsize=1024)
+def _rule_bytes(code, hk, hv, dk, dv, tokens, sequences):
+    """Workspaces of a call of these sizes: forward, forward that keeps, backward."""
+    op = _lib.HelenDeltaRuleC()
+    op.struct_size = ctypes.sizeof(op)
+    op.dtype, op.heads_k, op.heads_v, op.width_k, op.width_v, op.tokens, op.sequences = code, hk, hv, dk, dv, tokens, sequences
+    op.offsets = 1       # (lengths may differ; not read)
+    got = [ctypes.c_size_t() for _ in range(3)]
+    _lib.check(_lib.load().helen_delta_rule_bytes(ctypes.byref(op), *(ctypes.byref(x) for x in got)))
+    return tuple(int(x.value) for x in got)
+
+
 class _Call(object):
-    """A checked delta rule call: the C description and the tensors it points into."""
+    """A checked delta rule call: what its C description is packed from, and the tensors it points into."""
 
     def __init__(self, q, k, v, g, beta, scale, initial_state, offsets):
-        self.tokens, self.hk, self.hv, self.dk, self.dv = _heads(q, k, v, g, beta)
-        self.device, self.dtype = q.device, q.dtype
+        self.sizes = device, code, n, hk, hv, dk, dv = _heads(q, k, v, g, beta)
+        self.device, self.dtype, self.tokens, self.hv, self.dv = device, q.dtype, n, hv, dv
         self.q, self.k, self.v = _inner(q, 16), _inner(k, 16), _inner(v, 16)
         self.g, self.beta = g, beta
-        whole = True                       # every row belongs to a sequence, as far as the host can tell
-        if offsets is None:
-            sequences = 1
-            self.offsets = None
-        else:
+        self.whole = True                  # every row belongs to a sequence, as far as the host can tell
+        sequences = 1
+        if offsets is not None:
             if isinstance(offsets, (list, tuple)):
                 offsets = torch.tensor(offsets, dtype=torch.int64)
-            _need(isinstance(offsets, torch.Tensor) and offsets.dim() == 1 and offsets.numel() >= 2
-                  and offsets.dtype in (torch.int32, torch.int64), "offsets must be one row of at least two int32 / int64")
+            if not (isinstance(offsets, torch.Tensor) and offsets.dim() == 1 and offsets.numel() >= 2
+                    and offsets.dtype in (torch.int32, torch.int64)):
+                _fail("offsets must be one row of at least two int32 / int64")
             sequences = offsets.numel() - 1
-            whole = False
+            self.whole = False
             if offsets.is_cuda:
-                _on_gpu("offsets", offsets, q.device)
+                _same_gpu("offsets", offsets, device)
             else:
                 at = offsets.tolist()
-                _need(at[0] == 0 and at[-1] <= self.tokens and all(a <= b for a, b in zip(at, at[1:])),
-                      "offsets must ascend from 0 to at most %d" % self.tokens)
-                whole = at[-1] == self.tokens
-            self.offsets = offsets.to(device=q.device, dtype=torch.int32).contiguous()
+                if at[0] != 0 or at[-1] > n or any(a > b for a, b in zip(at, at[1:])):
+                    _fail("offsets must ascend from 0 to at most %d" % n)
+                self.whole = at[-1] == n
+            if not offsets.is_cuda or offsets.dtype != torch.int32 or not offsets.is_contiguous():
+                offsets = offsets.to(device=q.device, dtype=torch.int32).contiguous()
+        self.offsets = offsets
         self.sequences = sequences
-        self.whole = whole
-        self.state_shape = (sequences, self.hv, self.dk, self.dv)
-        self.initial = _state("initial_state", initial_state, self.state_shape, q.device)
-        c = self.c = _lib.HelenDeltaRuleC()
-        c.struct_size = ctypes.sizeof(c)
-        c.device, c.dtype = q.device.index, _TYPES[q.dtype]
-        c.heads_k, c.heads_v, c.width_k, c.width_v = self.hk, self.hv, self.dk, self.dv
-        c.tokens, c.sequences = self.tokens, sequences
-        c.scale = float(self.dk ** -0.5 if scale is None else scale)
-        c.offsets = _ptr(self.offsets)
-        c.q, c.k, c.v, c.g, c.beta = (_ptr(t) for t in (self.q, self.k, self.v, self.g, self.beta))
-        c.q_stride, c.k_stride, c.v_stride = _pair(self.q), _pair(self.k), _pair(self.v)
-        c.g_stride, c.beta_stride = _pair(self.g), _pair(self.beta)
-        c.initial_state = _ptr(self.initial)
+        self.state_shape = (sequences, hv, dk, dv)
+        self.initial = _state("initial_state", initial_state, self.state_shape, device)
+        self.scale = dk ** -0.5 if scale is None else float(scale)
+        self.work = _rule_bytes(code, hk, hv, dk, dv, n, sequences)
 
-    def bytes(self):
-        got = [ctypes.c_size_t() for _ in range(3)]
-        _lib.check(_lib.load().helen_delta_rule_bytes(ctypes.byref(self.c), *(ctypes.byref(x) for x in got)))
-        return [int(x.value) for x in got]
+    def pack(self, o=None, final=None, zero_tail=0, d_o=None, d_final=None, grads=(None,) * 6):
+        device, code, n, hk, hv, dk, dv = self.sizes
+        q, k, v, g, beta = self.q, self.k, self.v, self.g, self.beta
+        qs, ks, vs, gs, bs = q.stride(), k.stride(), v.stride(), g.stride(), beta.stride()
+        os = o.stride() if o is not None else (0, 0)
+        ds = d_o.stride() if d_o is not None else (0, 0)
+        return _RULE.pack(_RULE.size, device, code, hk, hv, dk, dv, n, self.sequences, zero_tail, self.scale,
+                          _ptr(self.offsets), q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
+                          qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], gs[0], gs[1], bs[0], bs[1],
+                          _ptr(self.initial), _ptr(o), os[0], os[1], _ptr(final), _ptr(d_o), ds[0], ds[1], _ptr(d_final),
+                          *map(_ptr, grads))
 
-    def forward(self, o, keep):
+    def forward(self, o, keep, zero_tail=0):
         """-> (final_state, workspace); `o` None computes the states alone."""
-        final = torch.empty(self.state_shape, dtype=torch.float32, device=self.device)
-        c = self.c
-        c.o, c.final_state = _ptr(o), final.data_ptr()
-        if o is not None:
-            c.o_stride = _pair(o)
-        plain, kept, _ = self.bytes()
-        work = torch.empty(kept if keep else plain, dtype=torch.uint8, device=self.device)
-        _lib.check(_lib.load().helen_delta_rule_forward(ctypes.byref(c), int(keep), work.data_ptr(), work.numel(),
-                                                        _stream(self.device)))
+        at = self.q.device
+        final = torch.empty(self.state_shape, dtype=torch.float32, device=at)
+        size = self.work[1 if keep else 0]
+        work = torch.empty(size, dtype=torch.uint8, device=at)
+        rc = _lib.load().helen_delta_rule_forward(self.pack(o, final, zero_tail), int(keep), work.data_ptr(), size,
+                                                  _stream(self.device))
+        if rc:
+            _lib.check(rc)
         return final, work
 
 
@@ -171,11 +217,10 @@ def delta_rule(q, k, v, g, beta, scale=None, initial_state=None, offsets=None, o
     call = _Call(q, k, v, g, beta, scale, initial_state, offsets)
     shape = (call.tokens, call.hv, call.dv)
     if out is None:
-        o = torch.empty(shape, dtype=call.dtype, device=call.device)
-        call.c.zero_tail = 0 if call.whole else 1
+        o, tail = torch.empty(shape, dtype=call.dtype, device=q.device), 0 if call.whole else 1
     else:
-        o = _output("out", out, shape, call.dtype, call.device)
-    final, work = call.forward(o, keep)
+        o, tail = _output("out", out, shape, call.dtype, call.device), 0
+    final, work = call.forward(o, keep, tail)
     return (o, final, work) if keep else (o, final)
 
 
@@ -185,28 +230,27 @@ def delta_rule_backward(d_o, q, k, v, g, beta, scale=None, initial_state=None, o
     arguments are those of the forward call; `saved` is what it returned with keep=True (without it the states are computed
     again).  d_initial_state is returned whether or not there was an initial state."""
     call = _Call(q, k, v, g, beta, scale, initial_state, offsets)
-    _on_gpu("d_o", d_o, call.device)
-    _need(d_o.dtype == call.dtype and tuple(d_o.shape) == (call.tokens, call.hv, call.dv),
-          "d_o must be %s %s" % (call.dtype, (call.tokens, call.hv, call.dv)))
+    _same_gpu("d_o", d_o, call.device)
+    if d_o.dtype != call.dtype or tuple(d_o.shape) != (call.tokens, call.hv, call.dv):
+        _fail("d_o must be %s %s" % (call.dtype, (call.tokens, call.hv, call.dv)))
     d_o = _inner(d_o, 16)
     d_final = _state("d_final_state", d_final_state, call.state_shape, call.device)
-    _, kept, own = call.bytes()
+    _, kept, own = call.work
     if saved is None:
         _, saved = call.forward(None, True)
     else:
-        _on_gpu("saved", saved, call.device)
-        _need(saved.dtype == torch.uint8 and saved.numel() == kept and saved.is_contiguous(),
-              "saved is not what delta_rule(..., keep=True) returned for these arguments")
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    dg, dbeta = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (g, beta))
-    d_initial = torch.empty(call.state_shape, dtype=torch.float32, device=call.device)
-    c = call.c
-    c.d_o, c.d_o_stride, c.d_final_state = d_o.data_ptr(), _pair(d_o), _ptr(d_final)
-    c.grad_q, c.grad_k, c.grad_v, c.grad_g, c.grad_beta = (t.data_ptr() for t in (dq, dk, dv, dg, dbeta))
-    c.grad_initial_state = d_initial.data_ptr()
-    work = torch.empty(own, dtype=torch.uint8, device=call.device)
-    _lib.check(_lib.load().helen_delta_rule_backward(ctypes.byref(c), saved.data_ptr(), saved.numel(), work.data_ptr(),
-                                                     work.numel(), _stream(call.device)))
+        _same_gpu("saved", saved, call.device)
+        if saved.dtype != torch.uint8 or saved.numel() != kept or not saved.is_contiguous():
+            _fail("saved is not what delta_rule(..., keep=True) returned for these arguments")
+    at = q.device
+    dq, dk, dv = (torch.empty(t.shape, dtype=call.dtype, device=at) for t in (q, k, v))
+    dg, dbeta = (torch.empty(g.shape, dtype=torch.float32, device=at) for _ in range(2))
+    d_initial = torch.empty(call.state_shape, dtype=torch.float32, device=at)
+    work = torch.empty(own, dtype=torch.uint8, device=at)
+    op = call.pack(d_o=d_o, d_final=d_final, grads=(dq, dk, dv, dg, dbeta, d_initial))
+    rc = _lib.load().helen_delta_rule_backward(op, saved.data_ptr(), kept, work.data_ptr(), own, _stream(call.device))
+    if rc:
+        _lib.check(rc)
     return dq, dk, dv, dg, dbeta, d_initial
 
 
@@ -217,38 +261,41 @@ def delta_rule_step(q, k, v, g, beta, state, slots=None, scale=None, out=None):
               zero.  Rows that name the same entry are successive tokens of one stream, taken in the order of the rows.  Any
               other number outside the pool makes that row's output NaN and changes no state
     -> o [rows, heads_v, width_v]."""
-    n, hk, hv, dk, dv = _heads(q, k, v, g, beta)
-    device = q.device
-    _on_gpu("state", state, device)
-    _need(state.dtype == torch.float32 and state.dim() == 4 and tuple(state.shape[1:]) == (hv, dk, dv),
-          "state must be float32 [pool, %d, %d, %d]" % (hv, dk, dv))
-    pool = state.shape[0]
-    _need(pool == 0 or state[0].is_contiguous(), "the entries of state must be contiguous")
-    per = hv * dk * dv
-    stride = state.stride(0) if pool > 1 else per
-    _need(stride >= per and stride % 4 == 0 and state.data_ptr() % 16 == 0, "the entries of state overlap or are not 16-byte aligned")
+    device, code, n, hk, hv, dk, dv = _heads(q, k, v, g, beta)
+    _same_gpu("state", state, device)
+    s_shape = state.shape
+    if state.dtype != torch.float32 or len(s_shape) != 4 or s_shape[1:] != (hv, dk, dv):
+        _fail("state must be float32 [pool, %d, %d, %d]" % (hv, dk, dv))
+    pool, per = s_shape[0], hv * dk * dv
+    stride = per
+    if pool > 0 and state.numel():
+        strides = state.stride()
+        if strides[1:] != (dk * dv, dv, 1) and not state[0].is_contiguous():
+            _fail("the entries of state must be contiguous")
+        stride = strides[0] if pool > 1 else per
+        if stride < per or stride % 4 or state.data_ptr() % 16:
+            _fail("the entries of state overlap or are not 16-byte aligned")
     if slots is None:
-        _need(n <= pool, "%d rows over a pool of %d states" % (n, pool))
+        if n > pool:
+            _fail("%d rows over a pool of %d states" % (n, pool))
     else:
-        _on_gpu("slots", slots, device)
-        _need(slots.dtype == torch.int32 and tuple(slots.shape) == (n,), "slots must be int32 [%d]" % n)
+        _same_gpu("slots", slots, device)
+        if slots.dtype != torch.int32 or slots.shape != (n,):
+            _fail("slots must be int32 [%d]" % n)
         slots = slots.contiguous()
     if out is None:
-        o = torch.empty((n, hv, dv), dtype=q.dtype, device=device)
+        o = torch.empty((n, hv, dv), dtype=q.dtype, device=q.device)
     else:
         o = _output("out", out, (n, hv, dv), q.dtype, device)
     q, k, v = _inner(q), _inner(k), _inner(v, 16)
-    c = _lib.HelenDeltaStepC()
-    c.struct_size = ctypes.sizeof(c)
-    c.device, c.dtype = device.index, _TYPES[q.dtype]
-    c.heads_k, c.heads_v, c.width_k, c.width_v, c.rows, c.pool = hk, hv, dk, dv, n, pool
-    c.scale = float(dk ** -0.5 if scale is None else scale)
-    c.slots = _ptr(slots)
-    c.q, c.k, c.v, c.g, c.beta, c.state, c.o = (t.data_ptr() for t in (q, k, v, g, beta, state, o))
-    c.q_stride, c.k_stride, c.v_stride = _pair(q), _pair(k), _pair(v)
-    c.g_stride, c.beta_stride, c.o_stride = _pair(g), _pair(beta), _pair(o)
-    c.state_stride = stride
-    _lib.check(_lib.load().helen_delta_rule_step(ctypes.byref(c), _stream(device)))
+    qs, ks, vs, gs, bs, os = q.stride(), k.stride(), v.stride(), g.stride(), beta.stride(), o.stride()
+    op = _STEP.pack(_STEP.size, device, code, hk, hv, dk, dv, n, pool, dk ** -0.5 if scale is None else scale,
+                    0 if slots is None else slots.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+                    beta.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], gs[0], gs[1], bs[0], bs[1],
+                    state.data_ptr(), stride, o.data_ptr(), os[0], os[1])
+    rc = _lib.load().helen_delta_rule_step(op, _stream(device))
+    if rc:
+        _lib.check(rc)
     return o
 
 
@@ -260,74 +307,96 @@ def _rows(t):
     return _inner(t)
 
 
-def _norm_call(x, weight, bias, name):
-    _on_gpu("x", x)
-    _need(x.dtype in _TYPES, "x is %s: float32, bfloat16 or float16 are supported" % x.dtype)
-    _need(x.dim() >= 1 and x.shape[-1] >= 1, "x must have a last dimension of at least one element")
-    width = x.shape[-1]
+def _norm_sizes(x, weight, bias):
+    """-> (device, type of x, type of the weight, width)."""
+    device = _gpu_index("x", x)
+    dtype = x.dtype
+    code = _TYPES.get(dtype)
+    if code is None:
+        _fail("x is %s: float32, bfloat16 or float16 are supported" % dtype)
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        _fail("x must have a last dimension of at least one element")
+    width = shape[-1]
     kind = None
     for label, t in (("weight", weight), ("bias", bias)):
         if t is not None:
-            _on_gpu(label, t, x.device)
-            _need(tuple(t.shape) == (width,), "%s must be [%d]" % (label, width))
-            _need(t.dtype in (x.dtype, torch.float32), "%s is %s: x's type %s or float32 is needed" % (label, t.dtype, x.dtype))
-            _need(kind in (None, t.dtype), "weight and bias must be of one type")
-            kind = t.dtype
-    c = _lib.HelenLayerNormC()
-    c.struct_size = ctypes.sizeof(c)
-    c.device, c.dtype, c.weight_dtype = x.device.index, _TYPES[x.dtype], _TYPES[kind or torch.float32]
-    c.width = width
-    return c, width
+            _same_gpu(label, t, device)
+            if t.shape != (width,):
+                _fail("%s must be [%d]" % (label, width))
+            of = t.dtype
+            if of != dtype and of != torch.float32:
+                _fail("%s is %s: x's type %s or float32 is needed" % (label, of, dtype))
+            if kind is not None and kind != of:
+                _fail("weight and bias must be of one type")
+            kind = of
+    return device, code, _lib.HELEN_TYPE_FP32 if kind is None else _TYPES[kind], width
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
     """Layer norm over the last dimension: y = (x - mean) rstd weight + bias with rstd = 1 / sqrt(var + eps).
     x [..., width] float32, bfloat16 or float16, weight / bias [width] of x's type or float32.  Rows of any stride and alignment.
     -> (y, mean, rstd), mean and rstd float32 [...] for layer_norm_backward."""
-    c, width = _norm_call(x, weight, bias, "layer_norm")
+    device, code, kind, width = _norm_sizes(x, weight, bias)
     rows = _rows(x)
-    n = rows.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else _output("out", out, tuple(x.shape), x.dtype, x.device)
-    _need(out is None or y.is_contiguous() or y.dim() == 2, "out must be contiguous or have two dimensions")
+    shape, at = x.shape, x.device
+    if out is None:
+        y = torch.empty(shape, dtype=x.dtype, device=at)
+    else:
+        y = _output("out", out, tuple(shape), x.dtype, device)
+        if y.dim() != 2 and not y.is_contiguous():
+            _fail("out must be contiguous or have two dimensions")
     flat = y if y.dim() == 2 else y.view(-1, width)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
+    mean = torch.empty(shape[:-1], dtype=torch.float32, device=at)
+    rstd = torch.empty(shape[:-1], dtype=torch.float32, device=at)
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    c.rows, c.eps = n, float(eps)
-    c.x, c.x_stride, c.y, c.y_stride = rows.data_ptr(), rows.stride(0), flat.data_ptr(), flat.stride(0)
-    c.weight, c.bias, c.mean, c.rstd = _ptr(weight), _ptr(bias), mean.data_ptr(), rstd.data_ptr()
-    _lib.check(_lib.load().helen_layer_norm_forward(ctypes.byref(c), _stream(x.device)))
+    op = _NORM.pack(_NORM.size, device, code, kind, width, rows.shape[0], eps, rows.data_ptr(), rows.stride(0), _ptr(weight),
+                    _ptr(bias), flat.data_ptr(), flat.stride(0), mean.data_ptr(), rstd.data_ptr(), 0, 0, 0, 0, 0, 0)
+    rc = _lib.load().helen_layer_norm_forward(op, _stream(device))
+    if rc:
+        _lib.check(rc)
     return y, mean, rstd
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_bytes(code, kind, width, rows):
+    op = _NORM.pack(_NORM.size, 0, code, kind, width, rows, 0.0, *(0,) * 14)
+    need = ctypes.c_size_t()
+    _lib.check(_lib.load().helen_layer_norm_bytes(op, ctypes.byref(need)))
+    return int(need.value)
 
 
 def layer_norm_backward(dy, x, weight, mean, rstd, bias=True):
     """Gradients of layer_norm: dy like x, weight (or None), mean and rstd as layer_norm returned them
     -> (dx, dweight, dbias); dweight is None without a weight, dbias None with bias=False.  dweight and dbias have the weight's
     type (float32 without one) and are summed in float32 in a fixed order."""
-    c, width = _norm_call(x, weight, None, "layer_norm_backward")
-    _on_gpu("dy", dy, x.device)
-    _need(dy.dtype == x.dtype and dy.shape == x.shape, "dy must be %s %s" % (x.dtype, tuple(x.shape)))
+    device, code, kind, width = _norm_sizes(x, weight, None)
+    shape, at = x.shape, x.device
+    _same_gpu("dy", dy, device)
+    if dy.dtype != x.dtype or dy.shape != shape:
+        _fail("dy must be %s %s" % (x.dtype, tuple(shape)))
     for name, t in (("mean", mean), ("rstd", rstd)):
-        _on_gpu(name, t, x.device)
-        _need(t.dtype == torch.float32 and t.shape == x.shape[:-1], "%s must be float32 %s" % (name, tuple(x.shape[:-1])))
+        _same_gpu(name, t, device)
+        if t.dtype != torch.float32 or t.shape != shape[:-1]:
+            _fail("%s must be float32 %s" % (name, tuple(shape[:-1])))
     rows, drows = _rows(x), _rows(dy)
     mean, rstd = mean.contiguous(), rstd.contiguous()
     weight = None if weight is None else weight.contiguous()
-    kind = torch.float32 if weight is None else weight.dtype
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    of = torch.float32 if weight is None else weight.dtype
+    dx = torch.empty(shape, dtype=x.dtype, device=at)
     flat = dx if dx.dim() == 2 else dx.view(-1, width)
-    dweight = None if weight is None else torch.empty(width, dtype=kind, device=x.device)
-    dbias = torch.empty(width, dtype=kind, device=x.device) if bias else None
-    c.rows = rows.shape[0]
-    c.x, c.x_stride, c.dy, c.dy_stride = rows.data_ptr(), rows.stride(0), drows.data_ptr(), drows.stride(0)
-    c.dx, c.dx_stride = flat.data_ptr(), flat.stride(0)
-    c.weight, c.mean, c.rstd, c.dweight, c.dbias = _ptr(weight), mean.data_ptr(), rstd.data_ptr(), _ptr(dweight), _ptr(dbias)
-    lib = _lib.load()
-    need = ctypes.c_size_t()
-    _lib.check(lib.helen_layer_norm_bytes(ctypes.byref(c), ctypes.byref(need)))
-    work = torch.empty(max(int(need.value), 16), dtype=torch.uint8, device=x.device)
-    _lib.check(lib.helen_layer_norm_backward(ctypes.byref(c), work.data_ptr(), work.numel(), _stream(x.device)))
+    dweight = None if weight is None else torch.empty(width, dtype=of, device=at)
+    dbias = torch.empty(width, dtype=of, device=at) if bias else None
+    n = rows.shape[0]
+    size = _norm_bytes(code, kind, width, n)
+    work = torch.empty(size, dtype=torch.uint8, device=at)
+    op = _NORM.pack(_NORM.size, device, code, kind, width, n, 0.0, rows.data_ptr(), rows.stride(0), _ptr(weight), 0, 0, 0,
+                    mean.data_ptr(), rstd.data_ptr(), drows.data_ptr(), drows.stride(0), flat.data_ptr(), flat.stride(0),
+                    _ptr(dweight), _ptr(dbias))
+    rc = _lib.load().helen_layer_norm_backward(op, work.data_ptr(), size, _stream(device))
+    if rc:
+        _lib.check(rc)
     return dx, dweight, dbias
 
 

@@ -200,6 +200,19 @@ def test_layer_norm_refuses(change, text):
     assert lib.helen_layer_norm_backward(ctypes.byref(c), None, 0, None) == -1
 
 
+@pytest.mark.parametrize("packer, structure", [("_RULE", "HelenDeltaRuleC"), ("_STEP", "HelenDeltaStepC"), ("_NORM", "HelenLayerNormC")])
+def test_packed_descriptions_have_the_layout_of_the_structures(packer, structure):
+    packer, structure = getattr(ops, packer), getattr(_lib, structure)
+    assert packer.size == ctypes.sizeof(structure)
+    count = len(packer.unpack(bytes(packer.size)))
+    got = structure.from_buffer_copy(packer.pack(*range(1, count + 1)))
+    flat = []
+    for name, _ in structure._fields_:
+        value = getattr(got, name)
+        flat += list(value) if hasattr(value, "__len__") else [value]
+    assert [int(x) for x in flat] == list(range(1, count + 1))
+
+
 def test_tensors_on_the_host_are_refused():
     x = make([4], 1, 1, 64, 64, torch.float32, False)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
