@@ -25,23 +25,27 @@ template <typename In>
 struct Pieces {
     typedef typename In::raw raw;
     static constexpr int V = 16 / (int)sizeof(raw);
-    typedef raw vec __attribute__((ext_vector_type(16 / sizeof(raw)), aligned(sizeof(raw))));
-    static __device__ __forceinline__ void load(const raw* p, int left, float (&to)[V]) {
+    typedef raw vec __attribute__((ext_vector_type(16 / sizeof(raw))));
+    typedef vec vec_any __attribute__((aligned(sizeof(raw))));
+    // as they lie in memory, zero behind the row's end (`left` elements)
+    static __device__ __forceinline__ vec read(const raw* p, int left) {
+        vec t;
         if (left >= V) {
-            const vec t = *(const vec*)p;
-#pragma unroll
-            for (int i = 0; i < V; ++i) to[i] = In::to_f32(t[i]);
+            t = *(const vec_any*)p;
         } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) to[i] = i < left ? In::to_f32(p[i]) : 0.f;
+            for (int i = 0; i < V; ++i) t[i] = i < left ? p[i] : raw(0);
         }
+        return t;
     }
+    static __device__ __forceinline__ void widen(const vec t, float (&to)[V]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) to[i] = In::to_f32(t[i]);
+    }
+    static __device__ __forceinline__ void load(const raw* p, int left, float (&to)[V]) { widen(read(p, left), to); }
     static __device__ __forceinline__ void store(raw* p, int left, const float (&from)[V]) {
         if (left >= V) {
-            vec t;
-#pragma unroll
-            for (int i = 0; i < V; ++i) t[i] = In::from_f32(from[i]);
-            *(vec*)p = t;
+            Columns<In, V>::store(p, from);
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i)
@@ -68,80 +72,124 @@ __device__ __forceinline__ void load_weight(const void* w, int at, int left, flo
     }
 }
 
-// sum over the L lanes of a row; L = 256: over the workgroup (`red` has four floats and is free again after the call)
+// sum over the L lanes of a row; L = 256: over the workgroup (`red` is free again after the call)
 template <int L, int N>
 __device__ __forceinline__ void row_sum(float (&x)[N], float (*red)[N]) {
+    static_assert(L >= 16, "a row of 16 lanes is summed by rotations");
 #pragma unroll
-    for (int m = 1; m < (L < 64 ? L : 64); m <<= 1)
-#pragma unroll
-        for (int n = 0; n < N; ++n) x[n] += __shfl_xor(x[n], m);
+    for (int n = 0; n < N; ++n) {
+        x[n] = dpp_add<0x121>(dpp_add<0x122>(dpp_add<0x124>(dpp_add<0x128>(x[n]))));
+        if constexpr (L > 16) {
+            x[n] += __shfl_xor(x[n], 16);
+            x[n] += __shfl_xor(x[n], 32);
+        }
+    }
     if constexpr (L == 256) {
         const int w = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
             for (int n = 0; n < N; ++n) red[w][n] = x[n];
-        __syncthreads();
+        lds_barrier();
 #pragma unroll
         for (int n = 0; n < N; ++n) x[n] = (red[0][n] + red[1][n]) + (red[2][n] + red[3][n]);
-        __syncthreads();
+        lds_barrier();
     }
 }
 
+// Bandwidth is what bounds both directions.  A workgroup takes rows `groups` apart and has the next one's loads in flight while it
+// works on a row; the weights of its columns stay in registers.
 template <typename In, typename W, int L, int NV>
 __global__ __launch_bounds__(256) void norm_forward_kernel(const NormArgs a) {
     typedef typename In::raw raw;
-    constexpr int V = Pieces<In>::V;
+    typedef Pieces<In> P;
+    constexpr int V = P::V;
     __shared__ float red[4][1];
     const int t = threadIdx.x % L;
-    const long row = blockIdx.x * (long)(256 / L) + threadIdx.x / L;
+    const long step = (long)a.groups * (256 / L);
+    long row = blockIdx.x * (long)(256 / L) + threadIdx.x / L;
     if (row >= a.rows) return;          // (L = 256: the whole workgroup)
-    const raw* x = (const raw*)a.x + row * a.x_t;
-    float v[NV][V], s[1] = {0.f};
+    typename P::vec next[NV];
+    float w[NV][V], b[NV][V];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int at = (t + i * L) * V;
-        Pieces<In>::load(x + at, a.width - at, v[i]);
-#pragma unroll
-        for (int e = 0; e < V; ++e) s[0] += v[i][e];
+        next[i] = P::read((const raw*)a.x + row * a.x_t + at, a.width - at);
     }
-    row_sum<L, 1>(s, red);
-    const float mean = s[0] / a.width;
-    s[0] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            v[i][e] -= mean;
-            s[0] += (t + i * L) * V + e < a.width ? v[i][e] * v[i][e] : 0.f;
-        }
-    row_sum<L, 1>(s, red);
-    const float rstd = 1.f / sqrtf(s[0] / a.width + a.eps);
-    if (t == 0) {
-        if (a.mean) a.mean[row] = mean;
-        if (a.rstd) a.rstd[row] = rstd;
-    }
-    raw* y = (raw*)a.y + row * a.y_t;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int at = (t + i * L) * V, left = a.width - at;
-        if (left <= 0) continue;
-        float w[V], b[V];
-        load_weight<W, V>(a.w, at, left, w, 1.f);
-        load_weight<W, V>(a.b, at, left, b, 0.f);
+        const int at = (t + i * L) * V;
+        load_weight<W, V>(a.w, at, a.width - at, w[i], 1.f);
+        load_weight<W, V>(a.b, at, a.width - at, b[i], 0.f);
+    }
+    while (true) {
+        float v[NV][V], s[1] = {0.f};
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[i][e] = v[i][e] * rstd * w[e] + b[e];
-        Pieces<In>::store(y + at, left, v[i]);
+        for (int i = 0; i < NV; ++i) P::widen(next[i], v[i]);
+        const long after = row + step;
+        if (after < a.rows) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int at = (t + i * L) * V;
+                next[i] = P::read((const raw*)a.x + after * a.x_t + at, a.width - at);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[0] += v[i][e];
+        row_sum<L, 1>(s, red);
+        const float mean = s[0] / a.width;
+        s[0] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                v[i][e] -= mean;
+                s[0] += (t + i * L) * V + e < a.width ? v[i][e] * v[i][e] : 0.f;
+            }
+        row_sum<L, 1>(s, red);
+        const float rstd = 1.f / sqrtf(s[0] / a.width + a.eps);
+        if (t == 0) {
+            if (a.mean) a.mean[row] = mean;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int at = (t + i * L) * V, left = a.width - at;
+            if (left <= 0) continue;
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[i][e] = v[i][e] * rstd * w[i][e] + b[i][e];
+            P::store((raw*)a.y + row * a.y_t + at, left, v[i]);
+        }
+        if (after >= a.rows) break;
+        row = after;
     }
 }
 
 template <typename In, typename W, int L, int NV>
 __global__ __launch_bounds__(256) void norm_backward_kernel(const NormArgs a) {
     typedef typename In::raw raw;
-    constexpr int V = Pieces<In>::V, R = 256 / L;
+    typedef Pieces<In> P;
+    constexpr int V = P::V, R = 256 / L;
     __shared__ float red[4][2];
     __shared__ float cols[R > 1 ? 256 * V : 1];
     const int t = threadIdx.x % L;
+    const long step = (long)a.groups * R;
     float w[NV][V], dw[NV][V], db[NV][V];
+    typename P::vec nx[NV], ny[NV];
+    float nmean = 0.f, nrstd = 0.f;
+    long row = blockIdx.x * (long)R + threadIdx.x / L;
+    auto read = [&](long r) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int at = (t + i * L) * V;
+            nx[i] = P::read((const raw*)a.x + r * a.x_t + at, a.width - at);
+            ny[i] = P::read((const raw*)a.dy + r * a.dy_t + at, a.width - at);
+        }
+        nmean = a.mean[r];
+        nrstd = a.rstd[r];
+    };
+    if (row < a.rows) read(row);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int at = (t + i * L) * V;
@@ -149,17 +197,15 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(const NormArgs a) {
 #pragma unroll
         for (int e = 0; e < V; ++e) dw[i][e] = db[i][e] = 0.f;
     }
-    for (long row = blockIdx.x * (long)R + threadIdx.x / L; row < a.rows; row += (long)a.groups * R) {
-        const raw* x = (const raw*)a.x + row * a.x_t;
-        const raw* dy = (const raw*)a.dy + row * a.dy_t;
-        const float mean = a.mean[row], rstd = a.rstd[row];
+    for (; row < a.rows; row += step) {
         float h[NV][V], g[NV][V], s[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int at = (t + i * L) * V;
-            Pieces<In>::load(x + at, a.width - at, h[i]);
-            Pieces<In>::load(dy + at, a.width - at, g[i]);
+            P::widen(nx[i], h[i]);
+            P::widen(ny[i], g[i]);
         }
+        const float mean = nmean, rstd = nrstd;
+        if (row + step < a.rows) read(row + step);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -180,7 +226,7 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(const NormArgs a) {
             if (left <= 0) continue;
 #pragma unroll
             for (int e = 0; e < V; ++e) h[i][e] = rstd * (g[i][e] - c0 - h[i][e] * c1);
-            Pieces<In>::store(dx + at, left, h[i]);
+            P::store(dx + at, left, h[i]);
         }
     }
     // the workgroup's sums of its columns: [group][dw | db][width]
@@ -193,13 +239,14 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(const NormArgs a) {
 #pragma unroll
             for (int e = 0; e < V; ++e) x[e] = k ? db[i][e] : dw[i][e];
             if constexpr (R > 1) {
-                __syncthreads();
+                lds_barrier();
 #pragma unroll
                 for (int e = 0; e < V; ++e) cols[e * 256 + threadIdx.x] = x[e];
-                __syncthreads();
+                lds_barrier();
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     x[e] = 0.f;
+#pragma unroll
                     for (int r = 0; r < R; ++r) x[e] += cols[e * 256 + r * L + t];
                 }
             }
@@ -296,21 +343,29 @@ __global__ __launch_bounds__(256) void norm_backward_wide_kernel(const NormArgs 
     }
 }
 
-// the workgroups' sums, added in their order: 32 columns and 8 runs of groups a workgroup
+// the workgroups' sums, added in a fixed order: 32 columns and 32 runs of groups a workgroup
 template <typename W>
-__global__ __launch_bounds__(256) void norm_reduce_kernel(const NormArgs a) {
-    __shared__ float part[8][33];
+__global__ __launch_bounds__(1024) void norm_reduce_kernel(const NormArgs a) {
+    __shared__ float part[32][33];
     const int c = threadIdx.x & 31, run = threadIdx.x >> 5;
     const long at = blockIdx.x * 32l + c;
     float x = 0.f;
-    if (at < 2l * a.width)
-        for (int g = run; g < a.groups; g += 8) x += a.partial[(long)g * 2 * a.width + at];
+    if (at < 2l * a.width) {
+        const float* p = a.partial + at;
+        for (int g = run; g < a.groups; g += 32 * 16) {
+            float y[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = g + 32 * i < a.groups ? p[(long)(g + 32 * i) * 2 * a.width] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x += y[i];
+        }
+    }
     part[run][c] = x;
-    __syncthreads();
+    lds_barrier();
     if (run == 0 && at < 2l * a.width) {
         float sum = 0.f;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) sum += part[r][c];
+        for (int r = 0; r < 32; ++r) sum += part[r][c];
         void* to = at < a.width ? a.dw : a.db;
         if (to) ((typename W::raw*)to)[at < a.width ? at : at - a.width] = W::from_f32(sum);
     }

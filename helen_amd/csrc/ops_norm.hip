@@ -29,13 +29,14 @@ NormPlan norm_plan(int width, int dtype) {
     if (pieces <= 1024) return {256, 4};
     return {0, 0};
 }
-// workgroups of the backward pass: each writes one partial sum of the weight's gradient
-int norm_groups(const HelenLayerNorm& op) {
+// workgroups of a pass: what the chip holds at once; of the backward pass each writes one partial sum of the weight's gradient
+int norm_groups(const HelenLayerNorm& op, int most) {
     const NormPlan p = norm_plan(op.width, op.dtype);
     const int64_t rows = p.lanes ? 256 / p.lanes : 1;
     const int64_t all = (op.rows + rows - 1) / rows;
-    return (int)(all < 1024 ? (all > 0 ? all : 1) : 1024);
+    return (int)(all < most ? (all > 0 ? all : 1) : most);
 }
+constexpr int kNormForwardGroups = 2048, kNormBackwardGroups = 1024;
 
 int check(const HelenLayerNorm* op, bool backward) {
     if (!op) return fail(HELEN_EINVAL, "layer norm: null description");
@@ -68,11 +69,11 @@ template <typename In, typename W>
 void launch_norm(const NormArgs& a, int dtype, bool backward, hipStream_t s) {
     const NormPlan p = norm_plan(a.width, dtype);
     const dim3 block(256);
-    const auto grid = [&](int lanes) { return dim3(backward ? (unsigned)a.groups : (unsigned)((a.rows + 256 / lanes - 1) / (256 / lanes))); };
+    const dim3 grid((unsigned)a.groups);
 #define HELEN_NORM(L, NV)                                                                                            \
     if (p.lanes == L && p.pieces == NV) {                                                                            \
-        if (backward) hipLaunchKernelGGL((norm_backward_kernel<In, W, L, NV>), grid(L), block, 0, s, a);             \
-        else hipLaunchKernelGGL((norm_forward_kernel<In, W, L, NV>), grid(L), block, 0, s, a);                       \
+        if (backward) hipLaunchKernelGGL((norm_backward_kernel<In, W, L, NV>), grid, block, 0, s, a);             \
+        else hipLaunchKernelGGL((norm_forward_kernel<In, W, L, NV>), grid, block, 0, s, a);                       \
         return;                                                                                                      \
     }
     HELEN_NORM(16, 1)
@@ -96,7 +97,7 @@ void launch_norm(const HelenLayerNorm& op, const NormArgs& a, bool backward, hip
 }
 template <typename W>
 void launch_reduce(const NormArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL(norm_reduce_kernel<W>, dim3((2u * a.width + 31) / 32), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(norm_reduce_kernel<W>, dim3((2u * a.width + 31) / 32), dim3(1024), 0, s, a);
 }
 
 }  // namespace
@@ -150,7 +151,9 @@ int helen_layer_norm_forward(const HelenLayerNorm* op, void* stream) {
     if (op->rows == 0) return HELEN_OK;
     OnDevice on(op->device);
     if (on.status() != hipSuccess) return fail(HELEN_ENODEV, "layer norm: device %d: %s", op->device, hipGetErrorString(on.status()));
-    launch_norm(*op, args_of(*op), false, (hipStream_t)stream);
+    NormArgs a = args_of(*op);
+    a.groups = norm_groups(*op, kNormForwardGroups);
+    launch_norm(*op, a, false, (hipStream_t)stream);
     return launched("layer norm forward");
 }
 
@@ -158,14 +161,14 @@ int helen_layer_norm_bytes(const HelenLayerNorm* op, size_t* backward_bytes) {
     if (!op || op->struct_size != sizeof(HelenLayerNorm)) return fail(HELEN_EINVAL, "layer norm: null or foreign description");
     if (!backward_bytes) return fail(HELEN_EINVAL, "layer norm: null output");
     if (!type_known(op->dtype) || op->width < 1 || op->rows < 0) return fail(HELEN_EINVAL, "layer norm: %lld rows of width %d", (long long)op->rows, op->width);
-    *backward_bytes = (size_t)norm_groups(*op) * 2 * op->width * sizeof(float);
+    *backward_bytes = (size_t)norm_groups(*op, kNormBackwardGroups) * 2 * op->width * sizeof(float);
     return HELEN_OK;
 }
 
 int helen_layer_norm_backward(const HelenLayerNorm* op, void* workspace, size_t workspace_bytes, void* stream) {
     if (const int rc = check(op, true)) return rc;
     NormArgs a = args_of(*op);
-    a.groups = norm_groups(*op);
+    a.groups = norm_groups(*op, kNormBackwardGroups);
     const size_t need = (size_t)a.groups * 2 * op->width * sizeof(float);
     if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)
         return fail(HELEN_EINVAL, "layer norm: workspace of %zu bytes, %zu are needed, 16-byte aligned", workspace_bytes, need);
