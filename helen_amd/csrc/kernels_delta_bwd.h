@@ -483,30 +483,29 @@ __device__ __forceinline__ float sum_from(float x, int lane) {        // over th
 // ------------------------------------------------------------------------------------------------
 // dQ, dK, dbeta and dg of one chunk: a workgroup of DK / 16 waves per (slot, key head).  The value heads of the key head follow
 // one another and are summed in registers: no atomics, one order.
-//   64 x DK results: wave w has dk tiles 2 p, 2 p + 1 (p = w % (DK / 32)) of token tiles 2 mh, 2 mh + 1 (mh = w / (DK / 32))
+//   64 x DK results: wave w has dk tile w of all four token tiles
 //   64 x 64 results: the ten tiles on and below the diagonal go round the waves
-// dv is walked 32 columns a step: Z, E and dO of the step as fragments in LDS (two buffers, one barrier a step), the states
-// straight into registers; both are loaded a step ahead.
+// dv is walked 32 columns a step: Z, E and dO of the step as fragments in LDS (two buffers, one barrier a step), the rows of
+// S0 and dS1 straight into the registers of the one wave that needs them.  What it waits for is memory, so loads run two
+// steps ahead, over the ends of the heads too.
 // ------------------------------------------------------------------------------------------------
-template <typename In, int DK, bool SHARED>
+template <typename In, int DK, int PT, bool SHARED>
 __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) {
-    constexpr int NI = In::kTerms, KS = DK / 32, W = DK / 16, NP = DK / 32, TPW = (10 + W - 1) / W, RB = 64 / W;
+    constexpr int NI = In::kTerms, W = DK / 16, TPW = (10 + W - 1) / W, RB = 64 / W;
     typedef typename In::raw raw;
     constexpr int kStage = 4 * (6 + NI);
     __shared__ bf16x8 stage[2 * kStage * 64];
-    __shared__ bf16x8 fr[3 * (8 + 2 * kTriFrags) * 64];
+    __shared__ bf16x8 fr[PT * (8 + 2 * kTriFrags) * 64];
     __shared__ __attribute__((aligned(16))) Decays dec;
-    __shared__ float bs[64], scl[192], sums[2][NP][64], dbeta[64], gamma[NP], part[W][64];
+    __shared__ float bs[64], scl[192], sums[2][W][64], dbeta[64], gamma[W], part[W][64];
     static_assert(sizeof(stage) >= 3 * 64 * kTriStride * 4, "the 64 x 64 gradients take the stage's place");
     float* const gmat = (float*)stage;
     float* const hmat = gmat + 64 * kTriStride;
     float* const dmat = hmat + 64 * kTriStride;
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int j = lane & 15, q = lane >> 4;
-    const int p = w % NP, mh = w / NP;
+    const int lane0 = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slot = blockIdx.x / a.hk, h = blockIdx.x % a.hk;
     Span sp;
-    const int s = sequence_of(a, slot, lane, &sp);
+    const int s = sequence_of(a, slot, lane0, &sp);
     const int c = slot - sp.slot;
     const int start = sp.begin + c * kDeltaChunk;
     const int n = min(kDeltaChunk, sp.begin + sp.len - start);
@@ -527,7 +526,7 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
         return;
     }
     const size_t kslot = (size_t)slot * a.hk + h;
-    int tm[TPW], tn[TPW];          // this wave's 64 x 64 tiles; a wave that has fewer repeats its first and drops the result
+    int tm[TPW], tn[TPW];          // this wave's 64 x 64 tiles
     bool own[TPW];
 #pragma unroll
     for (int t = 0; t < TPW; ++t) {
@@ -536,205 +535,213 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
         tm[t] = id < 1 ? 0 : (id < 3 ? 1 : (id < 6 ? 2 : 3));
         tn[t] = id - tm[t] * (tm[t] + 1) / 2;
     }
-    f32x4 dQ[2][2], dK[2][2];      // [dk tile][token tile], summed over the value heads
+    f32x4 dQ[4], dK[4];            // by token tile, summed over the value heads
     if constexpr (SHARED) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int m = 0; m < 2; ++m) dQ[i][m] = dK[i][m] = splat4(0.f);
+        for (int m = 0; m < 4; ++m) dQ[m] = dK[m] = splat4(0.f);
     }
     const bool has_z = W == 4 || w < 4;     // who stages Z and dO, and who E, of token tile w & 3
-    const int lane0 = lane;
+    const int steps = a.dv_width / 32, last = a.group * steps - 1;
+    struct Rows {                  // of the states: dk row j of the wave's tile, columns 4 q and 16 + 4 q of the step
+        f32x4 s[2], d[2];
+    } rows[2];
+    struct Tokens {                // of the stage (eight waves: x is Z or E)
+        f32x4 x[2], e[2], y[2];
+    } toks[2];
+    auto load_rows = [&](int at, Rows& to, unsigned lane) {      // step `at` of all heads' steps
+        const int step = min(at, last), head = step / steps, d0 = 32 * (step - head * steps);
+        const size_t base = (((size_t)slot * a.hv + h * a.group + head) * DK + 16 * w) * a.dv_width + d0;
+        const unsigned off = (lane & 15) * a.dv_width + 4 * (lane >> 4);
+        to.s[0] = *(const f32x4*)(a.states + base + off);
+        to.s[1] = *(const f32x4*)(a.states + base + 16 + off);
+        to.d[0] = *(const f32x4*)(a.dstates + base + off);
+        to.d[1] = *(const f32x4*)(a.dstates + base + 16 + off);
+    };
+    auto load_tokens = [&](int at, Tokens& to, unsigned lane) {
+        const int step = min(at, last), head = step / steps, d0 = 32 * (step - head * steps), hv = h * a.group + head;
+        const size_t base = (((size_t)slot * a.hv + hv) * kDeltaChunk + 16 * (w & 3)) * a.dv_width + d0;
+        const unsigned off = (lane & 15) * a.dv_width + 4 * (lane >> 4);
+        const float* const x = (has_z ? a.z : a.e) + base;
+        to.x[0] = *(const f32x4*)(x + off);
+        to.x[1] = *(const f32x4*)(x + 16 + off);
+        if constexpr (W == 4) {
+            to.e[0] = *(const f32x4*)(a.e + base + off);
+            to.e[1] = *(const f32x4*)(a.e + base + 16 + off);
+        }
+        if (has_z) {
+            const int row = min(16 * (w & 3) + (int)(lane & 15), n - 1);
+            const raw* const y = (const raw*)a.dout + (start + row) * a.do_t + hv * a.do_h + d0 + 4 * (lane >> 4);
+            to.y[0] = load4<In>(y);
+            to.y[1] = load4<In>(y + 16);
+        }
+    };
+    auto put = [&](bf16x8* to, const Tokens& from, unsigned lane) {
+        bf16x8 t[3];
+        split8<3>(from.x[0], from.x[1], t);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) to[((has_z ? 0 : 12) + (w & 3) * 3 + k) * 64 + lane] = t[k];
+        if (has_z) {
+            const bool live = 16 * (w & 3) + (int)(lane & 15) < n;
+            bf16x8 y[NI];
+            split8<NI>(live ? from.y[0] : splat4(0.f), live ? from.y[1] : splat4(0.f), y);
+#pragma unroll
+            for (int k = 0; k < NI; ++k) to[(24 + (w & 3) * NI + k) * 64 + lane] = y[k];
+        }
+        if constexpr (W == 4) {
+            split8<3>(from.e[0], from.e[1], t);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) to[(12 + (w & 3) * 3 + k) * 64 + lane] = t[k];
+        }
+    };
+    // gates of a head: g and beta by wave 0, the scales by waves 1 .. 3, a value a thread
+    float gate[2] = {0.f, 0.f};
+    auto load_gates = [&](int hv) {
+        if (w == 0) {
+            const int row = min(lane0, n - 1);
+            gate[0] = a.g[(start + row) * a.g_t + hv * a.g_h];
+            gate[1] = a.beta[(start + row) * a.b_t + hv * a.b_h];
+        } else if (w < 4) {
+            gate[0] = (a.sc + ((size_t)slot * a.hv + hv) * 256 + 64 * (w - 1))[lane0];
+        }
+    };
+    load_gates(h * a.group);
+    load_rows(0, rows[0], lane0);
+    load_tokens(0, toks[0], lane0);
+    load_rows(1, rows[1], lane0);
+    load_tokens(1, toks[1], lane0);
+
+    int at = 0;
     for (int hv = h * a.group; hv < (h + 1) * a.group; ++hv) {
-        const int lane = in_block(lane0), j = lane & 15, q = lane >> 4;     // (nothing of a head's addresses is kept over the loop)
-        const int srow = 16 * (w & 3) + j;
-        const size_t vslot = (size_t)slot * a.hv + hv;
+        const unsigned lane = in_block(lane0);      // (nothing of a head's addresses is kept over the loop)
+        const int j = lane & 15, q = lane >> 4;
         lds_barrier();
         if (w == 0) {
-            const bool in = lane < n;
-            dec.set(lane, in ? a.g[(start + lane) * a.g_t + hv * a.g_h] : 0.f);
-            bs[lane] = in ? a.beta[(start + lane) * a.b_t + hv * a.b_h] : 0.f;
+            dec.set(lane, (int)lane < n ? gate[0] : 0.f);
+            bs[lane] = (int)lane < n ? gate[1] : 0.f;
         } else if (w < 4) {
-            scl[threadIdx.x - 64] = a.sc[vslot * 256 + threadIdx.x - 64];
+            scl[64 * (w - 1) + lane] = gate[0];
         }
-        f32x4 x0, x1, e0, e1, y0, y1, sa[2][2], sd[2][2];   // (eight waves: x is Z or E)
-        auto load = [&](int d0) {
-            const size_t at = (vslot * kDeltaChunk + srow) * a.dv_width + d0 + 4 * q;
-            const float* xp = (has_z ? a.z : a.e) + at;
-            x0 = *(const f32x4*)xp;
-            x1 = *(const f32x4*)(xp + 16);
-            if (has_z) {
-                y0 = y1 = splat4(0.f);
-                if (srow < n) {
-                    const raw* yp = (const raw*)a.dout + (start + srow) * a.do_t + hv * a.do_h + d0 + 4 * q;
-                    y0 = load4<In>(yp);
-                    y1 = load4<In>(yp + 16);
-                }
-            }
-            if constexpr (W == 4) {
-                e0 = *(const f32x4*)(a.e + at);
-                e1 = *(const f32x4*)(a.e + at + 16);
-            }
+        load_gates(min(hv + 1, (h + 1) * a.group - 1));
+        f32x4 q1[4], k1[4], k2[4], da[TPW], dp[TPW];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const size_t sat = (vslot * DK + 16 * (2 * p + i) + j) * a.dv_width + d0 + 4 * q;
-                sa[i][0] = *(const f32x4*)(a.states + sat);
-                sa[i][1] = *(const f32x4*)(a.states + sat + 16);
-                sd[i][0] = *(const f32x4*)(a.dstates + sat);
-                sd[i][1] = *(const f32x4*)(a.dstates + sat + 16);
-            }
-        };
-        auto put = [&](bf16x8* to) {
-            bf16x8 t[3];
-            split8<3>(x0, x1, t);
-#pragma unroll
-            for (int k = 0; k < 3; ++k) to[((has_z ? 0 : 12) + (w & 3) * 3 + k) * 64 + lane] = t[k];
-            if (has_z) {
-                bf16x8 y[NI];
-                split8<NI>(y0, y1, y);
-#pragma unroll
-                for (int k = 0; k < NI; ++k) to[(24 + (w & 3) * NI + k) * 64 + lane] = y[k];
-            }
-            if constexpr (W == 4) {
-                split8<3>(e0, e1, t);
-#pragma unroll
-                for (int k = 0; k < 3; ++k) to[(12 + (w & 3) * 3 + k) * 64 + lane] = t[k];
-            }
-        };
-        f32x4 q1[2][2], k1[2][2], k2[2][2], da[TPW], dp[TPW];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int m = 0; m < 2; ++m) q1[i][m] = k1[i][m] = k2[i][m] = splat4(0.f);
+        for (int m = 0; m < 4; ++m) q1[m] = k1[m] = k2[m] = splat4(0.f);
 #pragma unroll
         for (int t = 0; t < TPW; ++t) da[t] = dp[t] = splat4(0.f);
         float dots = 0.f;
-        load(0);
-        put(stage);
-        for (int d0 = 0, buf = 0; d0 < a.dv_width; d0 += 32, buf ^= 1) {
-            const bf16x8* const from = stage + buf * kStage * 64;
-            bf16x8 st[2][3], dt[2][3];
+        put(stage, toks[0], lane);
+        load_tokens(at + 2, toks[0], lane);
+        auto step = [&](int k, bool more, Rows& rw, Tokens& tk) {        // tk: the next step's tokens
+            const bf16x8* const from = stage + (k & 1) * kStage * 64;
+            bf16x8 st[3], dt[3];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) dots += sa[i][0][r] * sd[i][0][r] + sa[i][1][r] * sd[i][1][r];
-                split8<3>(sa[i][0], sa[i][1], st[i]);
-                split8<3>(sd[i][0], sd[i][1], dt[i]);
-            }
-            const bool more = d0 + 32 < a.dv_width;
-            if (more) load(d0 + 32);
+            for (int r = 0; r < 4; ++r) dots += rw.s[0][r] * rw.d[0][r] + rw.s[1][r] * rw.d[1][r];
+            split8<3>(rw.s[0], rw.s[1], st);
+            split8<3>(rw.d[0], rw.d[1], dt);
+            load_rows(at + k + 2, rw, lane);
             lds_barrier();
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                bf16x8 zf[3], ef[3], yf[NI];
+            for (int m = 0; m < 4; ++m) {
+                bf16x8 x[3], y[NI];
 #pragma unroll
-                for (int t = 0; t < 3; ++t) {
-                    zf[t] = from[((2 * mh + m) * 3 + t) * 64 + lane];
-                    ef[t] = from[(12 + (2 * mh + m) * 3 + t) * 64 + lane];
-                }
+                for (int t = 0; t < 3; ++t) x[t] = from[(m * 3 + t) * 64 + lane];
+                k1[m] = mm(x, st, k1[m]);
 #pragma unroll
-                for (int t = 0; t < NI; ++t) yf[t] = from[(24 + (2 * mh + m) * NI + t) * 64 + lane];
+                for (int t = 0; t < NI; ++t) y[t] = from[(24 + m * NI + t) * 64 + lane];
+                q1[m] = mm(y, st, q1[m]);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    q1[i][m] = mm(yf, st[i], q1[i][m]);
-                    k1[i][m] = mm(zf, st[i], k1[i][m]);
-                    k2[i][m] = mm(ef, dt[i], k2[i][m]);
-                }
+                for (int t = 0; t < 3; ++t) x[t] = from[(12 + m * 3 + t) * 64 + lane];
+                k2[m] = mm(x, dt, k2[m]);
             }
 #pragma unroll
             for (int t = 0; t < TPW; ++t) {
                 if (!own[t]) continue;
-                bf16x8 zf[3], ef[3], yf[NI];
+                bf16x8 x[3], e[3], y[NI];
 #pragma unroll
-                for (int k = 0; k < 3; ++k) {
-                    zf[k] = from[(tm[t] * 3 + k) * 64 + lane];
-                    ef[k] = from[(12 + tn[t] * 3 + k) * 64 + lane];
+                for (int i = 0; i < 3; ++i) {
+                    x[i] = from[(tm[t] * 3 + i) * 64 + lane];
+                    e[i] = from[(12 + tn[t] * 3 + i) * 64 + lane];
                 }
 #pragma unroll
-                for (int k = 0; k < NI; ++k) yf[k] = from[(24 + tm[t] * NI + k) * 64 + lane];
-                da[t] = mm(zf, ef, da[t]);
-                dp[t] = mm(yf, ef, dp[t]);
+                for (int i = 0; i < NI; ++i) y[i] = from[(24 + tm[t] * NI + i) * 64 + lane];
+                da[t] = mm(x, e, da[t]);
+                dp[t] = mm(y, e, dp[t]);
             }
-            if (more) put(stage + (buf ^ 1) * kStage * 64);
+            if (more) {
+                put(stage + ((k & 1) ^ 1) * kStage * 64, tk, lane);
+                load_tokens(at + k + 3, tk, lane);
+            }
+        };
+        for (int k = 0; k < steps; k += 2) {             // (steps is even)
+            step(k, true, rows[0], toks[1]);
+            step(k + 1, k + 2 < steps, rows[1], toks[0]);
         }
-        // K^T and Q^T of this wave's dk tiles: B operands below, and -- element r of half m of step ks -- the values of token
+        // (the last step leaves toks[0] as it was: the next head's first)
+        at += steps;
+        // K^T and Q^T of this wave's dk tile: B operands below, and -- element r of half m of step ks -- the values of token
         // 16 (2 ks + m) + 4 q + r that the dots need
-        bf16x8 kt[2][2][NI], qt[2][2][NI];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                for (int t = 0; t < NI; ++t) {
-                    const size_t at = ((kslot * (DK / 16) * 2 + 2 * (2 * p + i) + ks) * NI + t) * 64 + lane;
-                    kt[i][ks][t] = a.ktf[at];
-                    qt[i][ks][t] = a.qtf[at];
-                }
+        bf16x8 kt[2][NI], qt[2][NI];
         f32x4 kk[TPW], qk[TPW];
 #pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int t = 0; t < NI; ++t) {
+                const size_t f = ((kslot * (DK / 16) * 2 + 2 * w + ks) * NI + t) * 64;
+                kt[ks][t] = (a.ktf + f)[lane];
+                qt[ks][t] = (a.qtf + f)[lane];
+            }
+#pragma unroll
         for (int t = 0; t < TPW; ++t) {
-            const f32x4* at = a.dots + (kslot * 10 + tm[t] * (tm[t] + 1) / 2 + tn[t]) * 128 + lane;
-            kk[t] = at[0];
-            qk[t] = at[64];
+            const f32x4* const x = a.dots + (kslot * 10 + tm[t] * (tm[t] + 1) / 2 + tn[t]) * 128;
+            kk[t] = x[lane];
+            qk[t] = (x + 64)[lane];
         }
-        if (mh == 0) {
-            dots = sum64(dots);
-            if (lane == 0) gamma[p] = dots;
-        }
+        dots = sum64(dots);
+        if (lane == 0) gamma[w] = dots;
         // the 64 x 64 gradients, in the stage's place
         lds_barrier();
-        {
 #pragma unroll
-            for (int t = 0; t < TPW; ++t) {
-                if (!own[t]) continue;
-                const f32x4 decay = dec.rows(tm[t], tn[t], j, q);
-                const int col = 16 * tn[t] + j;
-                const float beta = bs[col], beta1 = beta_of(beta);
+        for (int t = 0; t < TPW; ++t) {
+            if (!own[t]) continue;
+            const f32x4 decay = dec.rows(tm[t], tn[t], j, q);
+            const int col = 16 * tn[t] + j;
+            const float beta = bs[col], beta1 = beta_of(beta);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * tm[t] + 4 * q + r;
-                    if (col == i) dbeta[i] = da[t][r] / beta1;
-                    const float e = col <= i ? decay[r] : 0.f;
-                    const float A = col < i ? -da[t][r] * (beta1 * e) : 0.f, P = col <= i ? a.scale * beta * dp[t][r] : 0.f;
-                    if (col <= i) gmat[i * kTriStride + col] = gmat[col * kTriStride + i] = A;
-                    hmat[i * kTriStride + col] = P * e;
-                    dmat[i * kTriStride + col] = col < i ? A * kk[t][r] + P * (qk[t][r] * e) : 0.f;
-                }
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * tm[t] + 4 * q + r;
+                if (col == i) dbeta[i] = da[t][r] / beta1;
+                const float e = col <= i ? decay[r] : 0.f;
+                const float A = col < i ? -da[t][r] * (beta1 * e) : 0.f, P = col <= i ? a.scale * beta * dp[t][r] : 0.f;
+                if (col <= i) gmat[i * kTriStride + col] = gmat[col * kTriStride + i] = A;
+                hmat[i * kTriStride + col] = P * e;
+                dmat[i * kTriStride + col] = col < i ? A * kk[t][r] + P * (qk[t][r] * e) : 0.f;
             }
         }
         // rows' scales, and the dots with q and k that dg needs
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const int t0 = 16 * (2 * mh + m) + 4 * q;
+        for (int m = 0; m < 4; ++m) {
+            const int t0 = 16 * m + 4 * q;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float beta = scl[t0 + r], eb = scl[64 + t0 + r], ec = scl[128 + t0 + r];
-                float from = 0.f, to = 0.f;
+                float kv = 0.f, qv = 0.f;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float kv = 0.f, qv = 0.f;
-#pragma unroll
-                    for (int t = NI - 1; t >= 0; --t) {
-                        kv += (float)(mh ? kt[i][1][t] : kt[i][0][t])[4 * m + r];
-                        qv += (float)(mh ? qt[i][1][t] : qt[i][0][t])[4 * m + r];
-                    }
-                    q1[i][m][r] *= a.scale * eb;
-                    k1[i][m][r] *= -eb;
-                    k2[i][m][r] *= ec * beta;
-                    from += qv * q1[i][m][r] + kv * k1[i][m][r];
-                    to += kv * k2[i][m][r];
-                    k1[i][m][r] += k2[i][m][r];
+                for (int t = NI - 1; t >= 0; --t) {
+                    kv += (float)kt[m >> 1][t][4 * (m & 1) + r];
+                    qv += (float)qt[m >> 1][t][4 * (m & 1) + r];
                 }
-                from = sum16(from);
-                to = sum16(to);
+                q1[m][r] *= a.scale * eb;
+                k1[m][r] *= -eb;
+                k2[m][r] *= ec * beta;
+                const float from = sum16(qv * q1[m][r] + kv * k1[m][r]), to = sum16(kv * k2[m][r]);
+                k1[m][r] += k2[m][r];
                 if (j == 0) {
-                    sums[0][p][t0 + r] = from;
-                    sums[1][p][t0 + r] = to;
+                    sums[0][w][t0 + r] = from;
+                    sums[1][w][t0 + r] = to;
                 }
             }
         }
         lds_barrier();
-        // A operands of the products with K and Q: G + G^T (8 fragments), H, H^T
+        // A operands of the products with K and Q: G + G^T (8 fragments), H, H^T, in as many terms as the results' type asks for
         for (int f = w; f < 8 + 2 * kTriFrags; f += W) {
             f32x4 lo, hi;
             if (f < 8) {
@@ -755,10 +762,10 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
                     hi[e] = hmat[(32 * ks + 16 + 4 * q + e) * kTriStride + 16 * mt + j];
                 }
             }
-            bf16x8 t[3];
-            split8<3>(lo, hi, t);
+            bf16x8 t[PT];
+            split8<PT>(lo, hi, t);
 #pragma unroll
-            for (int k = 0; k < 3; ++k) fr[(f * 3 + k) * 64 + lane] = t[k];
+            for (int k = 0; k < PT; ++k) fr[(f * PT + k) * 64 + lane] = t[k];
         }
         // dg: sums of column `lane` over rows i >= m, for m in this wave's rows; what the rows below this wave's give follows
         float run[RB];
@@ -767,7 +774,7 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
 #pragma unroll
             for (int m = RB - 1; m >= 0; --m) {
                 const int i = RB * w + m;
-                below += lane < i ? dmat[i * kTriStride + lane] : 0.f;
+                below += (int)lane < i ? dmat[i * kTriStride + lane] : 0.f;
                 run[m] = below;
             }
             part[w][lane] = below;
@@ -775,36 +782,31 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
         lds_barrier();
         // dQ += H K,  dK += (G + G^T) K + H^T Q
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const int mt = 2 * mh + m;
+        for (int m = 0; m < 4; ++m)
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                bf16x8 x[3];
+                bf16x8 x[PT];
 #pragma unroll
-                for (int t = 0; t < 3; ++t) x[t] = fr[((2 * mt + ks) * 3 + t) * 64 + lane];
+                for (int t = 0; t < PT; ++t) x[t] = fr[((2 * m + ks) * PT + t) * 64 + lane];
+                k1[m] = mm<PT, NI, PT - 1>(x, kt[ks], k1[m]);
+                if (ks <= m / 2) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) k1[i][m] = mm(x, kt[i][ks], k1[i][m]);
-                if (ks <= mh) {
-#pragma unroll
-                    for (int t = 0; t < 3; ++t) x[t] = fr[((8 + tri_index(mt, ks)) * 3 + t) * 64 + lane];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) q1[i][m] = mm(x, kt[i][ks], q1[i][m]);
+                    for (int t = 0; t < PT; ++t) x[t] = fr[((8 + tri_index(m, ks)) * PT + t) * 64 + lane];
+                    q1[m] = mm<PT, NI, PT - 1>(x, kt[ks], q1[m]);
                 }
-                if (ks >= mh) {
+                if (ks >= m / 2) {
 #pragma unroll
-                    for (int t = 0; t < 3; ++t) x[t] = fr[((8 + kTriFrags + trt_index(mt, ks)) * 3 + t) * 64 + lane];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) k1[i][m] = mm(x, qt[i][ks], k1[i][m]);
+                    for (int t = 0; t < PT; ++t) x[t] = fr[((8 + kTriFrags + trt_index(m, ks)) * PT + t) * 64 + lane];
+                    k1[m] = mm<PT, NI, PT - 1>(x, qt[ks], k1[m]);
                 }
             }
-        }
         // dg_m of this wave's rows: the rectangle, what leaves before m and arrives from m on, what the state carries over
         {
             float below = 0.f, f = 0.f, g = 0.f, hold = 0.f;
 #pragma unroll
             for (int k = 1; k < W; ++k) below += k > w ? part[k][lane] : 0.f;
 #pragma unroll
-            for (int k = 0; k < NP; ++k) {
+            for (int k = 0; k < W; ++k) {
                 f += sums[0][k][lane];
                 g += sums[1][k][lane];
                 hold += gamma[k];
@@ -813,39 +815,36 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
             float mine = sum_from(f, lane) + sum_before(g, lane) + whole * hold;
 #pragma unroll
             for (int m = 0; m < RB; ++m) {
-                const float x = sum64(lane < RB * w + m ? run[m] + below : 0.f);
-                mine += lane == RB * w + m ? x : 0.f;
+                const float x = sum64((int)lane < RB * w + m ? run[m] + below : 0.f);
+                mine += (int)lane == RB * w + m ? x : 0.f;
             }
-            if (lane / RB == w && lane < n) {
+            if ((int)lane / RB == w && (int)lane < n) {
                 a.dg[(size_t)(start + lane) * a.hv + hv] = mine;
                 a.dbeta[(size_t)(start + lane) * a.hv + hv] = dbeta[lane];
             }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                if constexpr (SHARED) {
-                    dQ[i][m] += q1[i][m];
-                    dK[i][m] += k1[i][m];
-                } else {
-                    dQ[i][m] = q1[i][m];
-                    dK[i][m] = k1[i][m];
-                }
+        for (int m = 0; m < 4; ++m) {
+            if constexpr (SHARED) {
+                dQ[m] += q1[m];
+                dK[m] += k1[m];
+            } else {
+                dQ[m] = q1[m];
+                dK[m] = k1[m];
             }
+        }
     }
+    const int j = lane0 & 15, q = lane0 >> 4;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int m = 0; m < 4; ++m)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = 16 * (2 * mh + m) + 4 * q + r;
-                if (t >= n) continue;
-                const size_t at = ((size_t)(start + t) * a.hk + h) * DK + 16 * (2 * p + i) + j;
-                ((raw*)a.dq)[at] = In::from_f32(dQ[i][m][r]);
-                ((raw*)a.dk)[at] = In::from_f32(dK[i][m][r]);
-            }
+        for (int r = 0; r < 4; ++r) {
+            const int t = 16 * m + 4 * q + r;
+            if (t >= n) continue;
+            const size_t to = ((size_t)(start + t) * a.hk + h) * DK + 16 * w + j;
+            ((raw*)a.dq)[to] = In::from_f32(dQ[m][r]);
+            ((raw*)a.dk)[to] = In::from_f32(dK[m][r]);
+        }
 }
 
 }  // namespace helen
