@@ -1267,8 +1267,12 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
     }
 }
 
-// Which of the two: below this number of 16-column chains the eight-wave kernel
-inline bool chains_are_few(const DeltaArgs& a) { return (long)a.nseq * a.hv * (a.dv_width / 16) < 1024; }
+// Which of the two: the eight-wave kernel while each of its workgroups has a CU to itself.  One sequence of 2048 tokens, bf16, width
+// 128, forward / forward + keep / backward in us, four waves against eight: 256 chains 104, 120, 205 against 75, 95, 170; 288
+// chains 108, 140, 244 against 123, 168, 255; 512 chains 116, 192, 312 against 135, 228, 341 (fp16, fp32 and width 64 cross
+// over at the same place, ragged sequences too).
+constexpr int kComputeUnits = 256;
+inline bool chains_are_few(const DeltaArgs& a) { return (long)a.nseq * a.hv * (a.dv_width / 16) <= kComputeUnits; }
 inline unsigned chain_grid(const DeltaArgs& a, int columns) {
     return (unsigned)(((long)a.nseq * a.hv * (a.dv_width / columns) + 7) / 8 * 8);
 }
