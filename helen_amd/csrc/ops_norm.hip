@@ -29,14 +29,27 @@ NormPlan norm_plan(int width, int dtype) {
     if (pieces <= 1024) return {256, 4};
     return {0, 0};
 }
-// workgroups of a pass: what the chip holds at once; of the backward pass each writes one partial sum of the weight's gradient
-int norm_groups(const HelenLayerNorm& op, int most) {
+// strips of columns of the wide kernels' second backward pass
+int norm_strips(int width, int dtype) {
+    const int per = 256 * (16 / type_size(dtype));
+    return (width + per - 1) / per;
+}
+// Workgroups of a pass.  Forward: more rows in flight against one load of the weight; 32000 x 2048 bf16 44 us with 2048, 42.4 with
+// 4096, 41.2 with 8192, but 8192 x 8192 44 with 4096 and 47.5 with 8192, where none has a second row.  Backward: each writes
+// one partial sum of the weight's gradient and the second kernel reads it; 32000 x 2048 bf16 109 us with 256, 78 with 512, 87 with
+// 1024, 96 with 2048, and 262143 x 128 43, 37, 45, 42.  The wide kernels: 2048 with their strips.
+constexpr int kNormForwardGroups = 4096, kNormBackwardGroups = 512, kNormWideGroups = 2048;
+int norm_groups(const HelenLayerNorm& op, bool backward) {
     const NormPlan p = norm_plan(op.width, op.dtype);
-    const int64_t rows = p.lanes ? 256 / p.lanes : 1;
-    const int64_t all = (op.rows + rows - 1) / rows;
+    const int64_t rows = p.lanes ? 256 / p.lanes : 1, all = (op.rows + rows - 1) / rows;
+    const int strips = norm_strips(op.width, op.dtype);
+    const int most = !backward ? kNormForwardGroups : (p.lanes ? kNormBackwardGroups : (kNormWideGroups + strips - 1) / strips);
     return (int)(all < most ? (all > 0 ? all : 1) : most);
 }
-constexpr int kNormForwardGroups = 2048, kNormBackwardGroups = 1024;
+size_t norm_backward_bytes(const HelenLayerNorm& op) {
+    const bool wide = !norm_plan(op.width, op.dtype).lanes;
+    return ((size_t)norm_groups(op, true) * 2 * op.width + (wide ? 2 * (size_t)op.rows : 0)) * sizeof(float);
+}
 
 int check(const HelenLayerNorm* op, bool backward) {
     if (!op) return fail(HELEN_EINVAL, "layer norm: null description");
@@ -84,8 +97,12 @@ void launch_norm(const NormArgs& a, int dtype, bool backward, hipStream_t s) {
     HELEN_NORM(256, 2)
     HELEN_NORM(256, 4)
 #undef HELEN_NORM
-    if (backward) hipLaunchKernelGGL((norm_backward_wide_kernel<In, W>), dim3((unsigned)a.groups), block, 0, s, a);
-    else hipLaunchKernelGGL((norm_forward_wide_kernel<In, W>), dim3((unsigned)a.rows), block, 0, s, a);
+    if (!backward) {
+        hipLaunchKernelGGL((norm_forward_wide_kernel<In, W>), dim3((unsigned)a.rows), block, 0, s, a);
+        return;
+    }
+    if (a.rows > 0) hipLaunchKernelGGL((norm_backward_sums_kernel<In, W>), dim3((unsigned)a.rows), block, 0, s, a);
+    hipLaunchKernelGGL((norm_backward_strip_kernel<In, W>), dim3((unsigned)norm_strips(a.width, dtype), (unsigned)a.groups), block, 0, s, a);
 }
 void launch_norm(const HelenLayerNorm& op, const NormArgs& a, bool backward, hipStream_t s) {
     const bool f32w = op.weight_dtype == HELEN_TYPE_FP32;
@@ -152,7 +169,7 @@ int helen_layer_norm_forward(const HelenLayerNorm* op, void* stream) {
     OnDevice on(op->device);
     if (on.status() != hipSuccess) return fail(HELEN_ENODEV, "layer norm: device %d: %s", op->device, hipGetErrorString(on.status()));
     NormArgs a = args_of(*op);
-    a.groups = norm_groups(*op, kNormForwardGroups);
+    a.groups = norm_groups(*op, false);
     launch_norm(*op, a, false, (hipStream_t)stream);
     return launched("layer norm forward");
 }
@@ -161,18 +178,19 @@ int helen_layer_norm_bytes(const HelenLayerNorm* op, size_t* backward_bytes) {
     if (!op || op->struct_size != sizeof(HelenLayerNorm)) return fail(HELEN_EINVAL, "layer norm: null or foreign description");
     if (!backward_bytes) return fail(HELEN_EINVAL, "layer norm: null output");
     if (!type_known(op->dtype) || op->width < 1 || op->rows < 0) return fail(HELEN_EINVAL, "layer norm: %lld rows of width %d", (long long)op->rows, op->width);
-    *backward_bytes = (size_t)norm_groups(*op, kNormBackwardGroups) * 2 * op->width * sizeof(float);
+    *backward_bytes = norm_backward_bytes(*op);
     return HELEN_OK;
 }
 
 int helen_layer_norm_backward(const HelenLayerNorm* op, void* workspace, size_t workspace_bytes, void* stream) {
     if (const int rc = check(op, true)) return rc;
     NormArgs a = args_of(*op);
-    a.groups = norm_groups(*op, kNormBackwardGroups);
-    const size_t need = (size_t)a.groups * 2 * op->width * sizeof(float);
+    a.groups = norm_groups(*op, true);
+    const size_t need = norm_backward_bytes(*op);
     if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)
         return fail(HELEN_EINVAL, "layer norm: workspace of %zu bytes, %zu are needed, 16-byte aligned", workspace_bytes, need);
     a.partial = (float*)workspace;
+    a.sums = a.partial + (size_t)a.groups * 2 * op->width;
     OnDevice on(op->device);
     if (on.status() != hipSuccess) return fail(HELEN_ENODEV, "layer norm: device %d: %s", op->device, hipGetErrorString(on.status()));
     hipStream_t s = (hipStream_t)stream;
