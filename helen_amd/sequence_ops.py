@@ -7,6 +7,8 @@ are calls of their own; `DeltaRule` and `LayerNorm` tie them into torch's autogr
 
 A call keeps nothing: workspaces come from torch's allocator, so calls on several streams may run at once and a call may be
 captured into a graph.  Nothing here waits for the device.
+
+Outputs may not overlap inputs or themselves; the exception is layer_norm's `out`, which may be `x`.
 """
 import ctypes
 import functools
@@ -113,8 +115,7 @@ def _state(name, t, shape, device):
     _same_gpu(name, t, device)
     if t.dtype != torch.float32 or tuple(t.shape) != shape:
         _fail("%s must be float32 %s" % (name, shape))
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
+    return t.contiguous()
 
 
 def _output(name, t, shape, dtype, device):
@@ -123,6 +124,13 @@ def _output(name, t, shape, dtype, device):
         _fail("%s must be %s %s" % (name, dtype, shape))
     if t.numel() and t.stride(-1) != 1:
         _fail("%s must have a contiguous last dimension" % name)
+    if not t.is_contiguous():
+        reach = 0                         # of the dimensions with smaller strides
+        for stride, size in sorted(zip(t.stride(), t.shape)):
+            if size > 1:
+                if stride <= reach:
+                    _fail("the elements of %s overlap" % name)
+                reach += stride * (size - 1)
     return t
 
 
@@ -163,8 +171,11 @@ class _Call(object):
                 if at[0] != 0 or at[-1] > n or any(a > b for a, b in zip(at, at[1:])):
                     _fail("offsets must ascend from 0 to at most %d" % n)
                 self.whole = at[-1] == n
-            if not offsets.is_cuda or offsets.dtype != torch.int32 or not offsets.is_contiguous():
-                offsets = offsets.to(device=q.device, dtype=torch.int32).contiguous()
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("offsets on the host cannot be captured into a graph: pass them on the GPU")
+                offsets = offsets.to(torch.int32).pin_memory().to(q.device, non_blocking=True)
+            if offsets.dtype != torch.int32 or not offsets.is_contiguous():
+                offsets = offsets.to(torch.int32).contiguous()
         self.offsets = offsets
         self.sequences = sequences
         self.state_shape = (sequences, hv, dk, dv)
@@ -213,7 +224,12 @@ def delta_rule(q, k, v, g, beta, scale=None, initial_state=None, offsets=None, o
       out            where o goes (any strides with a contiguous last dimension); rows behind the last sequence are left as
                      they are there, and zero in a fresh o
       keep           True: also return what delta_rule_backward needs of this call
-    -> (o, final_state) or (o, final_state, saved).  States stay float32-class whatever the type of q, k, v."""
+    -> (o, final_state) or (o, final_state, saved).  States stay float32-class whatever the type of q, k, v.
+
+    g is a decay: at most 0, -inf included (it forgets the state).  Positive values are taken as they are as long as e to their sum
+    over 64 tokens is a float32.  Tokens are worked on in chunks of 64 (from the sequence's start): a NaN or an infinity in a
+    token's q, k, v, g or beta reaches the results of its whole chunk, earlier tokens included, and what follows it, in its own
+    sequence and heads; other sequences and heads stay as they are."""
     call = _Call(q, k, v, g, beta, scale, initial_state, offsets)
     shape = (call.tokens, call.hv, call.dv)
     if out is None:
@@ -289,7 +305,7 @@ def delta_rule_step(q, k, v, g, beta, state, slots=None, scale=None, out=None):
         o = _output("out", out, (n, hv, dv), q.dtype, device)
     q, k, v = _inner(q), _inner(k), _inner(v, 16)
     qs, ks, vs, gs, bs, os = q.stride(), k.stride(), v.stride(), g.stride(), beta.stride(), o.stride()
-    op = _STEP.pack(_STEP.size, device, code, hk, hv, dk, dv, n, pool, dk ** -0.5 if scale is None else scale,
+    op = _STEP.pack(_STEP.size, device, code, hk, hv, dk, dv, n, pool, dk ** -0.5 if scale is None else float(scale),
                     0 if slots is None else slots.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
                     beta.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], gs[0], gs[1], bs[0], bs[1],
                     state.data_ptr(), stride, o.data_ptr(), os[0], os[1])
@@ -335,7 +351,7 @@ def _norm_sizes(x, weight, bias):
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
     """Layer norm over the last dimension: y = (x - mean) rstd weight + bias with rstd = 1 / sqrt(var + eps).
-    x [..., width] float32, bfloat16 or float16, weight / bias [width] of x's type or float32.  Rows of any stride and alignment.
+    x [..., width] float32, bfloat16 or float16, weight / bias [width] of x's type or float32.  Rows of any stride and alignment; `out` may be x itself.
     -> (y, mean, rstd), mean and rstd float32 [...] for layer_norm_backward."""
     device, code, kind, width = _norm_sizes(x, weight, bias)
     rows = _rows(x)

@@ -282,6 +282,48 @@ def test_delta_rule_packed_sequences(dtype, hk, hv, dk, dv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("hk, hv, dk, dv", [(4, 8, 128, 128), (16, 16, 64, 64), (5, 5, 128, 256)])
+def test_delta_rule_more_chains_than_compute_units(dtype, hk, hv, dk, dv):
+    """320 and 400 chains of 16 columns (the other tests' few sequences stay below 256)."""
+    lengths = [70, 64, 1, 131, 33]
+    check_delta(make(lengths, hk, hv, dk, dv, TYPES[dtype], True, seed=hv), lengths)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("hk, hv, dk, dv", [(1, 2, 128, 128), (2, 2, 64, 256)])
+def test_delta_rule_six_chunks(dtype, hk, hv, dk, dv):
+    lengths = [380, 320]
+    check_delta(make(lengths, hk, hv, dk, dv, TYPES[dtype], True, seed=dv), lengths)
+
+
+@pytest.mark.gpu
+def test_outputs_that_overlap_and_host_offsets_in_a_capture_are_refused():
+    x = gpu(make([10], 1, 2, 64, 64, torch.float32, False))
+    args = (x["q"], x["k"], x["v"], x["g"], x["beta"])
+    row = torch.zeros(1, 2, 64, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        ops.delta_rule(*args, out=row.expand(10, 2, 64))
+    with pytest.raises(ValueError, match="overlap"):
+        ops.delta_rule_step(*args, torch.zeros(10, 2, 64, 64, device="cuda"), out=torch.zeros(200, device="cuda").as_strided((10, 2, 64), (6, 64, 1)))
+    with pytest.raises(ValueError, match="overlap"):
+        ops.layer_norm(x["v"], out=row[:, :1].expand(10, 2, 64))
+    want = ops.delta_rule(*args, offsets=torch.tensor([0, 3, 10], dtype=torch.int32, device="cuda"))
+    apart = torch.zeros(2, 10, 64, device="cuda").transpose(0, 1)
+    got = ops.delta_rule(*args, offsets=[0, 3, 10], out=apart)
+    assert got[0].data_ptr() == apart.data_ptr() and all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = x["v"] * 2
+        with pytest.raises(RuntimeError, match="host cannot be captured"):
+            ops.delta_rule(*args, offsets=[0, 3, 10])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, x["v"] * 2)
+
+
+@pytest.mark.gpu
 def test_delta_rule_many_short_sequences():
     lengths = [(7 * i) % 5 for i in range(300)]
     check_delta(make(lengths, 1, 1, 64, 64, torch.bfloat16, False, seed=3), lengths)
@@ -635,6 +677,29 @@ def test_layer_norm_autograd_and_differences():
         want = (4 * slope[1] - slope[0]) / 3
         have = float((leaves[i].grad.double() * way.double()).sum())
         assert abs(have - want) <= 1e-3 * abs(want) + 1e-3, (i, have, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, rows, width", [("bf16", 20000, 16), ("fp32", 5000, 300), ("fp16", 4200, 130), ("bf16", 4100, 1030),
+                                                ("bf16", 700, 9001), ("fp32", 600, 4100)])
+def test_layer_norm_more_rows_than_workgroups(dtype, rows, width):
+    gen = torch.Generator().manual_seed(rows + width)
+    x, dy = (torch.randn(rows, width, generator=gen).to(TYPES[dtype]).cuda() for _ in range(2))
+    w = (1 + 0.2 * torch.randn(width, generator=gen)).to(TYPES[dtype]).cuda()
+    check_norm(x, w, w, dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [33, 20000])
+def test_layer_norm_in_place_and_wide_without_rows(width):
+    x = torch.randn(7, width, generator=torch.Generator().manual_seed(width)).cuda()
+    want = ops.layer_norm(x)
+    got = ops.layer_norm(x, out=x)
+    assert got[0].data_ptr() == x.data_ptr() and all(torch.equal(a, b) for a, b in zip(got, want))
+    none, w = x[:0], torch.ones(width, device="cuda")
+    y, mean, rstd = ops.layer_norm(none, w)
+    dx, dw, db = ops.layer_norm_backward(none, none, w, mean, rstd)
+    assert y.shape == dx.shape == (0, width) and not dw.any() and not db.any()
 
 
 # ------------------------------------------------------------------------------------------------------------- together
