@@ -32,6 +32,11 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
+template <bool B>
+struct Is {
+    static constexpr bool value = B;
+};
+
 constexpr int kDeltaChunk = 64;
 constexpr int kTriFrags = 6;      // 16 x 32 fragments of a 64 x 64 triangle that are not all zero
 
@@ -177,7 +182,7 @@ struct DeltaArgs {
     bf16x8 *kf, *ktf, *qf, *qtf;
     bf16x8 *tf, *ttf, *pf, *ptf;
     f32x4* dots;                // kept: [slot, hk][10 tiles][K K^T | Q K^T][lane]
-    float* sc;                  // [slot, hv][4][64]: beta, e^b, e^c, e^{b_C} in every place
+    float* sc;                  // [slot, hv][4][64]: beta, e^b (its last one is e^{b_C}), e^c, beta e^c
     float *states, *e;          // kept for the backward pass: [slot, hv, Dk, Dv], [slot, hv, 64, Dv]
     float *dstates, *z;         // backward: [slot, hv, Dk, Dv], [slot, hv, 64, Dv]
 };
@@ -283,19 +288,17 @@ struct Decays {
         tail4[lane] = exp_decay(e <= 2 ? t4 : 0.f);
     }
     __device__ __forceinline__ float block(int b) const { return head[16 * b + 15]; }
-    // e^b and e^c of token `lane`, and of the whole chunk
-    __device__ __forceinline__ void ends(int lane, float* from_start, float* to_end, float* whole) const {
-        float a = head[lane], b = tail[lane], all = 1.f;
+    // e^b and e^c of token `lane`
+    __device__ __forceinline__ void ends(int lane, float* from_start, float* to_end) const {
+        float a = head[lane], b = tail[lane];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             const float x = block(m);
             a *= m < (lane >> 4) ? x : 1.f;
             b *= m > (lane >> 4) ? x : 1.f;
-            all *= x;
         }
         *from_start = a;
         *to_end = b;
-        *whole = all;
     }
     __device__ __forceinline__ float between(int mt, int nt) const {
         float x = 1.f;
@@ -509,13 +512,13 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? (BWD ? 3 : 4) : 1) void delt
         }
         lds_barrier();
         if (w == 2) {
-            float from_start, to_end, whole;
-            dec.ends(lane, &from_start, &to_end, &whole);
+            float from_start, to_end;
+            dec.ends(lane, &from_start, &to_end);
             float* sc = a.sc + vslot * 256;
             sc[lane] = bs[lane];
             (sc + 64)[lane] = from_start;
             (sc + 128)[lane] = to_end;
-            (sc + 192)[lane] = whole;
+            (sc + 192)[lane] = bs[lane] * to_end;
         }
         // A to LDS, P to memory: row 16 tm + j, columns 16 tn + 4 q + r
         f32x4 P[3];
@@ -731,7 +734,14 @@ struct ChainAddress {
 #pragma unroll
                 for (int t = 0; t < NI; ++t) to[i][ks][t] = (from + ((2 * i + ks) * NI + t) * 64)[lane];
     }
-    // row tile w of T or P; row tiles 0 and 1 have one k step, their other one is zeros
+    // Row tile w of T or P; row tiles 0 and 1 have one k step.  A kernel that does not tell the waves apart takes the other one from
+    // the zeros.
+    template <int N>
+    __device__ __forceinline__ void triangle(const bf16x8* from, int c, bf16x8 (&to)[1][N]) const {
+        from += ((vslot + (size_t)c * hv) * kTriFrags + w) * N * 64;
+#pragma unroll
+        for (int t = 0; t < N; ++t) to[0][t] = (from + t * 64)[lane];
+    }
     template <int N>
     __device__ __forceinline__ void triangle(const bf16x8* from, int c, bf16x8 (&to)[2][N]) const {
         from += ((vslot + (size_t)c * hv) * kTriFrags + tri_index(w, 0)) * N * 64;
@@ -743,6 +753,11 @@ struct ChainAddress {
         }
     }
     // row tile w of T^T or P^T; row tiles 2 and 3 have only the second k step
+    __device__ __forceinline__ void transposed(const bf16x8* from, int c, bf16x8 (&to)[1][3]) const {
+        from += ((vslot + (size_t)c * hv) * kTriFrags + trt_index(w, 1)) * 3 * 64;
+#pragma unroll
+        for (int t = 0; t < 3; ++t) to[0][t] = (from + t * 64)[lane];
+    }
     __device__ __forceinline__ void transposed(const bf16x8* from, int c, bf16x8 (&to)[2][3]) const {
         from += ((vslot + (size_t)c * hv) * kTriFrags + trt_index(w, 1)) * 3 * 64;
         const bf16x8* const first = w < 2 ? from - 3 * 64 : zeros;
@@ -826,7 +841,8 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
     load_state<MW, NC>(a.s0, a.zeros, st, a.dv_width, S);
 
     bf16x8 kf[KS][NI], qf[KS][NI], kt[MW][2][NI], tf[2][3], pf[2][PT];
-    f32x4 beta, eb, ec, whole;
+    f32x4 beta, eb, ec;
+    float whole;
     Columns<In, NC> v[4];
     const int row = 16 * w + 4 * q;                 // this lane's tokens: row .. row + 3
     const ChainAddress<In, DK> at(a, sp, h, hv, w, lane);
@@ -838,7 +854,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
         beta = *(const f32x4*)(sc + row);
         eb = *(const f32x4*)(sc + 64 + row);
         ec = *(const f32x4*)(sc + 128 + row);
-        whole = *(const f32x4*)(sc + 192 + row);
+        whole = (sc + 64)[63];
         vrow.clamp(sp.len - c * kDeltaChunk);
         const raw* p = (const raw*)a.v + (sp.begin + c * kDeltaChunk) * a.v_t + hv * a.v_h;
 #pragma unroll
@@ -899,7 +915,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
                 if constexpr (NC > 1) osum[0][nc] = mm(qf[ks], b[ks][nc], osum[0][nc]);
             }
         const f32x4 after = ec, step = beta, head = eb;
-        const f32x4 hold = whole;
+        const float hold = whole;
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
 #pragma unroll
@@ -949,7 +965,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) S[i][nc][r] *= hold[r];
+                for (int r = 0; r < 4; ++r) S[i][nc][r] *= hold;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -1065,12 +1081,14 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
 #pragma unroll
     for (int r = 0; r < 4; ++r) tile_at[r] = (4 * q + r) * a.dv_width + col;
 
-    if (wave < 4) {
+    auto chain = [&](auto two_) {
+        constexpr bool TWO = decltype(two_)::value;
         f32x4 S[MW][1];
         load_state<MW, 1>(a.s0, a.zeros, (((size_t)s * a.hv + hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col, a.dv_width, S);
         struct Operands {        // of one chunk; the next one's are loaded into a second set meanwhile
-            bf16x8 kf[KS][NI], kt[MW][2][NI], tf[2][3];
-            f32x4 beta, eb, ec, whole;
+            bf16x8 kf[KS][NI], kt[MW][2][NI], tf[TWO ? 2 : 1][3];
+            f32x4 eb, weight;     // weight: beta e^c
+            float whole;
             Columns<In, 1> v[4];
         } first, second;
         bf16x8 own[3];
@@ -1086,9 +1104,8 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
         };
         auto load_scales = [&](int c, Operands& to) {
             const float* sc = a.sc + (at.vslot + (size_t)c * a.hv) * 256;
-            to.beta = *(const f32x4*)(sc + row);
-            to.ec = *(const f32x4*)(sc + 128 + row);
-            to.whole = *(const f32x4*)(sc + 192 + row);
+            to.weight = *(const f32x4*)(sc + 192 + row);
+            to.whole = (sc + 64)[63];
         };
         auto share_state = [&]() {
             if constexpr (OWN) {
@@ -1127,17 +1144,17 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
             lds_barrier();
             bf16x8 x[2][3];
             shared_frag<3, 1>(xbuf, 0, 0, lane, x[0]);
-            shared_frag<3, 1>(xbuf, 1, 0, lane, x[1]);
+            if constexpr (TWO) shared_frag<3, 1>(xbuf, 1, 0, lane, x[1]);
             f32x4 e0 = splat4(0.f), e1 = splat4(0.f);
             e0 = mm(now.tf[0], x[0], e0);
-            e1 = mm(now.tf[1], x[1], e1);
+            if constexpr (TWO) e1 = mm(now.tf[1], x[1], e1);
             at.template triangle<3>(a.tf, next, then.tf);
             load_scales(next, then);
-            between_products<12>();
+            between_products<TWO ? 12 : 6>();
             f32x4 E = e0 + e1;
             ebuf[w * 64 + lane] = E;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) E[r] *= now.beta[r] * now.ec[r];
+            for (int r = 0; r < 4; ++r) E[r] *= now.weight[r];
             share_tile<3, 1>(cbuf, w, 0, lane, E);
             issue_loads();
             lds_barrier();
@@ -1146,7 +1163,7 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
 #pragma unroll
             for (int i = 0; i < MW; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) S[i][0][r] *= now.whole[r];
+                for (int r = 0; r < 4; ++r) S[i][0][r] *= now.whole;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -1180,10 +1197,12 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
 #pragma unroll
             for (int i = 0; i < MW; ++i) store_tile<1>(to + (size_t)16 * i * a.dv_width, tile_at, S[i]);
         }
-    } else {
+    };
+    auto output = [&](auto two_) {
+        constexpr bool TWO = decltype(two_)::value;
         // The output transposed, S^T Q^T and U^T P^T (the operands change places, the fragments are the same): a lane then has
         // four neighbouring columns of one token, one store of a chunk
-        bf16x8 qf[KS][NI], pf[2][PT];
+        bf16x8 qf[KS][NI], pf[TWO ? 2 : 1][PT];
         f32x4 beta, O = splat4(0.f);
         float eb = 0.f;
         const int token = 16 * w + j;
@@ -1197,10 +1216,14 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
         auto finish = [&](int c) {
             bf16x8 x[2][PT];
             shared_frag<PT, 1>(ubuf, 0, 0, lane, x[0]);
-            shared_frag<PT, 1>(ubuf, 1, 0, lane, x[1]);
-            f32x4 p0 = splat4(0.f);
-            p0 = mm<PT, PT, PT - 1>(x[0], pf[0], p0);
-            O = mm<PT, PT, PT - 1>(x[1], pf[1], O) + p0;
+            if constexpr (TWO) {
+                shared_frag<PT, 1>(ubuf, 1, 0, lane, x[1]);
+                f32x4 p0 = splat4(0.f);
+                p0 = mm<PT, PT, PT - 1>(x[0], pf[0], p0);
+                O = mm<PT, PT, PT - 1>(x[1], pf[1], O) + p0;
+            } else {
+                O = mm<PT, PT, PT - 1>(x[0], pf[0], O);
+            }
             raw* const to = (raw*)a.o + (sp.begin + c * kDeltaChunk) * a.o_t + hv * a.o_h;
             const float y[4] = {a.scale * O[0], a.scale * O[1], a.scale * O[2], a.scale * O[3]};
             if (token < sp.len - c * kDeltaChunk) Columns<In, 4>::store(to + o_at, y);
@@ -1264,7 +1287,9 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
             lds_barrier();
         }
         if (chunks > 0) finish(chunks - 1);
-    }
+    };
+    if (wave < 4) w < 2 ? chain(Is<false>()) : chain(Is<true>());
+    else w < 2 ? output(Is<false>()) : output(Is<true>());
 }
 
 // Which of the two: the eight-wave kernel while each of its workgroups has a CU to itself.  One sequence of 2048 tokens, bf16, width

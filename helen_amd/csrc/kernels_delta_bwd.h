@@ -35,7 +35,8 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
     load_state<MW, NC>(a.ds1, a.zeros, st, a.dv_width, S);
 
     bf16x8 kf[KS][NI], kt[MW][2][NI], qt[MW][2][NI], tt[2][3], pt[2][3];
-    f32x4 beta, eb, ec, whole;
+    f32x4 beta, eb, ec;
+    float whole;
     Columns<In, NC> y[4];
     const int row = 16 * w + 4 * q;
     const ChainAddress<In, DK> at(a, sp, h, hv, w, lane);
@@ -57,7 +58,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
         beta = *(const f32x4*)(sc + row);
         eb = *(const f32x4*)(sc + 64 + row);
         ec = *(const f32x4*)(sc + 128 + row);
-        whole = *(const f32x4*)(sc + 192 + row);
+        whole = (sc + 64)[63];
     };
     // (no conditional loads, see delta_forward_kernel; rows behind the end meet q = k = 0)
     auto load_dout = [&](int c) {
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
                 P[ks][nc] = mm(pt[ks], b, P[ks][nc]);
             }
         const f32x4 head = eb;
-        const f32x4 hold = whole;
+        const float hold = whole;
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
             f32x4 x;
@@ -185,7 +186,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) S[i][nc][r] *= hold[r];
+                for (int r = 0; r < 4; ++r) S[i][nc][r] *= hold;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -235,12 +236,14 @@ __global__ __launch_bounds__(512) void delta_backward_long_kernel(const DeltaArg
 #pragma unroll
     for (int r = 0; r < 4; ++r) tile_at[r] = (4 * q + r) * a.dv_width + col;
 
-    if (wave < 4) {
+    auto chain = [&](auto two_) {
+        constexpr bool TWO = decltype(two_)::value;
         f32x4 S[MW][1];
         load_state<MW, 1>(a.ds1, a.zeros, (((size_t)s * a.hv + hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col, a.dv_width, S);
         struct Operands {
-            bf16x8 kf[KS][NI], kt[MW][2][NI], tt[2][3];
-            f32x4 beta, eb, ec, whole;
+            bf16x8 kf[KS][NI], kt[MW][2][NI], tt[TWO ? 2 : 1][3];
+            f32x4 beta, eb, ec;
+            float whole;
         } first, second;
         bf16x8 own[3];
         auto load_k = [&](int c, Operands& to) {
@@ -252,7 +255,7 @@ __global__ __launch_bounds__(512) void delta_backward_long_kernel(const DeltaArg
         auto load_scales = [&](int c, Operands& to) {
             const float* sc = a.sc + (at.vslot + (size_t)c * a.hv) * 256;
             to.eb = *(const f32x4*)(sc + 64 + row);
-            to.whole = *(const f32x4*)(sc + 192 + row);
+            to.whole = (sc + 64)[63];
         };
         auto share_state = [&]() {
             if constexpr (OWN) {
@@ -288,14 +291,14 @@ __global__ __launch_bounds__(512) void delta_backward_long_kernel(const DeltaArg
             issue_loads();
             lds_barrier();
             bf16x8 x[2][3];
-            shared_frag<3, 1>(dbuf, 0, 0, lane, x[0]);
             shared_frag<3, 1>(dbuf, 1, 0, lane, x[1]);
+            if constexpr (TWO) shared_frag<3, 1>(dbuf, 0, 0, lane, x[0]);
             f32x4 z0 = splat4(0.f), z1 = splat4(0.f);
-            z0 = mm(now.tt[0], x[0], z0);
-            z1 = mm(now.tt[1], x[1], z1);
+            if constexpr (TWO) z0 = mm(now.tt[0], x[0], z0);
+            z1 = mm(now.tt[TWO], x[1], z1);
             at.transposed(a.ttf, next, then.tt);
             load_scales(next, then);
-            between_products<12>();
+            between_products<TWO ? 12 : 6>();
             f32x4 Z = z0 + z1;
             zfull[w * 64 + lane] = Z;
 #pragma unroll
@@ -309,7 +312,7 @@ __global__ __launch_bounds__(512) void delta_backward_long_kernel(const DeltaArg
             for (int i = 0; i < MW; ++i) {
                 const f32x4 y = wfull[(MW * w + i) * 64 + lane];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) S[i][0][r] = now.whole[r] * S[i][0][r] + y[r];
+                for (int r = 0; r < 4; ++r) S[i][0][r] = now.whole * S[i][0][r] + y[r];
             }
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
@@ -344,8 +347,10 @@ __global__ __launch_bounds__(512) void delta_backward_long_kernel(const DeltaArg
 #pragma unroll
             for (int i = 0; i < MW; ++i) store_tile<1>(to + (size_t)16 * i * a.dv_width, tile_at, S[i]);
         }
-    } else {
-        bf16x8 qt[MW][2][NI], pt[2][3];
+    };
+    auto output = [&](auto two_) {
+        constexpr bool TWO = decltype(two_)::value;
+        bf16x8 qt[MW][2][NI], pt[TWO ? 2 : 1][3];
         f32x4 eb, W[MW];
         Columns<In, 1> y[4];
         RowOffsets yrow(a.do_t, row, col);
@@ -368,11 +373,11 @@ __global__ __launch_bounds__(512) void delta_backward_long_kernel(const DeltaArg
         };
         auto from_p = [&]() {
             bf16x8 b[2][NI];
-            shared_frag<NI, 1>(ybuf, 0, 0, lane, b[0]);
+            if constexpr (TWO) shared_frag<NI, 1>(ybuf, 0, 0, lane, b[0]);
             shared_frag<NI, 1>(ybuf, 1, 0, lane, b[1]);
             f32x4 p0 = splat4(0.f), p1 = splat4(0.f);
-            p0 = mm(pt[0], b[0], p0);
-            p1 = mm(pt[1], b[1], p1);
+            if constexpr (TWO) p0 = mm(pt[0], b[0], p0);
+            p1 = mm(pt[TWO], b[1], p1);
             pfull[w * 64 + lane] = p0 + p1;
         };
         auto from_q = [&]() {
@@ -451,7 +456,9 @@ __global__ __launch_bounds__(512) void delta_backward_long_kernel(const DeltaArg
             issue_loads();
             lds_barrier();
         }
-    }
+    };
+    if (wave < 4) w < 2 ? chain(Is<true>()) : chain(Is<false>());
+    else w < 2 ? output(Is<true>()) : output(Is<false>());
 }
 
 // sum over the 16 lanes of a quarter, over a wave, and running sums
