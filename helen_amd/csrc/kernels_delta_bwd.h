@@ -547,13 +547,16 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
 #pragma unroll
         for (int m = 0; m < 4; ++m) dQ[m] = dK[m] = splat4(0.f);
     }
-    const bool has_z = W == 4 || w < 4;     // who stages Z and dO, and who E, of token tile w & 3
+    // Who stages what of token tile w & 3: with four waves everything; with eight waves 0 .. 3 Z and the first half of dO's columns,
+    // 4 .. 7 E and the second half.  No load is conditional (behind one the compiler's counts of what is in flight are too low).
+    constexpr int YH = W == 4 ? 2 : 1;
+    const int second = W == 4 ? 0 : w >> 2;
     const int steps = a.dv_width / 32, last = a.group * steps - 1;
     struct Rows {                  // of the states: dk row j of the wave's tile, columns 4 q and 16 + 4 q of the step
         f32x4 s[2], d[2];
     } rows[2];
-    struct Tokens {                // of the stage (eight waves: x is Z or E)
-        f32x4 x[2], e[2], y[2];
+    struct Tokens {                // of the stage
+        f32x4 x[2], e[2], y[YH];
     } toks[2];
     auto load_rows = [&](int at, Rows& to, unsigned lane) {      // step `at` of all heads' steps
         const int step = min(at, last), head = step / steps, d0 = 32 * (step - head * steps);
@@ -568,31 +571,30 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
         const int step = min(at, last), head = step / steps, d0 = 32 * (step - head * steps), hv = h * a.group + head;
         const size_t base = (((size_t)slot * a.hv + hv) * kDeltaChunk + 16 * (w & 3)) * a.dv_width + d0;
         const unsigned off = (lane & 15) * a.dv_width + 4 * (lane >> 4);
-        const float* const x = (has_z ? a.z : a.e) + base;
+        const float* const x = (second ? a.e : a.z) + base;
         to.x[0] = *(const f32x4*)(x + off);
         to.x[1] = *(const f32x4*)(x + 16 + off);
         if constexpr (W == 4) {
             to.e[0] = *(const f32x4*)(a.e + base + off);
             to.e[1] = *(const f32x4*)(a.e + base + 16 + off);
         }
-        if (has_z) {
-            const int row = min(16 * (w & 3) + (int)(lane & 15), n - 1);
-            const raw* const y = (const raw*)a.dout + (start + row) * a.do_t + hv * a.do_h + d0 + 4 * (lane >> 4);
-            to.y[0] = load4<In>(y);
-            to.y[1] = load4<In>(y + 16);
-        }
+        const int row = min(16 * (w & 3) + (int)(lane & 15), n - 1);
+        const raw* const y = (const raw*)a.dout + (start + row) * a.do_t + hv * a.do_h + d0 + 16 * second + 4 * (lane >> 4);
+#pragma unroll
+        for (int i = 0; i < YH; ++i) to.y[i] = load4<In>(y + 16 * i);
     };
     auto put = [&](bf16x8* to, const Tokens& from, unsigned lane) {
         bf16x8 t[3];
         split8<3>(from.x[0], from.x[1], t);
 #pragma unroll
-        for (int k = 0; k < 3; ++k) to[((has_z ? 0 : 12) + (w & 3) * 3 + k) * 64 + lane] = t[k];
-        if (has_z) {
-            const bool live = 16 * (w & 3) + (int)(lane & 15) < n;
-            bf16x8 y[NI];
-            split8<NI>(live ? from.y[0] : splat4(0.f), live ? from.y[1] : splat4(0.f), y);
+        for (int k = 0; k < 3; ++k) to[(12 * second + (w & 3) * 3 + k) * 64 + lane] = t[k];
+        const bool live = 16 * (w & 3) + (int)(lane & 15) < n;
 #pragma unroll
-            for (int k = 0; k < NI; ++k) to[(24 + (w & 3) * NI + k) * 64 + lane] = y[k];
+        for (int i = 0; i < YH; ++i) {
+            u32x2 y[NI];
+            split4<NI>(live ? from.y[i] : splat4(0.f), y);
+#pragma unroll
+            for (int k = 0; k < NI; ++k) ((u32x2*)(to + (24 + (w & 3) * NI + k) * 64 + lane))[second + i] = y[k];
         }
         if constexpr (W == 4) {
             split8<3>(from.e[0], from.e[1], t);
