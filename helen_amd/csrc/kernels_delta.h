@@ -698,6 +698,8 @@ __device__ __forceinline__ void issue_loads() { asm volatile("" ::: "memory"); }
 // fragments) stay on one of them.  The grid is padded to a multiple of eight.
 __device__ __forceinline__ unsigned xcd_order(unsigned block, unsigned grid) { return (block & 7) * (grid >> 3) + (block >> 3); }
 
+constexpr int kColumnTiles = 2;    // of a four-wave chain
+
 // Where a wave of a chain finds its left-hand fragments: uniform bases plus the lane
 template <typename In, int DK>
 struct ChainAddress {
@@ -816,14 +818,17 @@ __device__ __forceinline__ void load_state(const float* state, const void* zeros
 }
 
 // ------------------------------------------------------------------------------------------------
-// The chain: a workgroup per (sequence, value head, 16 NC columns of the state).  Each of its four waves owns a quarter of
+// The chain: a workgroup per (sequence, value head, 32 columns of the state).  Each of its four waves owns a quarter of
 // the ROWS of everything: token tile w of R, U and O, the dk tiles of S from w DK/64 on.  The other waves' rows of a right-hand
 // operand (S, R, U) come through LDS as bf16 terms, three barriers a chunk; every left-hand fragment is read by
 // one wave only, straight into registers, and the next chunk's are loaded into the registers the present chunk is done with.
+// What bounds it: two workgroups a CU take turns at the matrix pipe (a chunk of one is 228 products of 16 cycles on each SIMD at
+// width 128, bf16) and at the loads (90 KB of fragments a chunk).  Two column tiles share every left-hand fragment; with one, 64
+// sequences of 1000 tokens took 249 us, with two 170 us (4 key heads and 8 value heads of 128, bf16).
 // ------------------------------------------------------------------------------------------------
-template <typename In, int DK, int PT, bool KEEP, int NC>
+template <typename In, int DK, int PT, bool KEEP>
 __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_kernel(const DeltaArgs a) {
-    constexpr int NI = In::kTerms, KS = DK / 32, MW = DK / 64;
+    constexpr int NC = kColumnTiles, NI = In::kTerms, KS = DK / 32, MW = DK / 64;
     typedef typename In::raw raw;
     __shared__ bf16x8 sbuf[KS * 3 * NC * 64], xbuf[2 * 3 * NC * 64], ubuf[2 * PT * NC * 64], cbuf[2 * 3 * NC * 64];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -898,31 +903,24 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
     lds_barrier();
     for (int c = 0; c < chunks; ++c) {
         const int next = min(c + 1, chunks - 1), n = sp.len - c * kDeltaChunk;
-        // Two sums each where there is one column tile: a product waits for the one before it in the same sum
-        constexpr int NS = NC == 1 ? 2 : 1;
-        f32x4 R[NC], O[NC], U[NC], sums[NS][NC], osum[NS][NC];
-        bf16x8 b[KS][NC][3];
+        f32x4 R[NC], O[NC], U[NC];
 #pragma unroll
-        for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-            for (int k = 0; k < NS; ++k) sums[k][nc] = osum[k][nc] = splat4(0.f);
+        for (int nc = 0; nc < NC; ++nc) R[nc] = O[nc] = splat4(0.f);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc) {
-                shared_frag<3, NC>(sbuf, ks, nc, lane, b[ks][nc]);
-                sums[ks % NS][nc] = mm(kf[ks], b[ks][nc], sums[ks % NS][nc]);
-                if constexpr (NC > 1) osum[0][nc] = mm(qf[ks], b[ks][nc], osum[0][nc]);
+                bf16x8 b[3];
+                shared_frag<3, NC>(sbuf, ks, nc, lane, b);
+                R[nc] = mm(kf[ks], b, R[nc]);
+                O[nc] = mm(qf[ks], b, O[nc]);
             }
         const f32x4 after = ec, step = beta, head = eb;
         const float hold = whole;
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float x = NS == 2 ? sums[0][nc][r] + sums[NS - 1][nc][r] : sums[0][nc][r];
-                R[nc][r] = v[r].get(nc) - eb[r] * x;
-            }
+            for (int r = 0; r < 4; ++r) R[nc][r] = v[r].get(nc) - eb[r] * R[nc][r];
             share_tile<3, NC>(xbuf, w, nc, lane, R[nc]);
         }
         load_k(next);
@@ -939,13 +937,6 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
             u1 = mm(tf[1], x[1], u1);
             U[nc] = u0 + u1;
         }
-        // one column tile: Q S0 fills the wait for U
-        if constexpr (NC == 1) {
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) osum[ks % NS][0] = mm(qf[ks], b[ks][0], osum[ks % NS][0]);
-        }
-#pragma unroll
-        for (int nc = 0; nc < NC; ++nc) O[nc] = NS == 2 ? osum[0][nc] + osum[NS - 1][nc] : osum[0][nc];
         if constexpr (KEEP) store_tile<NC>(a.e + ((at.vslot + (size_t)c * a.hv) * kDeltaChunk + 16 * w) * a.dv_width, tile_at, U);
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
@@ -1298,7 +1289,7 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
 // over at the same place, ragged sequences too).
 constexpr int kComputeUnits = 256;
 inline bool chains_are_few(const DeltaArgs& a) { return (long)a.nseq * a.hv * (a.dv_width / 16) <= kComputeUnits; }
-inline unsigned chain_grid(const DeltaArgs& a, int columns) {
+inline unsigned chain_grid(const DeltaArgs& a, int columns) {      // columns of the state a workgroup takes
     return (unsigned)(((long)a.nseq * a.hv * (a.dv_width / columns) + 7) / 8 * 8);
 }
 

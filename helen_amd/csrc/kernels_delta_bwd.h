@@ -15,9 +15,9 @@
 namespace helen {
 
 // The reverse chain, built like delta_forward_kernel: wave w owns token tile w of dO, dU and Z and its quarter of dS's rows.
-template <typename In, int DK, int NC>
+template <typename In, int DK>
 __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_kernel(const DeltaArgs a) {
-    constexpr int NI = In::kTerms, KS = DK / 32, MW = DK / 64;
+    constexpr int NC = kColumnTiles, NI = In::kTerms, KS = DK / 32, MW = DK / 64;
     typedef typename In::raw raw;
     __shared__ bf16x8 sbuf[KS * 3 * NC * 64], ybuf[2 * NI * NC * 64], wbuf[2 * 3 * NC * 64], dbuf[2 * 3 * NC * 64], zbuf[2 * 3 * NC * 64];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -100,21 +100,16 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
     lds_barrier();
     for (int c = chunks - 1; c >= 0; --c) {
         const int next = max(c - 1, 0), n = sp.len - c * kDeltaChunk;
-        constexpr int NS = NC == 1 ? 2 : 1;
-        f32x4 E[NS][NC], P[2][NC];
+        f32x4 D[NC], P[2][NC];
 #pragma unroll
-        for (int nc = 0; nc < NC; ++nc) {
-            P[0][nc] = P[1][nc] = splat4(0.f);
-#pragma unroll
-            for (int k = 0; k < NS; ++k) E[k][nc] = splat4(0.f);
-        }
+        for (int nc = 0; nc < NC; ++nc) D[nc] = P[0][nc] = P[1][nc] = splat4(0.f);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc) {
                 bf16x8 b[3];
                 shared_frag<3, NC>(sbuf, ks, nc, lane, b);
-                E[ks % NS][nc] = mm(kf[ks], b, E[ks % NS][nc]);
+                D[nc] = mm(kf[ks], b, D[nc]);
             }
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc)
@@ -131,11 +126,10 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
             f32x4 x;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float e = NS == 2 ? E[0][nc][r] + E[NS - 1][nc][r] : E[0][nc][r];
-                E[0][nc][r] = beta_of(beta[r]) * (ec[r] * e + a.scale * (P[0][nc][r] + P[1][nc][r]));
+                D[nc][r] = beta_of(beta[r]) * (ec[r] * D[nc][r] + a.scale * (P[0][nc][r] + P[1][nc][r]));
                 x[r] = a.scale * eb[r] * dout(nc, r);
             }
-            share_tile<3, NC>(dbuf, w, nc, lane, E[0][nc]);
+            share_tile<3, NC>(dbuf, w, nc, lane, D[nc]);
             share_tile<3, NC>(wbuf, w, nc, lane, x);
         }
         load_rows(next);

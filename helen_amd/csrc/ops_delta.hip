@@ -111,7 +111,7 @@ template <typename In, int DK, int PT, bool KEEP>
 void launch_forward(const DeltaArgs& a, hipStream_t s) {
     if (a.tokens > 0) hipLaunchKernelGGL((delta_prep_kernel<In, DK, PT, KEEP>), dim3((unsigned)a.slots * a.hk), dim3(256), 0, s, a);
     if (chains_are_few(a)) hipLaunchKernelGGL((delta_forward_long_kernel<In, DK, PT, KEEP>), dim3(chain_grid(a, 16)), dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((delta_forward_kernel<In, DK, PT, KEEP, 2>), dim3(chain_grid(a, 32)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((delta_forward_kernel<In, DK, PT, KEEP>), dim3(chain_grid(a, 16 * kColumnTiles)), dim3(256), 0, s, a);
 }
 template <typename In, int DK, int PT>
 void launch_forward(const DeltaArgs& a, int keep, hipStream_t s) {

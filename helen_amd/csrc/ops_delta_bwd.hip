@@ -9,7 +9,7 @@ namespace {
 template <typename In, int DK>
 void launch(const DeltaArgs& a, hipStream_t s) {
     if (chains_are_few(a)) hipLaunchKernelGGL((delta_backward_long_kernel<In, DK>), dim3(chain_grid(a, 16)), dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((delta_backward_kernel<In, DK, 2>), dim3(chain_grid(a, 32)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((delta_backward_kernel<In, DK>), dim3(chain_grid(a, 16 * kColumnTiles)), dim3(256), 0, s, a);
     if (a.tokens == 0) return;
     const dim3 chunks((unsigned)a.slots * a.hk), block(DK * 4);
     if (a.group == 1) hipLaunchKernelGGL((delta_grads_kernel<In, DK, In::kTerms == 3 ? 3 : 2, false>), chunks, block, 0, s, a);
