@@ -364,6 +364,8 @@ constexpr int kTriStride = 68;    // floats per row of a 64 x 64 matrix in LDS: 
 // What becomes a left-hand operand is computed transposed, (Q K^T)^T = K Q^T: a result tile then already lies as that operand
 // (lane = row, four neighbouring columns), so P goes from the accumulators to memory, and A to LDS and back in whole
 // fragments.  K^T comes from the matrix pipe too: K times a selection of 16 columns is K's tile with lane = dk.
+// What bounds it: bandwidth, mostly its own writing.  16,384 tokens, 16 key and 32 value heads of 128, bf16: 0.60 GB in 115 us,
+// 5.2 TB/s, what a large copy reaches; the four workgroups a CU (35 KB of LDS, 128 registers) took it there from 140 us.
 // ------------------------------------------------------------------------------------------------
 template <typename In, int DK, int PT, bool BWD>
 __global__ __launch_bounds__(256, In::kTerms == 1 ? (BWD ? 3 : 4) : 1) void delta_prep_kernel(const DeltaArgs a) {
@@ -822,9 +824,10 @@ __device__ __forceinline__ void load_state(const float* state, const void* zeros
 // the ROWS of everything: token tile w of R, U and O, the dk tiles of S from w DK/64 on.  The other waves' rows of a right-hand
 // operand (S, R, U) come through LDS as bf16 terms, three barriers a chunk; every left-hand fragment is read by
 // one wave only, straight into registers, and the next chunk's are loaded into the registers the present chunk is done with.
-// What bounds it: two workgroups a CU take turns at the matrix pipe (a chunk of one is 228 products of 16 cycles on each SIMD at
-// width 128, bf16) and at the loads (90 KB of fragments a chunk).  Two column tiles share every left-hand fragment; with one, 64
-// sequences of 1000 tokens took 249 us, with two 170 us (4 key heads and 8 value heads of 128, bf16).
+// What bounds it: the way through a chunk.  Two workgroups fit a CU (registers), so a SIMD has two waves to hide behind each other
+// 108 products of 16 cycles, some 400 VALU instructions (the splits), 85 LDS accesses and 45 loads a wave and chunk.  64
+// sequences of 1000 tokens, 4 heads of 128, bf16: 169 us, 150 TFLOP/s of the recurrence's own 6 Dk Dv a token.  Two column
+// tiles share every left-hand fragment: with one it takes 244 us, and keeping the states 370 instead of 232 (32 x 1000, 8 heads).
 // ------------------------------------------------------------------------------------------------
 template <typename In, int DK, int PT, bool KEEP>
 __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_kernel(const DeltaArgs a) {
@@ -1013,11 +1016,15 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
 // The same for few long chains: 16 columns of the state, and eight waves.  A wave alone on its SIMD issues an instruction
 // every 5 to 9 cycles, and the chain is as long as what its waves have to issue; so waves 0 .. 3 do only what the next chunk
 // waits for (R, E and S), and waves 4 .. 7, one on each SIMD beside them, the output and every store: from S, E and U as they
-// pass by in LDS, a phase later.
+// pass by in LDS, a phase later.  Waves whose row tile of T and P has one k step run code of their own (without: 510 us, not 473).
+// What bounds it: a chunk is 4,000 to 4,400 cycles, in which the CU's loads come back in order, 83 KB of them, 64 bytes a cycle at
+// best.  16,384 tokens, 32 heads of 128, bf16: 473 us, 109 TFLOP/s; the four-wave kernel on 256 chains takes 1.4 times as long.
 // ------------------------------------------------------------------------------------------------
 // Fetches a chunk's fragments into the XCD's L2 before the workgroups of its head need them.  They all come by at the same time, and
 // loads that miss there run at half the rate of loads that hit (28 - 35 against 16 cycles a KiB and CU).  Each of the head's
-// waves takes another part: one load, a lane a line of 128 bytes.  The value is handed to `settle` a chunk later.
+// waves takes another part: one load, a lane a line of 128 bytes.  The value is handed to `settle` a chunk later.  8191 tokens in two
+// sequences, 16 heads of 128: forward chain 215 us without, 194 with, reverse chain 226 and 182; 16,384 tokens x 32 heads: no
+// difference.
 struct Piece {
     const bf16x8* at;
     int kib;

@@ -68,6 +68,11 @@ def _inner(t, bytes_=0):
     return t
 
 
+def _like(t):
+    """A new contiguous tensor of t's shape and type (empty_like is the cheapest allocation a call can make)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
@@ -300,7 +305,7 @@ def delta_rule_step(q, k, v, g, beta, state, slots=None, scale=None, out=None):
             _fail("slots must be int32 [%d]" % n)
         slots = slots.contiguous()
     if out is None:
-        o = torch.empty((n, hv, dv), dtype=q.dtype, device=q.device)
+        o = _like(v)
     else:
         o = _output("out", out, (n, hv, dv), q.dtype, device)
     q, k, v = _inner(q), _inner(k), _inner(v, 16)
@@ -355,16 +360,16 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
     -> (y, mean, rstd), mean and rstd float32 [...] for layer_norm_backward."""
     device, code, kind, width = _norm_sizes(x, weight, bias)
     rows = _rows(x)
-    shape, at = x.shape, x.device
+    shape = x.shape
     if out is None:
-        y = torch.empty(shape, dtype=x.dtype, device=at)
+        y = _like(x)
     else:
         y = _output("out", out, tuple(shape), x.dtype, device)
         if y.dim() != 2 and not y.is_contiguous():
             _fail("out must be contiguous or have two dimensions")
     flat = y if y.dim() == 2 else y.view(-1, width)
-    mean = torch.empty(shape[:-1], dtype=torch.float32, device=at)
-    rstd = torch.empty(shape[:-1], dtype=torch.float32, device=at)
+    mean = x.new_empty(shape[:-1], dtype=torch.float32)
+    rstd = torch.empty_like(mean)
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     op = _NORM.pack(_NORM.size, device, code, kind, width, rows.shape[0], eps, rows.data_ptr(), rows.stride(0), _ptr(weight),
@@ -400,7 +405,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd, bias=True):
     mean, rstd = mean.contiguous(), rstd.contiguous()
     weight = None if weight is None else weight.contiguous()
     of = torch.float32 if weight is None else weight.dtype
-    dx = torch.empty(shape, dtype=x.dtype, device=at)
+    dx = _like(x)
     flat = dx if dx.dim() == 2 else dx.view(-1, width)
     dweight = None if weight is None else torch.empty(width, dtype=of, device=at)
     dbias = torch.empty(width, dtype=of, device=at) if bias else None
