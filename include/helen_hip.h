@@ -280,8 +280,12 @@ enum { HELEN_TYPE_FP32 = 0, HELEN_TYPE_BF16 = 1, HELEN_TYPE_FP16 = 2 };
  *                  offsets[i + 1] (empty ones are allowed; rows behind the last one belong to none); NULL: tokens is a
  *                  multiple of sequences and all have the same length.  Offsets that break this give wrong values, never an
  *                  access out of range.
+ *   g              a decay: at most 0, -inf included.  Positive values work as long as e to their sum over 64 tokens is finite.
+ *                  A NaN or an infinity in a token's inputs reaches its whole chunk of 64 tokens (counted from the sequence's
+ *                  start), earlier ones included, and what follows, in its own sequence and heads alone.
  *   q, k           [tokens, heads_k, width_k];  v, o, d_o  [tokens, heads_v, width_v];  g, beta  [tokens, heads_v];
  *                  stride[0] between tokens, stride[1] between heads.  q, k, v, d_o: 16-byte aligned, strides too.
+ *                  Tokens of q, k, v, o, d_o at most 2^24 elements apart.  o overlaps no input.
  *   initial_state  float32 [sequences, heads_v, width_k, width_v] or NULL (zero);  final_state the same or NULL
  *   o              NULL: only the states are wanted.  Rows behind the last sequence are left as they are, or set to zero
  *                  where zero_tail is 1.
@@ -351,7 +355,7 @@ int helen_delta_rule_step(const HelenDeltaStep* op, void* stream);
 
 /*
  * Layer norm over the last dimension: y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps), statistics float32.
- *   x, y, dy, dx   [rows, width], rows `*_stride` elements apart, any alignment of their type
+ *   x, y, dy, dx   [rows, width], rows `*_stride` elements apart, any alignment of their type; y may be x
  *   weight, bias   [width] of weight_dtype (dtype's own or float32), either may be NULL (one, zero)
  *   mean, rstd     float32 [rows]: written by the forward call (or NULL), read by the backward call
  * Backward: dx, and dweight / dbias of weight_dtype, either NULL if not wanted: sums over all rows in a fixed order
