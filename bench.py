@@ -679,8 +679,9 @@ def end_to_end(windows_per_rank, workers, batch, weights, rank, world, single_de
          (helen_amd/stitch_stream.py) = `polish_seconds`, and the FASTA compared with the two-phase stitch of the same
          prediction files.
     Every bench rank writes its share of the inputs (direct emitter of libhelen_io.so, RAM-backed directory); rank 0 then
-    runs the commands, which start their OWN process per device exactly as the CLI does, while the other bench ranks
-    sleep on a file (not in a collective: their GPUs must be idle).  Returns the `end_to_end` object on rank 0."""
+    runs the commands, which start their OWN process per device exactly as the CLI does; the other bench ranks return and
+    end (their GPUs must be idle, and a GPU takes a limited number of processes at once).  Nothing collective may follow on
+    any rank.  Returns the `end_to_end` object on rank 0."""
     import shutil
     import tempfile
 
@@ -713,7 +714,7 @@ def end_to_end(windows_per_rank, workers, batch, weights, rank, world, single_de
     if d is None:
         return {"value": None, "skipped": "/dev/shm may take %.1f GB, the %d-rank leg needs %.1f GB"
                                           % (ram_backed_budget_bytes() / 1e9, world, need / 1e9)} if rank == 0 else None
-    done = os.path.join(d, "done")
+    together = os.path.join(d, "together")
     try:
         img_dir = os.path.join(d, "img")
         os.makedirs(img_dir, exist_ok=True)
@@ -732,10 +733,15 @@ def end_to_end(windows_per_rank, workers, batch, weights, rank, world, single_de
             write_error = next((e for e in gather_strings(dist, world, write_error or "") if e), None)
         if write_error:
             return {"value": None, "error": "writing the synthetic inputs failed: " + write_error} if rank == 0 else None
-        if rank != 0:
-            while not os.path.exists(done):
+        others = gather_strings(dist, world, str(os.getpid()))[1:] if dist is not None else []
+        if rank != 0:                   # (a rank that ends while another is still inside the exchange breaks its connection)
+            while not os.path.exists(together):
                 time.sleep(0.05)
             return None
+        open(together, "w").close()
+        limit = time.time() + 20.0
+        while any(os.path.exists("/proc/" + pid) for pid in others) and time.time() < limit:
+            time.sleep(0.05)
         model = os.path.join(d, "model.pkl")
         ModelHandler.save_model(weights, None, 128, 1, 0, model)
         out = os.path.join(d, "out")
@@ -858,8 +864,9 @@ def end_to_end(windows_per_rank, workers, batch, weights, rank, world, single_de
                         "%.1f s to %s" % (world, windows_per_rank, t_write, os.path.dirname(d))}
     finally:
         if rank == 0:
-            open(done, "w").close()
-            time.sleep(0.2)
+            if dist is not None and not os.path.exists(together):       # (an error on the way: the others wait for this)
+                open(together, "w").close()
+                time.sleep(0.2)
             shutil.rmtree(d, ignore_errors=True)
 
 
@@ -1221,7 +1228,8 @@ def main():
             out["end_to_end"] = e2e
         print(json.dumps(out))
     if dist is not None:
-        dist.all_reduce(token_cpu)
+        if e2e_windows <= 0:       # (otherwise the ranks end one by one, see end_to_end)
+            dist.all_reduce(token_cpu)
         dist.destroy_process_group()
 
 
