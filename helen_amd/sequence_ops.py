@@ -202,10 +202,9 @@ class _Call(object):
 
     def forward(self, o, keep, zero_tail=0):
         """-> (final_state, workspace); `o` None computes the states alone."""
-        at = self.q.device
-        final = torch.empty(self.state_shape, dtype=torch.float32, device=at)
+        final = self.q.new_empty(self.state_shape, dtype=torch.float32)
         size = self.work[1 if keep else 0]
-        work = torch.empty(size, dtype=torch.uint8, device=at)
+        work = self.q.new_empty(size, dtype=torch.uint8)
         rc = _lib.load().helen_delta_rule_forward(self.pack(o, final, zero_tail), int(keep), work.data_ptr(), size,
                                                   _stream(self.device))
         if rc:
@@ -238,7 +237,7 @@ def delta_rule(q, k, v, g, beta, scale=None, initial_state=None, offsets=None, o
     call = _Call(q, k, v, g, beta, scale, initial_state, offsets)
     shape = (call.tokens, call.hv, call.dv)
     if out is None:
-        o, tail = torch.empty(shape, dtype=call.dtype, device=q.device), 0 if call.whole else 1
+        o, tail = _like(v), 0 if call.whole else 1
     else:
         o, tail = _output("out", out, shape, call.dtype, call.device), 0
     final, work = call.forward(o, keep, tail)
@@ -263,11 +262,9 @@ def delta_rule_backward(d_o, q, k, v, g, beta, scale=None, initial_state=None, o
         _same_gpu("saved", saved, call.device)
         if saved.dtype != torch.uint8 or saved.numel() != kept or not saved.is_contiguous():
             _fail("saved is not what delta_rule(..., keep=True) returned for these arguments")
-    at = q.device
-    dq, dk, dv = (torch.empty(t.shape, dtype=call.dtype, device=at) for t in (q, k, v))
-    dg, dbeta = (torch.empty(g.shape, dtype=torch.float32, device=at) for _ in range(2))
-    d_initial = torch.empty(call.state_shape, dtype=torch.float32, device=at)
-    work = torch.empty(own, dtype=torch.uint8, device=at)
+    dq, dk, dv, dg, dbeta = _like(q), _like(k), _like(v), _like(g), _like(beta)
+    d_initial = q.new_empty(call.state_shape, dtype=torch.float32)
+    work = q.new_empty(own, dtype=torch.uint8)
     op = call.pack(d_o=d_o, d_final=d_final, grads=(dq, dk, dv, dg, dbeta, d_initial))
     rc = _lib.load().helen_delta_rule_backward(op, saved.data_ptr(), kept, work.data_ptr(), own, _stream(call.device))
     if rc:
@@ -393,7 +390,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd, bias=True):
     -> (dx, dweight, dbias); dweight is None without a weight, dbias None with bias=False.  dweight and dbias have the weight's
     type (float32 without one) and are summed in float32 in a fixed order."""
     device, code, kind, width = _norm_sizes(x, weight, None)
-    shape, at = x.shape, x.device
+    shape = x.shape
     _same_gpu("dy", dy, device)
     if dy.dtype != x.dtype or dy.shape != shape:
         _fail("dy must be %s %s" % (x.dtype, tuple(shape)))
@@ -404,14 +401,15 @@ def layer_norm_backward(dy, x, weight, mean, rstd, bias=True):
     rows, drows = _rows(x), _rows(dy)
     mean, rstd = mean.contiguous(), rstd.contiguous()
     weight = None if weight is None else weight.contiguous()
-    of = torch.float32 if weight is None else weight.dtype
     dx = _like(x)
     flat = dx if dx.dim() == 2 else dx.view(-1, width)
-    dweight = None if weight is None else torch.empty(width, dtype=of, device=at)
-    dbias = torch.empty(width, dtype=of, device=at) if bias else None
+    dweight = None if weight is None else torch.empty_like(weight)
+    dbias = None
+    if bias:
+        dbias = x.new_empty(width, dtype=torch.float32) if weight is None else torch.empty_like(weight)
     n = rows.shape[0]
     size = _norm_bytes(code, kind, width, n)
-    work = torch.empty(size, dtype=torch.uint8, device=at)
+    work = x.new_empty(size, dtype=torch.uint8)
     op = _NORM.pack(_NORM.size, device, code, kind, width, n, 0.0, rows.data_ptr(), rows.stride(0), _ptr(weight), 0, 0, 0,
                     mean.data_ptr(), rstd.data_ptr(), drows.data_ptr(), drows.stride(0), flat.data_ptr(), flat.stride(0),
                     _ptr(dweight), _ptr(dbias))
