@@ -179,7 +179,7 @@ struct DeltaArgs {
     bf16x8* zeros;              // three fragments of zeros: the k step of a triangle's row tile that lies above the diagonal
     int zero_tail;              // rows behind the last sequence: 1 = zero them, 0 = leave them
     // workspace: fragments per (slot, key head) and per (slot, value head)
-    bf16x8 *kf, *ktf, *qf, *qtf;
+    bf16x8 *kf, *ktf, *qf, *qtf;           // (kf, qf null where the chain takes the inputs' rows)
     bf16x8 *tf, *ttf, *pf, *ptf;
     f32x4* dots;                // kept: [slot, hk][10 tiles][K K^T | Q K^T][lane]
     float* sc;                  // [slot, hv][4][64]: beta, e^b (its last one is e^{b_C}), e^c, beta e^c
@@ -364,8 +364,8 @@ constexpr int kTriStride = 68;    // floats per row of a 64 x 64 matrix in LDS: 
 // What becomes a left-hand operand is computed transposed, (Q K^T)^T = K Q^T: a result tile then already lies as that operand
 // (lane = row, four neighbouring columns), so P goes from the accumulators to memory, and A to LDS and back in whole
 // fragments.  K^T comes from the matrix pipe too: K times a selection of 16 columns is K's tile with lane = dk.
-// What bounds it: bandwidth, mostly its own writing.  16,384 tokens, 16 key and 32 value heads of 128, bf16: 0.60 GB in 115 us,
-// 5.2 TB/s, what a large copy reaches; the four workgroups a CU (35 KB of LDS, 128 registers) took it there from 140 us.
+// What bounds it: bandwidth, mostly its own writing.  16,384 tokens, 16 key and 32 value heads of 128, bf16: 0.60 GB in 109 us,
+// 5.5 TB/s, what a large copy reaches; the four workgroups a CU (35 KB of LDS, 128 registers) took it there from 140 us.
 // ------------------------------------------------------------------------------------------------
 template <typename In, int DK, int PT, bool BWD>
 __global__ __launch_bounds__(256, In::kTerms == 1 ? (BWD ? 3 : 4) : 1) void delta_prep_kernel(const DeltaArgs a) {
@@ -424,31 +424,48 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? (BWD ? 3 : 4) : 1) void delt
         bf16x8 kf[KS][NI], qf[KS][NI];
         const int row = 16 * w + j;
         const bool live = row < n;
-        const raw* kp = (const raw*)a.k + (start + (live ? row : 0)) * a.k_t + h * a.k_h + 4 * q;
-        const raw* qp = (const raw*)a.q + (start + (live ? row : 0)) * a.q_t + h * a.q_h + 4 * q;
-        f32x4 kx[KS][2], qx[KS][2];
+        const raw* kp = (const raw*)a.k + (start + (live ? row : 0)) * a.k_t + h * a.k_h + 8 * q;
+        const raw* qp = (const raw*)a.q + (start + (live ? row : 0)) * a.q_t + h * a.q_h + 8 * q;
+        if constexpr (NI == 1) {
+            const bf16x8 none = __builtin_bit_cast(bf16x8, (u32x4){0u, 0u, 0u, 0u});
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                kf[ks][0] = *(const bf16x8*)(kp + 32 * ks);
+                qf[ks][0] = *(const bf16x8*)(qp + 32 * ks);
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                kf[ks][0] = live ? kf[ks][0] : none;
+                qf[ks][0] = live ? qf[ks][0] : none;
+            }
+        } else {
+            f32x4 kx[KS][2], qx[KS][2];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    kx[ks][i] = load4<In>(kp + 32 * ks + 4 * i);
+                    qx[ks][i] = load4<In>(qp + 32 * ks + 4 * i);
+                }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const f32x4 zero = splat4(0.f);
+                split8<NI>(live ? kx[ks][0] : zero, live ? kx[ks][1] : zero, kf[ks]);
+                split8<NI>(live ? qx[ks][0] : zero, live ? qx[ks][1] : zero, qf[ks]);
+            }
+        }
+        const size_t rows_at = (((size_t)slot * a.hk + h) * 4 + w) * KS * NI * 64;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                kx[ks][i] = load4<In>(kp + 32 * ks + 16 * i);
-                qx[ks][i] = load4<In>(qp + 32 * ks + 16 * i);
-            }
-        bf16x8* const kto = a.kf + (((size_t)slot * a.hk + h) * 4 + w) * KS * NI * 64;
-        bf16x8* const qto = a.qf + (kto - a.kf);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const f32x4 zero = splat4(0.f);
-            split8<NI>(live ? kx[ks][0] : zero, live ? kx[ks][1] : zero, kf[ks]);
-            split8<NI>(live ? qx[ks][0] : zero, live ? qx[ks][1] : zero, qf[ks]);
 #pragma unroll
             for (int t = 0; t < NI; ++t) {
                 kfr[((w * KS + ks) * NI + t) * 64 + lane] = kf[ks][t];
                 qfr[((w * KS + ks) * NI + t) * 64 + lane] = qf[ks][t];
-                (kto + (ks * NI + t) * 64)[lane] = kf[ks][t];
-                (qto + (ks * NI + t) * 64)[lane] = qf[ks][t];
+                if (NI > 1 || BWD || a.kf) {
+                    (a.kf + rows_at + (ks * NI + t) * 64)[lane] = kf[ks][t];
+                    (a.qf + rows_at + (ks * NI + t) * 64)[lane] = qf[ks][t];
+                }
             }
-        }
         // K^T, Q^T: half (w & 1) of the fragments of token step w >> 1, dk tiles 2 ks + i
         const unsigned one = q == (j >> 2) ? 0x3f80u << (16 * (j & 1)) : 0u;
         const unsigned lo = j & 2 ? 0u : one, hi = j & 2 ? one : 0u;
@@ -712,16 +729,8 @@ struct ChainAddress {
     unsigned lane;
     __device__ __forceinline__ ChainAddress(const DeltaArgs& a, const Span& sp, int h, int head, int wave, int l)
         : zeros(a.zeros), kslot((size_t)sp.slot * a.hk + h), vslot((size_t)sp.slot * a.hv + head), hk(a.hk), hv(a.hv), w(wave), lane(l) {}
-    // row tile w of K or Q
-    __device__ __forceinline__ void rows(const bf16x8* from, int c, bf16x8 (&to)[DK / 32][NI]) const {
-        from += (kslot + (size_t)c * hk) * kSlot + w * (DK / 32) * NI * 64;
-#pragma unroll
-        for (int ks = 0; ks < DK / 32; ++ks)
-#pragma unroll
-            for (int t = 0; t < NI; ++t) to[ks][t] = (from + (ks * NI + t) * 64)[lane];
-    }
-    // the same with the k steps in the order first, first + 1, ..: to[i] is step (first + i) % (DK / 32)
-    __device__ __forceinline__ void rows_from(int first, const bf16x8* from, int c, bf16x8 (&to)[DK / 32][NI]) const {
+    // row tile w of K or Q with the k steps in the order first, first + 1, ..: to[i] is step (first + i) % (DK / 32)
+    __device__ __forceinline__ void rows(int first, const bf16x8* from, int c, bf16x8 (&to)[DK / 32][NI]) const {
         from += (kslot + (size_t)c * hk) * kSlot + w * (DK / 32) * NI * 64;
 #pragma unroll
         for (int i = 0; i < DK / 32; ++i)
@@ -772,6 +781,30 @@ struct ChainAddress {
         }
     }
 };
+// Row tile w of K or Q straight from the inputs: in bf16 the rows are the fragments; dead rows stand for the last live one (what
+// comes of them meets zeros).  The preparation then writes 32 KB less a key head and chunk, and the loads are of 64 bytes a row.
+// 64 sequences of 1000 tokens, 4 heads of 128: preparation 88 -> 60 us, chain 169 -> 176.  Chains that also write their states lose more
+// than that (32 x 1000 tokens: 97 -> 84, 230 -> 247, reverse 235 -> 243), and so do the eight-wave ones (16,384 tokens: 116 -> 91,
+// 473 -> 555): they take the fragments.
+template <typename In, int DK>
+struct InputRows {
+    typedef typename In::raw raw;
+    const raw* from;
+    long stride;
+    unsigned col;
+    int row, len;
+    __device__ __forceinline__ InputRows(const void* rows, long t, long head_at, const Span& sp, int w, int lane)
+        : from((const raw*)rows + sp.begin * t + head_at), stride(t), col(8 * (lane >> 4)), row(16 * w + (lane & 15)), len(sp.len) {}
+    __device__ __forceinline__ void load(int c, bf16x8 (&to)[DK / 32][1]) const {
+        const raw* const p = from + c * kDeltaChunk * stride;
+        const unsigned off = min(row, len - c * kDeltaChunk - 1) * (unsigned)stride + col;
+#pragma unroll
+        for (int i = 0; i < DK / 32; ++i) to[i][0] = *(const bf16x8*)(p + 32 * i + off);
+    }
+};
+// Dk of row 4 q + r of tile t of the states as the chains hold them: state_row(t) + 8 q + r
+__device__ __forceinline__ constexpr int state_row(int tile) { return 32 * (tile >> 1) + 4 * (tile & 1); }
+
 // Element offsets of a lane's four rows of a chunk in a [tokens, ..] tensor (the host has checked that they fit 32 bits); rows
 // from n on stand for row n - 1.
 struct RowOffsets {
@@ -802,7 +835,7 @@ __device__ __forceinline__ void store_tile(float* to, const unsigned (&at)[4], c
     }
 }
 
-// A wave's rows of a state [DK, dv]: MW row tiles, 16 rows of stride `dv` apart; zero where there is no state.  The loads are not
+// A wave's rows of a state [DK, dv]: MW row tiles; zero where there is no state.  The loads are not
 // conditional (they read some zeros then): behind a skipped load the compiler waits for everything that is in flight.
 template <int MW, int NC>
 __device__ __forceinline__ void load_state(const float* state, const void* zeros, size_t at, int dv, f32x4 (&S)[MW][NC]) {
@@ -813,7 +846,7 @@ __device__ __forceinline__ void load_state(const float* state, const void* zeros
     for (int i = 0; i < MW; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const Cols x = Cols::load(from + (16 * i + r) * stride);
+            const Cols x = Cols::load(from + (4 * i + r) * stride);
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc) S[i][nc][r] = state ? x.get(nc) : 0.f;
         }
@@ -826,8 +859,8 @@ __device__ __forceinline__ void load_state(const float* state, const void* zeros
 // one wave only, straight into registers, and the next chunk's are loaded into the registers the present chunk is done with.
 // What bounds it: the way through a chunk.  Two workgroups fit a CU (registers), so a SIMD has two waves to hide behind each other
 // 108 products of 16 cycles, some 400 VALU instructions (the splits), 85 LDS accesses and 45 loads a wave and chunk.  64
-// sequences of 1000 tokens, 4 heads of 128, bf16: 169 us, 150 TFLOP/s of the recurrence's own 6 Dk Dv a token.  Two column
-// tiles share every left-hand fragment: with one it takes 244 us, and keeping the states 370 instead of 232 (32 x 1000, 8 heads).
+// sequences of 1000 tokens, 4 heads of 128, bf16: 176 us, 143 TFLOP/s of the recurrence's own 6 Dk Dv a token.  Two column
+// tiles share every left-hand fragment: 169 us with fragments of K and Q, and with one tile 244, and keeping the states 370 instead of 232 (32 x 1000, 8 heads).
 // ------------------------------------------------------------------------------------------------
 template <typename In, int DK, int PT, bool KEEP>
 __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_kernel(const DeltaArgs a) {
@@ -843,7 +876,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
     const int col = NC * (16 * (item % groups) + j);    // column tile nc has columns 16 NC g + NC j + nc: a lane's are neighbours
     const Span sp = span_of(a, s);
     const int chunks = (sp.len + kDeltaChunk - 1) / kDeltaChunk;
-    const size_t st = (((size_t)s * a.hv + hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col;
+    const size_t st = (((size_t)s * a.hv + hv) * DK + state_row(MW * w) + 8 * q) * a.dv_width + col;
 
     f32x4 S[MW][NC];
     load_state<MW, NC>(a.s0, a.zeros, st, a.dv_width, S);
@@ -868,14 +901,24 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = Columns<In, NC>::load(p + vrow.at[r]);
     };
-    auto load_k = [&](int c) { at.rows(a.kf, c, kf); };
-    auto load_q = [&](int c) { at.rows(a.qf, c, qf); };
+    const InputRows<In, DK> krows(a.k, a.k_t, h * a.k_h, sp, w, lane), qrows(a.q, a.q_t, h * a.q_h, sp, w, lane);
+    auto load_k = [&](int c) {
+        if constexpr (NI == 1 && !KEEP) krows.load(c, kf);
+        else at.rows(0, a.kf, c, kf);
+    };
+    auto load_q = [&](int c) {
+        if constexpr (NI == 1 && !KEEP) qrows.load(c, qf);
+        else at.rows(0, a.qf, c, qf);
+    };
     auto load_kt = [&](int c) { at.columns(a.ktf, c, kt); };
     auto load_t = [&](int c) { at.template triangle<3>(a.tf, c, tf); };
     auto load_p = [&](int c) { at.template triangle<PT>(a.pf, c, pf); };
-    unsigned tile_at[4];                            // D tile of a [.., dv] matrix: this lane's four elements
+    unsigned tile_at[4], state_at[4];               // D tile of a [.., dv] matrix, of a state: this lane's four elements
 #pragma unroll
-    for (int r = 0; r < 4; ++r) tile_at[r] = (4 * q + r) * a.dv_width + col;
+    for (int r = 0; r < 4; ++r) {
+        tile_at[r] = (4 * q + r) * a.dv_width + col;
+        state_at[r] = (8 * q + r) * a.dv_width + col;
+    }
     auto share_state = [&](int c) {
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
@@ -889,9 +932,9 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
             }
         }
         if constexpr (KEEP) {
-            float* to = a.states + ((at.vslot + (size_t)c * a.hv) * DK + 16 * MW * w) * a.dv_width;
+            float* to = a.states + ((at.vslot + (size_t)c * a.hv) * DK + state_row(MW * w)) * a.dv_width;
 #pragma unroll
-            for (int i = 0; i < MW; ++i) store_tile<NC>(to + (size_t)16 * i * a.dv_width, tile_at, S[i]);
+            for (int i = 0; i < MW; ++i) store_tile<NC>(to + (size_t)4 * i * a.dv_width, state_at, S[i]);
         }
     };
     if (chunks > 0) {
@@ -1006,9 +1049,9 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
         lds_barrier();
     }
     if (a.s1) {
-        float* const to = a.s1 + (((size_t)s * a.hv + hv) * DK + 16 * MW * w) * a.dv_width;
+        float* const to = a.s1 + (((size_t)s * a.hv + hv) * DK + state_row(MW * w)) * a.dv_width;
 #pragma unroll
-        for (int i = 0; i < MW; ++i) store_tile<NC>(to + (size_t)16 * i * a.dv_width, tile_at, S[i]);
+        for (int i = 0; i < MW; ++i) store_tile<NC>(to + (size_t)4 * i * a.dv_width, state_at, S[i]);
     }
 }
 
@@ -1075,14 +1118,17 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
     const int chunks = (sp.len + kDeltaChunk - 1) / kDeltaChunk;
     const int row = 16 * w + 4 * q;
     const ChainAddress<In, DK> at(a, sp, h, hv, w, lane);
-    unsigned tile_at[4];
+    unsigned tile_at[4], state_at[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) tile_at[r] = (4 * q + r) * a.dv_width + col;
+    for (int r = 0; r < 4; ++r) {
+        tile_at[r] = (4 * q + r) * a.dv_width + col;
+        state_at[r] = (8 * q + r) * a.dv_width + col;
+    }
 
     auto chain = [&](auto two_) {
         constexpr bool TWO = decltype(two_)::value;
         f32x4 S[MW][1];
-        load_state<MW, 1>(a.s0, a.zeros, (((size_t)s * a.hv + hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col, a.dv_width, S);
+        load_state<MW, 1>(a.s0, a.zeros, (((size_t)s * a.hv + hv) * DK + state_row(MW * w) + 8 * q) * a.dv_width + col, a.dv_width, S);
         struct Operands {        // of one chunk; the next one's are loaded into a second set meanwhile
             bf16x8 kf[KS][NI], kt[MW][2][NI], tf[TWO ? 2 : 1][3];
             f32x4 eb, weight;     // weight: beta e^c
@@ -1091,7 +1137,7 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
         } first, second;
         bf16x8 own[3];
         RowOffsets vrow(a.v_t, row, col);
-        auto load_k = [&](int c, Operands& to) { at.rows_from(OWN ? w : 0, a.kf, c, to.kf); };
+        auto load_k = [&](int c, Operands& to) { at.rows(OWN ? w : 0, a.kf, c, to.kf); };
         auto load_tokens = [&](int c, Operands& to) {
             const float* sc = a.sc + (at.vslot + (size_t)c * a.hv) * 256;
             to.eb = *(const f32x4*)(sc + 64 + row);
@@ -1191,9 +1237,9 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
             step(c + 1, second, first);
         }
         if (a.s1) {
-            float* const to = a.s1 + (((size_t)s * a.hv + hv) * DK + 16 * MW * w) * a.dv_width;
+            float* const to = a.s1 + (((size_t)s * a.hv + hv) * DK + state_row(MW * w)) * a.dv_width;
 #pragma unroll
-            for (int i = 0; i < MW; ++i) store_tile<1>(to + (size_t)16 * i * a.dv_width, tile_at, S[i]);
+            for (int i = 0; i < MW; ++i) store_tile<1>(to + (size_t)4 * i * a.dv_width, state_at, S[i]);
         }
     };
     auto output = [&](auto two_) {
@@ -1236,7 +1282,7 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
         };
         unsigned fetched = 0;
         if (chunks > 0) {
-            at.rows(a.qf, 0, qf);
+            at.rows(0, a.qf, 0, qf);
             load_scales(0);
             settle(fetch_chunk(min(1, chunks - 1)));
             settle(fetch_chunk(min(2, chunks - 1)));
@@ -1260,17 +1306,17 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
                 sum[ks & 1] = mm(b, qf[ks], sum[ks & 1]);
             }
             if constexpr (KEEP) {
-                float* const to = a.states + ((at.vslot + (size_t)c * a.hv) * DK + 16 * MW * w) * a.dv_width;
+                float* const to = a.states + ((at.vslot + (size_t)c * a.hv) * DK + state_row(MW * w)) * a.dv_width;
 #pragma unroll
                 for (int i = 0; i < MW; ++i) {
                     const f32x4 x[1] = {sfull[(MW * w + i) * 64 + lane]};
-                    store_tile<1>(to + (size_t)16 * i * a.dv_width, tile_at, x);
+                    store_tile<1>(to + (size_t)4 * i * a.dv_width, state_at, x);
                 }
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) O[r] = eb * (sum[0][r] + sum[1][r]);
             const f32x4 step = beta;
-            at.rows(a.qf, next, qf);
+            at.rows(0, a.qf, next, qf);
             load_scales(next);
             issue_loads();
             lds_barrier();

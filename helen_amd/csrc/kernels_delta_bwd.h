@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
     const int col = NC * (16 * (item % groups) + j);
     const Span sp = span_of(a, s);
     const int chunks = (sp.len + kDeltaChunk - 1) / kDeltaChunk;
-    const size_t st = (((size_t)s * a.hv + hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col;
+    const size_t st = (((size_t)s * a.hv + hv) * DK + state_row(MW * w) + 8 * q) * a.dv_width + col;
 
     f32x4 S[MW][NC];
     load_state<MW, NC>(a.ds1, a.zeros, st, a.dv_width, S);
@@ -42,13 +42,14 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
     const int row = 16 * w + 4 * q;
     const ChainAddress<In, DK> at(a, sp, h, hv, w, lane);
     RowOffsets yrow(a.do_t, row, col);
-    unsigned tile_at[4], dv_at[4];
+    unsigned tile_at[4], state_at[4], dv_at[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
+        state_at[r] = (8 * q + r) * a.dv_width + col;
         tile_at[r] = (4 * q + r) * a.dv_width + col;
         dv_at[r] = (row + r) * a.hv * a.dv_width + col;
     }
-    auto load_rows = [&](int c) { at.rows(a.kf, c, kf); };
+    auto load_rows = [&](int c) { at.rows(0, a.kf, c, kf); };
     auto load_columns = [&](int c) {
         at.columns(a.ktf, c, kt);
         at.columns(a.qtf, c, qt);
@@ -84,9 +85,9 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
             share_tile<NI, NC>(ybuf, w, nc, lane,
                                (f32x4){dout(nc, 0), dout(nc, 1), dout(nc, 2), dout(nc, 3)});
         }
-        float* to = a.dstates + ((at.vslot + (size_t)c * a.hv) * DK + 16 * MW * w) * a.dv_width;
+        float* to = a.dstates + ((at.vslot + (size_t)c * a.hv) * DK + state_row(MW * w)) * a.dv_width;
 #pragma unroll
-        for (int i = 0; i < MW; ++i) store_tile<NC>(to + (size_t)16 * i * a.dv_width, tile_at, S[i]);
+        for (int i = 0; i < MW; ++i) store_tile<NC>(to + (size_t)4 * i * a.dv_width, state_at, S[i]);
     };
     if (chunks > 0) {
         const int c = chunks - 1;
@@ -201,9 +202,9 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
         lds_barrier();
     }
     if (a.ds0) {
-        float* const to = a.ds0 + (((size_t)s * a.hv + hv) * DK + 16 * MW * w) * a.dv_width;
+        float* const to = a.ds0 + (((size_t)s * a.hv + hv) * DK + state_row(MW * w)) * a.dv_width;
 #pragma unroll
-        for (int i = 0; i < MW; ++i) store_tile<NC>(to + (size_t)16 * i * a.dv_width, tile_at, S[i]);
+        for (int i = 0; i < MW; ++i) store_tile<NC>(to + (size_t)4 * i * a.dv_width, state_at, S[i]);
     }
 }
 
@@ -228,14 +229,17 @@ __global__ __launch_bounds__(512) void delta_backward_long_kernel(const DeltaArg
     const int chunks = (sp.len + kDeltaChunk - 1) / kDeltaChunk;
     const int row = 16 * w + 4 * q;
     const ChainAddress<In, DK> at(a, sp, h, hv, w, lane);
-    unsigned tile_at[4];
+    unsigned tile_at[4], state_at[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) tile_at[r] = (4 * q + r) * a.dv_width + col;
+    for (int r = 0; r < 4; ++r) {
+        tile_at[r] = (4 * q + r) * a.dv_width + col;
+        state_at[r] = (8 * q + r) * a.dv_width + col;
+    }
 
     auto chain = [&](auto two_) {
         constexpr bool TWO = decltype(two_)::value;
         f32x4 S[MW][1];
-        load_state<MW, 1>(a.ds1, a.zeros, (((size_t)s * a.hv + hv) * DK + 16 * MW * w + 4 * q) * a.dv_width + col, a.dv_width, S);
+        load_state<MW, 1>(a.ds1, a.zeros, (((size_t)s * a.hv + hv) * DK + state_row(MW * w) + 8 * q) * a.dv_width + col, a.dv_width, S);
         struct Operands {
             bf16x8 kf[KS][NI], kt[MW][2][NI], tt[TWO ? 2 : 1][3];
             f32x4 beta, eb, ec;
@@ -244,7 +248,7 @@ __global__ __launch_bounds__(512) void delta_backward_long_kernel(const DeltaArg
         bf16x8 own[3];
         auto load_k = [&](int c, Operands& to) {
             const float* sc = a.sc + (at.vslot + (size_t)c * a.hv) * 256;
-            at.rows_from(OWN ? w : 0, a.kf, c, to.kf);
+            at.rows(OWN ? w : 0, a.kf, c, to.kf);
             to.beta = *(const f32x4*)(sc + row);
             to.ec = *(const f32x4*)(sc + 128 + row);
         };
@@ -339,9 +343,9 @@ __global__ __launch_bounds__(512) void delta_backward_long_kernel(const DeltaArg
             step(c - 1, second, first);
         }
         if (a.ds0) {
-            float* const to = a.ds0 + (((size_t)s * a.hv + hv) * DK + 16 * MW * w) * a.dv_width;
+            float* const to = a.ds0 + (((size_t)s * a.hv + hv) * DK + state_row(MW * w)) * a.dv_width;
 #pragma unroll
-            for (int i = 0; i < MW; ++i) store_tile<1>(to + (size_t)16 * i * a.dv_width, tile_at, S[i]);
+            for (int i = 0; i < MW; ++i) store_tile<1>(to + (size_t)4 * i * a.dv_width, state_at, S[i]);
         }
     };
     auto output = [&](auto two_) {
@@ -424,11 +428,11 @@ __global__ __launch_bounds__(512) void delta_backward_long_kernel(const DeltaArg
             from_p();
             at.transposed(a.ptf, after, pt);
             {
-                float* const to = a.dstates + ((at.vslot + (size_t)c * a.hv) * DK + 16 * MW * w) * a.dv_width;
+                float* const to = a.dstates + ((at.vslot + (size_t)c * a.hv) * DK + state_row(MW * w)) * a.dv_width;
 #pragma unroll
                 for (int i = 0; i < MW; ++i) {
                     const f32x4 x[1] = {sfull[(MW * w + i) * 64 + lane]};
-                    store_tile<1>(to + (size_t)16 * i * a.dv_width, tile_at, x);
+                    store_tile<1>(to + (size_t)4 * i * a.dv_width, state_at, x);
                 }
             }
             issue_loads();
@@ -486,7 +490,7 @@ __device__ __forceinline__ float sum_from(float x, int lane) {        // over th
 // ------------------------------------------------------------------------------------------------
 // dQ, dK, dbeta and dg of one chunk: a workgroup of DK / 16 waves per (slot, key head).  The value heads of the key head follow
 // one another and are summed in registers: no atomics, one order.
-//   64 x DK results: wave w has dk tile w of all four token tiles
+//   64 x DK results: wave w has dk tile w (column j is state_row(w) + 8 (j / 4) + j % 4) of all four token tiles
 //   64 x 64 results: the ten tiles on and below the diagonal go round the waves
 // dv is walked 32 columns a step: Z, E and dO of the step as fragments in LDS (two buffers, one barrier a step), the rows of
 // S0 and dS1 straight into the registers of the one wave that needs them.  What it waits for is memory, so loads run two
@@ -559,8 +563,8 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
     } toks[2];
     auto load_rows = [&](int at, Rows& to, unsigned lane) {      // step `at` of all heads' steps
         const int step = min(at, last), head = step / steps, d0 = 32 * (step - head * steps);
-        const size_t base = (((size_t)slot * a.hv + h * a.group + head) * DK + 16 * w) * a.dv_width + d0;
-        const unsigned off = (lane & 15) * a.dv_width + 4 * (lane >> 4);
+        const size_t base = (((size_t)slot * a.hv + h * a.group + head) * DK + state_row(w)) * a.dv_width + d0;
+        const unsigned off = (8 * (lane >> 2 & 3) + (lane & 3)) * a.dv_width + 4 * (lane >> 4);
         to.s[0] = *(const f32x4*)(a.states + base + off);
         to.s[1] = *(const f32x4*)(a.states + base + 16 + off);
         to.d[0] = *(const f32x4*)(a.dstates + base + off);
@@ -849,7 +853,7 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
         for (int r = 0; r < 4; ++r) {
             const int t = 16 * m + 4 * q + r;
             if (t >= n) continue;
-            const size_t to = ((size_t)(start + t) * a.hk + h) * DK + 16 * w + j;
+            const size_t to = ((size_t)(start + t) * a.hk + h) * DK + state_row(w) + 8 * (j >> 2) + (j & 3);
             ((raw*)a.dq)[to] = In::from_f32(dQ[m][r]);
             ((raw*)a.dk)[to] = In::from_f32(dK[m][r]);
         }

@@ -27,9 +27,10 @@ size_t carve(const HelenDeltaRule& op, int keep, void* base, DeltaArgs* a) {
     const size_t rows = ks * (op.width_k / 8) * ni * 64, tri = vs * kTriFrags * 64;
     a->sink = c.take<float>(256);
     a->zeros = c.take<bf16x8>(3 * 64);
-    a->kf = c.take<bf16x8>(rows);
+    const bool from_inputs = ni == 1 && !keep && !chains_are_few(*a);       // (delta_forward_kernel's InputRows)
+    a->kf = from_inputs ? nullptr : c.take<bf16x8>(rows);
     a->ktf = c.take<bf16x8>(rows);
-    a->qf = c.take<bf16x8>(rows);
+    a->qf = from_inputs ? nullptr : c.take<bf16x8>(rows);
     a->tf = c.take<bf16x8>(tri * 3);
     a->pf = c.take<bf16x8>(tri * pt);
     a->sc = c.take<float>(vs * 256);

@@ -291,6 +291,31 @@ def test_delta_rule_more_chains_than_compute_units(dtype, hk, hv, dk, dv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dk", [64, 128])
+def test_delta_rule_more_chains_with_strided_and_short_inputs(dk):
+    """The chains that read q and k themselves: slices of one projection, heads first, broadcast keys, the last row the last of
+    its allocation."""
+    lengths = [70, 64, 1, 131, 33]
+    n = sum(lengths)
+    x = gpu(make(lengths, 4, 8, dk, 128, torch.bfloat16, True, seed=dk))
+    off = torch.tensor(ends(lengths), dtype=torch.int32).cuda()
+    kw = dict(initial_state=x["initial"], offsets=off)
+
+    def run(q, k):
+        return ops.delta_rule(q, k, x["v"], x["g"], x["beta"], **kw)
+    want = run(x["q"], x["k"])
+    kept = ops.delta_rule(x["q"], x["k"], x["v"], x["g"], x["beta"], keep=True, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(want, kept))
+    rows = torch.cat([x["q"].reshape(n, -1), x["k"].reshape(n, -1)], 1)
+    first = {m: x[m].transpose(0, 1).contiguous().transpose(0, 1) for m in ("q", "k")}
+    for q, k in ((rows[:, :4 * dk].unflatten(1, (4, dk)), rows[:, 4 * dk:].unflatten(1, (4, dk))), (first["q"], first["k"])):
+        assert q.data_ptr() % 16 == 0 and not q.is_contiguous()
+        assert all(torch.equal(a, b) for a, b in zip(run(q, k), want))
+    one = x["k"][:1].expand(n, -1, -1)
+    assert all(torch.equal(a, b) for a, b in zip(run(x["q"], one), run(x["q"], one.contiguous())))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("hk, hv, dk, dv", [(1, 2, 128, 128), (2, 2, 64, 256)])
 def test_delta_rule_six_chunks(dtype, hk, hv, dk, dv):
