@@ -18,9 +18,10 @@
 // them stay fp32-class whatever the inputs' type.  Decays between two positions are sums of the g between them, never a
 // difference of two running sums: a strong decay (or g = -inf, a reset) costs the other positions no digits.
 //
-// Fragments.  lane l: j = l & 15, q = l >> 4.  The k index of an MFMA may be permuted if both operands agree; here element
-// e = 0..7 of lane quarter q is k = 32 s + (e < 4 ? 4 q + e : 16 + 4 q + e - 4), which is exactly how two stacked D tiles of
-// 16 rows lie in the accumulators.  A result (S, U, R) thus becomes the next product's B operand without any exchange.
+// Fragments.  lane l: j = l & 15, q = l >> 4.  The k index of an MFMA may be permuted if both operands agree, so that a result (S,
+// U, R) becomes the next product's B operand without any exchange: two stacked D tiles lie in the accumulators as element
+// e = 0 .. 7 of lane quarter q.  Over tokens that is k = 32 s + (e < 4 ? 4 q + e : 16 + 4 q + e - 4); over dk the rows of S go to the
+// tiles in such an order (state_row) that it is k = 32 s + 8 q + e, eight neighbours of a row of K or Q.
 #pragma once
 #include "kernels_common.h"
 
