@@ -4,7 +4,7 @@
 // The right-hand form of o needs only the OLD state, so S^T k and S^T q are one pass over a state that stays in registers
 // between its load and its store: a state is read once and written once, and that is the whole cost.
 // Bound by bandwidth: 252 streams, 32 heads of 128 x 128: 1.06 GB in 211 us, 5.0 TB/s.  One stream is a launch and its host side:
-// 10.3 us a call, where a fill of one line costs 3.8.
+// 10.2 us a call, where a fill of one line costs 3.8.
 // A workgroup takes 64 columns of one row's head; rows of the call that name the same slot are successive tokens of one stream and
 // are taken in order by the workgroup of the first of them.
 #pragma once

@@ -427,7 +427,7 @@ def _no_capture(what):
 
 class DeltaRule(torch.autograd.Function):
     """delta_rule under autograd: DeltaRule.apply(q, k, v, g, beta, scale, initial_state, offsets) -> (o, final_state).
-    Keeps the forward call's states for the backward pass.  Not capturable: the explicit calls are."""
+    Keeps the forward call's states for the backward pass.  Neither pass may be captured: the explicit calls may."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, scale=None, initial_state=None, offsets=None):
@@ -451,7 +451,8 @@ class DeltaRule(torch.autograd.Function):
 
 
 class LayerNorm(torch.autograd.Function):
-    """layer_norm under autograd: LayerNorm.apply(x, weight, bias, eps) -> y.  Not capturable: the explicit calls are."""
+    """layer_norm under autograd: LayerNorm.apply(x, weight, bias, eps) -> y.  Neither pass may be captured: the explicit calls
+    may."""
 
     @staticmethod
     def forward(ctx, x, weight=None, bias=None, eps=1e-5):
