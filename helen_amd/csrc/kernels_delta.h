@@ -14,9 +14,10 @@
 //
 // Arithmetic: as in the fp32x3 recurrence, an fp32 value is the sum of three bf16 terms and a product of two such values the
 // six leading products of terms on v_mfma_f32_16x16x32_bf16 with fp32 accumulation.  bf16 inputs are ONE term (their products
-// with S are exact), fp16 inputs two, fp32 inputs three; S, U, R, T and P keep three, so states and everything that feeds
-// them stay fp32-class whatever the inputs' type.  Decays between two positions are sums of the g between them, never a
-// difference of two running sums: a strong decay (or g = -inf, a reset) costs the other positions no digits.
+// with S are exact), fp16 inputs two, fp32 inputs three; whatever is computed (S, E, U, R, T, P, the gradients' G and H) has
+// three in every product, so a call with 16-bit inputs gives the float32 call's results, rounded once.  Decays between two
+// positions are sums of the g between them, never a difference of two running sums: a strong decay (or g = -inf, a reset) costs
+// the other positions no digits.
 //
 // Fragments.  lane l: j = l & 15, q = l >> 4.  The k index of an MFMA may be permuted if both operands agree, so that a result (S,
 // U, R) becomes the next product's B operand without any exchange: two stacked D tiles lie in the accumulators as element
@@ -365,10 +366,11 @@ constexpr int kTriStride = 68;    // floats per row of a 64 x 64 matrix in LDS: 
 // What becomes a left-hand operand is computed transposed, (Q K^T)^T = K Q^T: a result tile then already lies as that operand
 // (lane = row, four neighbouring columns), so P goes from the accumulators to memory, and A to LDS and back in whole
 // fragments.  K^T comes from the matrix pipe too: K times a selection of 16 columns is K's tile with lane = dk.
-// What bounds it: bandwidth, mostly its own writing.  16,384 tokens, 16 key and 32 value heads of 128, bf16: 0.60 GB in 109 us,
-// 5.5 TB/s, what a large copy reaches; the four workgroups a CU (35 KB of LDS, 128 registers) took it there from 140 us.
+// What bounds it: bandwidth, mostly its own writing.  16,384 tokens, 16 key and 32 value heads of 128, bf16: 0.65 GB in 117 us,
+// 5.6 TB/s, what a large copy reaches; the four workgroups a CU (35 KB of LDS, 128 registers) took it there (from 140 us to 109, then with
+// P in two terms).
 // ------------------------------------------------------------------------------------------------
-template <typename In, int DK, int PT, bool BWD>
+template <typename In, int DK, bool BWD>
 __global__ __launch_bounds__(256, In::kTerms == 1 ? (BWD ? 3 : 4) : 1) void delta_prep_kernel(const DeltaArgs a) {
     constexpr int NI = In::kTerms, KS = DK / 32;
     constexpr int kTile = 64 + 4;               // an operand tile in LDS: [column / 4][row] x 4, column groups 17 apart
@@ -557,11 +559,11 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? (BWD ? 3 : 4) : 1) void delt
             atile[(tm[t] * (tm[t] + 1) / 2 + tn[t]) * 64 + lane] = A;
         }
         auto put_p = [&](int f, const f32x4 lo, const f32x4 hi) {
-            bf16x8 t[PT];
-            split8<PT>(lo, hi, t);
-            bf16x8* const to = a.pf + (vslot * kTriFrags + f) * PT * 64;
+            bf16x8 t[3];
+            split8<3>(lo, hi, t);
+            bf16x8* const to = a.pf + (vslot * kTriFrags + f) * 3 * 64;
 #pragma unroll
-            for (int k = 0; k < PT; ++k) (to + k * 64)[lane] = t[k];
+            for (int k = 0; k < 3; ++k) (to + k * 64)[lane] = t[k];
         };
         if (w == 0) {
             put_p(0, P[0], splat4(0.f));
@@ -859,15 +861,17 @@ __device__ __forceinline__ void load_state(const float* state, const void* zeros
 // operand (S, R, U) come through LDS as bf16 terms, three barriers a chunk; every left-hand fragment is read by
 // one wave only, straight into registers, and the next chunk's are loaded into the registers the present chunk is done with.
 // What bounds it: the way through a chunk.  Two workgroups fit a CU (registers), so a SIMD has two waves to hide behind each other
-// 108 products of 16 cycles, some 400 VALU instructions (the splits), 85 LDS accesses and 45 loads a wave and chunk.  64
-// sequences of 1000 tokens, 4 heads of 128, bf16: 176 us, 143 TFLOP/s of the recurrence's own 6 Dk Dv a token.  Two column
-// tiles share every left-hand fragment: 169 us with fragments of K and Q, and with one tile 244, and keeping the states 370 instead of 232 (32 x 1000, 8 heads).
+// 120 products of 16 cycles, some 400 VALU instructions (the splits), 85 LDS accesses and 45 loads a wave and chunk.  64
+// sequences of 1000 tokens, 4 heads of 128, bf16: 188 us, 134 TFLOP/s of the recurrence's own 6 Dk Dv a token (176 us with P
+// and U in two terms, when bf16 results were 1.1e-4 of their norm from a float32 evaluation's, not 3.5e-5).  Two column tiles
+// share every left-hand fragment; with one it was 244 us instead of 169, and keeping the states 370 instead of 232 (32 x 1000, 8
+// heads; both with fragments of K and Q, and two terms).
 // ------------------------------------------------------------------------------------------------
-template <typename In, int DK, int PT, bool KEEP>
+template <typename In, int DK, bool KEEP>
 __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_kernel(const DeltaArgs a) {
     constexpr int NC = kColumnTiles, NI = In::kTerms, KS = DK / 32, MW = DK / 64;
     typedef typename In::raw raw;
-    __shared__ bf16x8 sbuf[KS * 3 * NC * 64], xbuf[2 * 3 * NC * 64], ubuf[2 * PT * NC * 64], cbuf[2 * 3 * NC * 64];
+    __shared__ bf16x8 sbuf[KS * 3 * NC * 64], xbuf[2 * 3 * NC * 64], ubuf[2 * 3 * NC * 64], cbuf[2 * 3 * NC * 64];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int j = lane & 15, q = lane >> 4;
     const int groups = a.dv_width / (16 * NC);
@@ -882,7 +886,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
     f32x4 S[MW][NC];
     load_state<MW, NC>(a.s0, a.zeros, st, a.dv_width, S);
 
-    bf16x8 kf[KS][NI], qf[KS][NI], kt[MW][2][NI], tf[2][3], pf[2][PT];
+    bf16x8 kf[KS][NI], qf[KS][NI], kt[MW][2][NI], tf[2][3], pf[2][3];
     f32x4 beta, eb, ec;
     float whole;
     Columns<In, NC> v[4];
@@ -913,7 +917,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
     };
     auto load_kt = [&](int c) { at.columns(a.ktf, c, kt); };
     auto load_t = [&](int c) { at.template triangle<3>(a.tf, c, tf); };
-    auto load_p = [&](int c) { at.template triangle<PT>(a.pf, c, pf); };
+    auto load_p = [&](int c) { at.template triangle<3>(a.pf, c, pf); };
     unsigned tile_at[4], state_at[4];               // D tile of a [.., dv] matrix, of a state: this lane's four elements
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -989,7 +993,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
         for (int nc = 0; nc < NC; ++nc) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) U[nc][r] *= step[r];
-            share_tile<PT, NC>(ubuf, w, nc, lane, U[nc]);
+            share_tile<3, NC>(ubuf, w, nc, lane, U[nc]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) U[nc][r] *= after[r];
             share_tile<3, NC>(cbuf, w, nc, lane, U[nc]);
@@ -1013,22 +1017,19 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
 #pragma unroll
                 for (int i = 0; i < MW; ++i) S[i][nc] = mm(kt[i][ks], x, S[i][nc]);
             }
-        bf16x8 x[2][NC][PT];
-#pragma unroll
-        for (int nc = 0; nc < NC; ++nc) {
-            shared_frag<PT, NC>(ubuf, 0, nc, lane, x[0][nc]);
-            shared_frag<PT, NC>(ubuf, 1, nc, lane, x[1][nc]);
-        }
         load_kt(next);
         issue_loads();
         if (c + 1 < chunks) share_state(next);
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
+            bf16x8 x[2][3];
+            shared_frag<3, NC>(ubuf, 0, nc, lane, x[0]);
+            shared_frag<3, NC>(ubuf, 1, nc, lane, x[1]);
             f32x4 p0 = splat4(0.f);
 #pragma unroll
             for (int r = 0; r < 4; ++r) O[nc][r] *= head[r];
-            p0 = mm<PT, PT, PT - 1>(pf[0], x[0][nc], p0);
-            O[nc] = mm<PT, PT, PT - 1>(pf[1], x[1][nc], O[nc]) + p0;
+            p0 = mm(pf[0], x[0], p0);
+            O[nc] = mm(pf[1], x[1], O[nc]) + p0;
         }
         load_p(next);
         issue_loads();
@@ -1062,7 +1063,8 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
 // waits for (R, E and S), and waves 4 .. 7, one on each SIMD beside them, the output and every store: from S, E and U as they
 // pass by in LDS, a phase later.  Waves whose row tile of T and P has one k step run code of their own (without: 510 us, not 473).
 // What bounds it: a chunk is 4,000 to 4,400 cycles, in which the CU's loads come back in order, 83 KB of them, 64 bytes a cycle at
-// best.  16,384 tokens, 32 heads of 128, bf16: 473 us, 109 TFLOP/s; the four-wave kernel on 256 chains takes 1.4 times as long.
+// best.  16,384 tokens, 32 heads of 128, bf16: 498 us, 103 TFLOP/s (473 with P, U and S in two terms for the
+// output); the four-wave kernel on 256 chains takes 1.4 times as long.
 // ------------------------------------------------------------------------------------------------
 // Fetches a chunk's fragments into the XCD's L2 before the workgroups of its head need them.  They all come by at the same time, and
 // loads that miss there run at half the rate of loads that hit (28 - 35 against 16 cycles a KiB and CU).  Each of the head's
@@ -1101,12 +1103,12 @@ __device__ __forceinline__ void between_products() {
 // loop alone (it waits for what any path into the loop might have left).
 __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
-template <typename In, int DK, int PT, bool KEEP>
+template <typename In, int DK, bool KEEP>
 __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs a) {
     constexpr int NI = In::kTerms, KS = DK / 32, MW = DK / 64;
     constexpr bool OWN = MW == 2;        // a wave's rows of S are a whole k step: it takes that one from its registers
     typedef typename In::raw raw;
-    __shared__ bf16x8 sbuf[KS * 3 * 64], xbuf[2 * 3 * 64], ubuf[2 * PT * 64], cbuf[2 * 3 * 64];
+    __shared__ bf16x8 sbuf[KS * 3 * 64], xbuf[2 * 3 * 64], ubuf[2 * 3 * 64], cbuf[2 * 3 * 64];
     __shared__ f32x4 ebuf[4 * 64], sfull[KEEP ? 4 * MW * 64 : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
     const int j = lane & 15, q = lane >> 4;
@@ -1247,7 +1249,7 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
         constexpr bool TWO = decltype(two_)::value;
         // The output transposed, S^T Q^T and U^T P^T (the operands change places, the fragments are the same): a lane then has
         // four neighbouring columns of one token, one store of a chunk
-        bf16x8 qf[KS][NI], pf[TWO ? 2 : 1][PT];
+        bf16x8 qf[KS][NI], pf[TWO ? 2 : 1][3];
         f32x4 beta, O = splat4(0.f);
         float eb = 0.f;
         const int token = 16 * w + j;
@@ -1259,15 +1261,15 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
         };
         // o of chunk c: O + P U, and its store
         auto finish = [&](int c) {
-            bf16x8 x[2][PT];
-            shared_frag<PT, 1>(ubuf, 0, 0, lane, x[0]);
+            bf16x8 x[2][3];
+            shared_frag<3, 1>(ubuf, 0, 0, lane, x[0]);
             if constexpr (TWO) {
-                shared_frag<PT, 1>(ubuf, 1, 0, lane, x[1]);
+                shared_frag<3, 1>(ubuf, 1, 0, lane, x[1]);
                 f32x4 p0 = splat4(0.f);
-                p0 = mm<PT, PT, PT - 1>(x[0], pf[0], p0);
-                O = mm<PT, PT, PT - 1>(x[1], pf[1], O) + p0;
+                p0 = mm(x[0], pf[0], p0);
+                O = mm(x[1], pf[1], O) + p0;
             } else {
-                O = mm<PT, PT, PT - 1>(x[0], pf[0], O);
+                O = mm(x[0], pf[0], O);
             }
             raw* const to = (raw*)a.o + (sp.begin + c * kDeltaChunk) * a.o_t + hv * a.o_h;
             const float y[4] = {a.scale * O[0], a.scale * O[1], a.scale * O[2], a.scale * O[3]};
@@ -1276,9 +1278,9 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
         const int part = 4 * (item % groups) + w;
         auto fetch_chunk = [&](int c) {
             const bf16x8* const tri = a.tf + (at.vslot + (size_t)c * a.hv) * kTriFrags * 3 * 64;
-            const bf16x8* const pri = a.pf + (at.vslot + (size_t)c * a.hv) * kTriFrags * PT * 64;
+            const bf16x8* const pri = a.pf + (at.vslot + (size_t)c * a.hv) * kTriFrags * 3 * 64;
             const size_t k0 = (at.kslot + (size_t)c * a.hk) * at.kSlot;
-            const Piece piece[5] = {{a.kf + k0, DK / 8 * NI}, {tri, kTriFrags * 3}, {a.ktf + k0, DK / 8 * NI}, {a.qf + k0, DK / 8 * NI}, {pri, kTriFrags * PT}};
+            const Piece piece[5] = {{a.kf + k0, DK / 8 * NI}, {tri, kTriFrags * 3}, {a.ktf + k0, DK / 8 * NI}, {a.qf + k0, DK / 8 * NI}, {pri, kTriFrags * 3}};
             return fetch(piece, part, lane);
         };
         unsigned fetched = 0;
@@ -1294,16 +1296,15 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
             settle(fetched);
             fetched = fetch_chunk(min(c + kFetchAhead, chunks - 1));
             if (c > 0) finish(c - 1);
-            at.template triangle<PT>(a.pf, c, pf);
+            at.template triangle<3>(a.pf, c, pf);
             issue_loads();
             lds_barrier();
-            // (the terms of S that a product of PT terms an operand takes)
             f32x4 sum[2] = {splat4(0.f), splat4(0.f)};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                bf16x8 b[PT];
+                bf16x8 b[3];
 #pragma unroll
-                for (int t = 0; t < PT; ++t) b[t] = sbuf[(ks * 3 + t) * 64 + lane];
+                for (int t = 0; t < 3; ++t) b[t] = sbuf[(ks * 3 + t) * 64 + lane];
                 sum[ks & 1] = mm(b, qf[ks], sum[ks & 1]);
             }
             if constexpr (KEEP) {
@@ -1328,7 +1329,7 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) U[r] *= step[r];
-            share_tile<PT, 1>(ubuf, w, 0, lane, U);
+            share_tile<3, 1>(ubuf, w, 0, lane, U);
             lds_barrier();
         }
         if (chunks > 0) finish(chunks - 1);

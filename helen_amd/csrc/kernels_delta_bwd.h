@@ -495,17 +495,17 @@ __device__ __forceinline__ float sum_from(float x, int lane) {        // over th
 // dv is walked 32 columns a step: Z, E and dO of the step as fragments in LDS (two buffers, one barrier a step), the rows of
 // S0 and dS1 straight into the registers of the one wave that needs them.  What it waits for is memory, so loads run two
 // steps ahead, over the ends of the heads too, and every wave stages as much as the others.
-// What bounds it: one workgroup a CU (107 KB of LDS, 256 registers) has nothing to hide its start (a sixth of its time) and its
+// What bounds it: one workgroup a CU (128 KB of LDS, 256 registers) has nothing to hide its start (a sixth of its time) and its
 // 64 x 64 part (a third) behind; products and LDS reads of the steps are 40 % of it.  32 x 1000 tokens, 4 key and 8 value heads
-// of 128, bf16: 370 us for 0.85 GB of states, Z and E, 2.3 TB/s (500 us with loads one step ahead).
+// of 128, bf16: 375 us for 0.85 GB of states, Z and E, 2.3 TB/s (500 us with loads one step ahead).
 // ------------------------------------------------------------------------------------------------
-template <typename In, int DK, int PT, bool SHARED>
+template <typename In, int DK, bool SHARED>
 __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) {
     constexpr int NI = In::kTerms, W = DK / 16, TPW = (10 + W - 1) / W, RB = 64 / W;
     typedef typename In::raw raw;
     constexpr int kStage = 4 * (6 + NI);
     __shared__ bf16x8 stage[2 * kStage * 64];
-    __shared__ bf16x8 fr[PT * (8 + 2 * kTriFrags) * 64];
+    __shared__ bf16x8 fr[3 * (8 + 2 * kTriFrags) * 64];
     __shared__ __attribute__((aligned(16))) Decays dec;
     __shared__ float bs[64], scl[192], sums[2][W][64], dbeta[64], gamma[W], part[W][64];
     static_assert(sizeof(stage) >= 3 * 64 * kTriStride * 4, "the 64 x 64 gradients take the stage's place");
@@ -753,7 +753,7 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
             }
         }
         lds_barrier();
-        // A operands of the products with K and Q: G + G^T (8 fragments), H, H^T, in as many terms as the results' type asks for
+        // A operands of the products with K and Q: G + G^T (8 fragments), H, H^T
         for (int f = w; f < 8 + 2 * kTriFrags; f += W) {
             f32x4 lo, hi;
             if (f < 8) {
@@ -774,10 +774,10 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
                     hi[e] = hmat[(32 * ks + 16 + 4 * q + e) * kTriStride + 16 * mt + j];
                 }
             }
-            bf16x8 t[PT];
-            split8<PT>(lo, hi, t);
+            bf16x8 t[3];
+            split8<3>(lo, hi, t);
 #pragma unroll
-            for (int k = 0; k < PT; ++k) fr[(f * PT + k) * 64 + lane] = t[k];
+            for (int k = 0; k < 3; ++k) fr[(f * 3 + k) * 64 + lane] = t[k];
         }
         // dg: sums of column `lane` over rows i >= m, for m in this wave's rows; what the rows below this wave's give follows
         float run[RB];
@@ -797,19 +797,19 @@ __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) 
         for (int m = 0; m < 4; ++m)
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                bf16x8 x[PT];
+                bf16x8 x[3];
 #pragma unroll
-                for (int t = 0; t < PT; ++t) x[t] = fr[((2 * m + ks) * PT + t) * 64 + lane];
-                k1[m] = mm<PT, NI, PT - 1>(x, kt[ks], k1[m]);
+                for (int t = 0; t < 3; ++t) x[t] = fr[((2 * m + ks) * 3 + t) * 64 + lane];
+                k1[m] = mm(x, kt[ks], k1[m]);
                 if (ks <= m / 2) {
 #pragma unroll
-                    for (int t = 0; t < PT; ++t) x[t] = fr[((8 + tri_index(m, ks)) * PT + t) * 64 + lane];
-                    q1[m] = mm<PT, NI, PT - 1>(x, kt[ks], q1[m]);
+                    for (int t = 0; t < 3; ++t) x[t] = fr[((8 + tri_index(m, ks)) * 3 + t) * 64 + lane];
+                    q1[m] = mm(x, kt[ks], q1[m]);
                 }
                 if (ks >= m / 2) {
 #pragma unroll
-                    for (int t = 0; t < PT; ++t) x[t] = fr[((8 + kTriFrags + trt_index(m, ks)) * PT + t) * 64 + lane];
-                    k1[m] = mm<PT, NI, PT - 1>(x, qt[ks], k1[m]);
+                    for (int t = 0; t < 3; ++t) x[t] = fr[((8 + kTriFrags + trt_index(m, ks)) * 3 + t) * 64 + lane];
+                    k1[m] = mm(x, qt[ks], k1[m]);
                 }
             }
         // dg_m of this wave's rows: the rectangle, what leaves before m and arrives from m on, what the state carries over

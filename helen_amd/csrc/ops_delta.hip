@@ -23,7 +23,6 @@ size_t carve(const HelenDeltaRule& op, int keep, void* base, DeltaArgs* a) {
     Carver c{(char*)base};
     const size_t ks = (size_t)a->slots * a->hk, vs = (size_t)a->slots * a->hv;
     const int ni = op.dtype == HELEN_TYPE_BF16 ? 1 : (op.dtype == HELEN_TYPE_FP16 ? 2 : 3);
-    const int pt = op.dtype == HELEN_TYPE_FP32 ? 3 : 2;
     const size_t rows = ks * (op.width_k / 8) * ni * 64, tri = vs * kTriFrags * 64;
     a->sink = c.take<float>(256);
     a->zeros = c.take<bf16x8>(3 * 64);
@@ -32,7 +31,7 @@ size_t carve(const HelenDeltaRule& op, int keep, void* base, DeltaArgs* a) {
     a->ktf = c.take<bf16x8>(rows);
     a->qf = from_inputs ? nullptr : c.take<bf16x8>(rows);
     a->tf = c.take<bf16x8>(tri * 3);
-    a->pf = c.take<bf16x8>(tri * pt);
+    a->pf = c.take<bf16x8>(tri * 3);
     a->sc = c.take<float>(vs * 256);
     if (keep) {
         a->qtf = c.take<bf16x8>(rows);
@@ -108,15 +107,15 @@ int describe(const HelenDeltaRule* op, Check level, DeltaArgs* a) {
     return HELEN_OK;
 }
 
-template <typename In, int DK, int PT, bool KEEP>
+template <typename In, int DK, bool KEEP>
 void launch_forward(const DeltaArgs& a, hipStream_t s) {
-    if (a.tokens > 0) hipLaunchKernelGGL((delta_prep_kernel<In, DK, PT, KEEP>), dim3((unsigned)a.slots * a.hk), dim3(256), 0, s, a);
-    if (chains_are_few(a)) hipLaunchKernelGGL((delta_forward_long_kernel<In, DK, PT, KEEP>), dim3(chain_grid(a, 16)), dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((delta_forward_kernel<In, DK, PT, KEEP>), dim3(chain_grid(a, 16 * kColumnTiles)), dim3(256), 0, s, a);
+    if (a.tokens > 0) hipLaunchKernelGGL((delta_prep_kernel<In, DK, KEEP>), dim3((unsigned)a.slots * a.hk), dim3(256), 0, s, a);
+    if (chains_are_few(a)) hipLaunchKernelGGL((delta_forward_long_kernel<In, DK, KEEP>), dim3(chain_grid(a, 16)), dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((delta_forward_kernel<In, DK, KEEP>), dim3(chain_grid(a, 16 * kColumnTiles)), dim3(256), 0, s, a);
 }
-template <typename In, int DK, int PT>
+template <typename In, int DK>
 void launch_forward(const DeltaArgs& a, int keep, hipStream_t s) {
-    keep ? launch_forward<In, DK, PT, true>(a, s) : launch_forward<In, DK, PT, false>(a, s);
+    keep ? launch_forward<In, DK, true>(a, s) : launch_forward<In, DK, false>(a, s);
 }
 
 }  // namespace
@@ -151,13 +150,13 @@ int helen_delta_rule_forward(const HelenDeltaRule* op, int keep, void* workspace
     hipStream_t s = (hipStream_t)stream;
     switch (op->dtype) {
         case HELEN_TYPE_BF16:
-            if (op->width_k == 64) launch_forward<InBf16, 64, 2>(a, keep, s); else launch_forward<InBf16, 128, 2>(a, keep, s);
+            if (op->width_k == 64) launch_forward<InBf16, 64>(a, keep, s); else launch_forward<InBf16, 128>(a, keep, s);
             break;
         case HELEN_TYPE_FP16:
-            if (op->width_k == 64) launch_forward<InF16, 64, 2>(a, keep, s); else launch_forward<InF16, 128, 2>(a, keep, s);
+            if (op->width_k == 64) launch_forward<InF16, 64>(a, keep, s); else launch_forward<InF16, 128>(a, keep, s);
             break;
         default:
-            if (op->width_k == 64) launch_forward<InF32, 64, 3>(a, keep, s); else launch_forward<InF32, 128, 3>(a, keep, s);
+            if (op->width_k == 64) launch_forward<InF32, 64>(a, keep, s); else launch_forward<InF32, 128>(a, keep, s);
     }
     return launched("delta rule forward");
 }

@@ -12,8 +12,8 @@ void launch(const DeltaArgs& a, hipStream_t s) {
     else hipLaunchKernelGGL((delta_backward_kernel<In, DK>), dim3(chain_grid(a, 16 * kColumnTiles)), dim3(256), 0, s, a);
     if (a.tokens == 0) return;
     const dim3 chunks((unsigned)a.slots * a.hk), block(DK * 4);
-    if (a.group == 1) hipLaunchKernelGGL((delta_grads_kernel<In, DK, In::kTerms == 3 ? 3 : 2, false>), chunks, block, 0, s, a);
-    else hipLaunchKernelGGL((delta_grads_kernel<In, DK, In::kTerms == 3 ? 3 : 2, true>), chunks, block, 0, s, a);
+    if (a.group == 1) hipLaunchKernelGGL((delta_grads_kernel<In, DK, false>), chunks, block, 0, s, a);
+    else hipLaunchKernelGGL((delta_grads_kernel<In, DK, true>), chunks, block, 0, s, a);
 }
 
 }  // namespace

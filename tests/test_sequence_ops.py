@@ -828,3 +828,27 @@ def test_autograd_forms_refuse_capture():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, x["v"] * 2)
+
+
+# ------------------------------------------------------------------------------------------------- one arithmetic for all types
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hk, hv, dk, dv, lengths", [
+    (1, 2, 128, 128, [1, 200, 65]), (2, 4, 64, 64, [130, 33]), (1, 1, 128, 256, [300]),          # few chains
+    (4, 8, 128, 128, [70, 64, 1, 131, 33]), (16, 16, 64, 64, [70, 64, 1, 131, 33]),               # more than compute units
+])
+def test_delta_rule_of_16_bits_is_the_fp32_one_rounded_once(dtype, hk, hv, dk, dv, lengths):
+    """Every product takes the same terms whatever the type of q, k, v and d_o (those that a 16-bit value lacks are zeros), so
+    the same values in float32 give the same sums: o, dq, dk and dv are those of float32 rounded once, the rest is equal.  (What
+    `close` leaves a 16-bit o beside its rounding, two terms an operand, is therefore not used.)"""
+    x = gpu(make(lengths, hk, hv, dk, dv, TYPES[dtype], True, seed=dk + dv))
+    off = torch.tensor(ends(lengths), dtype=torch.int32).cuda()
+
+    def run(widen):
+        q, k, v, do = (x[n].float() if widen else x[n] for n in ("q", "k", "v", "do"))
+        args, kw = (q, k, v, x["g"], x["beta"]), dict(initial_state=x["initial"], offsets=off)
+        o, s, saved = ops.delta_rule(*args, keep=True, **kw)
+        return (o, s) + ops.delta_rule(*args, **kw) + ops.delta_rule_backward(do, *args, d_final_state=x["ds"], saved=saved, **kw)
+    names = ("o", "final_state", "o", "final_state", "dq", "dk", "dv", "dg", "dbeta", "d_initial")
+    for name, a, b in zip(names, run(False), run(True)):
+        assert torch.equal(a, b.to(a.dtype)), (name, float((a.double() - b.double()).norm() / b.double().norm()))
