@@ -8,7 +8,8 @@ are calls of their own; `DeltaRule` and `LayerNorm` tie them into torch's autogr
 A call keeps nothing: workspaces come from torch's allocator, so calls on several streams may run at once and a call may be
 captured into a graph.  Nothing here waits for the device.
 
-Outputs may not overlap inputs or themselves; the exception is layer_norm's `out`, which may be `x`.
+Outputs may not overlap inputs or themselves; the exception is layer_norm's `out`, which may be `x`.  What a call writes in place
+(`out`, a pool of states) counts as modified for autograd, and may not require a gradient itself while gradients are recorded.
 """
 import ctypes
 import functools
@@ -71,6 +72,16 @@ def _inner(t, bytes_=0):
 def _like(t):
     """A new contiguous tensor of t's shape and type (empty_like is the cheapest allocation a call can make)."""
     return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+_wrote = torch.autograd.graph.increment_version      # (writes through a pointer are not seen by autograd otherwise)
+
+
+def _in_place(name, t):
+    """`t` will be written: refused where autograd would take it for the result of what made it."""
+    if torch.is_grad_enabled() and getattr(t, "requires_grad", False):
+        raise RuntimeError("%s requires a gradient and is written in place: call under torch.no_grad(), or pass a tensor that "
+                           "does not" % name)
 
 
 def _ptr(t):
@@ -234,6 +245,7 @@ def delta_rule(q, k, v, g, beta, scale=None, initial_state=None, offsets=None, o
     over 64 tokens is a float32.  Tokens are worked on in chunks of 64 (from the sequence's start): a NaN or an infinity in a
     token's q, k, v, g or beta reaches the results of its whole chunk, earlier tokens included, and what follows it, in its own
     sequence and heads; other sequences and heads stay as they are."""
+    _in_place("out", out)
     call = _Call(q, k, v, g, beta, scale, initial_state, offsets)
     shape = (call.tokens, call.hv, call.dv)
     if out is None:
@@ -241,6 +253,8 @@ def delta_rule(q, k, v, g, beta, scale=None, initial_state=None, offsets=None, o
     else:
         o, tail = _output("out", out, shape, call.dtype, call.device), 0
     final, work = call.forward(o, keep, tail)
+    if out is not None:
+        _wrote(out)
     return (o, final, work) if keep else (o, final)
 
 
@@ -279,6 +293,8 @@ def delta_rule_step(q, k, v, g, beta, state, slots=None, scale=None, out=None):
               zero.  Rows that name the same entry are successive tokens of one stream, taken in the order of the rows.  Any
               other number outside the pool makes that row's output NaN and changes no state
     -> o [rows, heads_v, width_v]."""
+    _in_place("state", state)
+    _in_place("out", out)
     device, code, n, hk, hv, dk, dv = _heads(q, k, v, g, beta)
     _same_gpu("state", state, device)
     s_shape = state.shape
@@ -314,6 +330,9 @@ def delta_rule_step(q, k, v, g, beta, state, slots=None, scale=None, out=None):
     rc = _lib.load().helen_delta_rule_step(op, _stream(device))
     if rc:
         _lib.check(rc)
+    _wrote(state)
+    if out is not None:
+        _wrote(out)
     return o
 
 
@@ -355,6 +374,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
     """Layer norm over the last dimension: y = (x - mean) rstd weight + bias with rstd = 1 / sqrt(var + eps).
     x [..., width] float32, bfloat16 or float16, weight / bias [width] of x's type or float32.  Rows of any stride and alignment; `out` may be x itself.
     -> (y, mean, rstd), mean and rstd float32 [...] for layer_norm_backward."""
+    _in_place("out", out)
     device, code, kind, width = _norm_sizes(x, weight, bias)
     rows = _rows(x)
     shape = x.shape
@@ -374,6 +394,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
     rc = _lib.load().helen_layer_norm_forward(op, _stream(device))
     if rc:
         _lib.check(rc)
+    if out is not None:
+        _wrote(out)
     return y, mean, rstd
 
 

@@ -852,3 +852,55 @@ def test_delta_rule_of_16_bits_is_the_fp32_one_rounded_once(dtype, hk, hv, dk, d
     names = ("o", "final_state", "o", "final_state", "dq", "dk", "dv", "dg", "dbeta", "d_initial")
     for name, a, b in zip(names, run(False), run(True)):
         assert torch.equal(a, b.to(a.dtype)), (name, float((a.double() - b.double()).norm() / b.double().norm()))
+
+
+# ------------------------------------------------------------------------------------------- written in place, and autograd
+def test_what_is_written_in_place_may_not_require_a_gradient():
+    x = make([4], 1, 1, 64, 64, torch.float32, False)
+    args = (x["q"], x["k"], x["v"], x["g"], x["beta"])
+    leaf = torch.zeros(4, 1, 64, requires_grad=True)
+    state = torch.zeros(4, 1, 64, 64)
+    calls = [lambda: ops.delta_rule(*args, out=leaf), lambda: ops.delta_rule(*args, out=leaf * 2),
+             lambda: ops.delta_rule_step(*args, state, out=leaf), lambda: ops.layer_norm(x["v"], out=leaf),
+             lambda: ops.delta_rule_step(*args, state.clone().requires_grad_()), lambda: ops.layer_norm(leaf * 1, out=leaf[:])]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="written in place"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+
+
+@pytest.mark.gpu
+def test_autograd_sees_what_is_written_in_place():
+    x = gpu(make([10], 1, 2, 64, 64, torch.float32, False, seed=23))
+    args = (x["q"], x["k"], x["v"], x["g"], x["beta"])
+
+    def spoiled(t, write):
+        """A backward pass that needs t as it was has to fail after `write`, and says why."""
+        w = torch.ones(t.shape[-1], device="cuda", requires_grad=True)
+        z = (w * t).sum()
+        before = t._version
+        write()
+        assert t._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.backward()
+    out = torch.randn(10, 2, 64, device="cuda")
+    spoiled(out, lambda: ops.delta_rule(*args, out=out))
+    spoiled(out, lambda: ops.delta_rule_step(*args, torch.zeros(10, 2, 64, 64, device="cuda"), out=out))
+    spoiled(out, lambda: ops.layer_norm(x["v"], out=out))
+    spoiled(out, lambda: ops.layer_norm(out, out=out))
+    spoiled(out, lambda: ops.layer_norm(out[:, 0], out=out[:, 0]))
+    state = torch.zeros(10, 2, 64, 64, device="cuda")
+    spoiled(state, lambda: ops.delta_rule_step(*args, state))
+    rows, w = x["v"][:, 0].clone(), torch.ones(64, device="cuda", requires_grad=True)
+    y = ops.LayerNorm.apply(rows, w)
+    ops.layer_norm(rows, out=rows)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    # gradients that do not need what was overwritten are as they were
+    leaf = torch.randn(10, 2, 64, 64, device="cuda", requires_grad=True)
+    pool = leaf * 2
+    with torch.no_grad():
+        ops.delta_rule_step(*args, pool)
+    pool.sum().backward()
+    assert bool((leaf.grad == 2).all())
