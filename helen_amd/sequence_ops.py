@@ -3,7 +3,8 @@ pool of states) and layer norm (forward and backward).
 
 They stand beside HelenEngine.chunk_forward, the GRU layer with a carried hidden state: torch tensors in, torch tensors out,
 all compute in libhelen_hip.so (include/helen_hip.h), asynchronous on the current stream of the tensors' device.  Gradients
-are calls of their own; `DeltaRule` and `LayerNorm` tie them into torch's autograd.
+are calls of their own; `DeltaRule` and `LayerNorm` tie them into torch's autograd.  The plain calls record nothing: while
+gradients are recorded they refuse inputs that require one.
 
 A call keeps nothing: workspaces come from torch's allocator, so calls on several streams may run at once and a call may be
 captured into a graph.  Nothing here waits for the device.
@@ -82,6 +83,14 @@ def _in_place(name, t):
     if torch.is_grad_enabled() and getattr(t, "requires_grad", False):
         raise RuntimeError("%s requires a gradient and is written in place: call under torch.no_grad(), or pass a tensor that "
                            "does not" % name)
+
+
+def _plain(what, use, *inputs):
+    """A call that autograd cannot follow: refused where it would cut a graph without a word."""
+    if torch.is_grad_enabled():
+        for t in inputs:
+            if getattr(t, "requires_grad", False):
+                raise RuntimeError("%s records no gradients and an input requires one: %s under torch.no_grad()" % (what, use))
 
 
 def _ptr(t):
@@ -246,6 +255,7 @@ def delta_rule(q, k, v, g, beta, scale=None, initial_state=None, offsets=None, o
     token's q, k, v, g or beta reaches the results of its whole chunk, earlier tokens included, and what follows it, in its own
     sequence and heads; other sequences and heads stay as they are."""
     _in_place("out", out)
+    _plain("delta_rule", "use DeltaRule.apply, or call it", q, k, v, g, beta, initial_state)
     call = _Call(q, k, v, g, beta, scale, initial_state, offsets)
     shape = (call.tokens, call.hv, call.dv)
     if out is None:
@@ -295,6 +305,7 @@ def delta_rule_step(q, k, v, g, beta, state, slots=None, scale=None, out=None):
     -> o [rows, heads_v, width_v]."""
     _in_place("state", state)
     _in_place("out", out)
+    _plain("delta_rule_step", "call it", q, k, v, g, beta)
     device, code, n, hk, hv, dk, dv = _heads(q, k, v, g, beta)
     _same_gpu("state", state, device)
     s_shape = state.shape
@@ -375,6 +386,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
     x [..., width] float32, bfloat16 or float16, weight / bias [width] of x's type or float32.  Rows of any stride and alignment; `out` may be x itself.
     -> (y, mean, rstd), mean and rstd float32 [...] for layer_norm_backward."""
     _in_place("out", out)
+    _plain("layer_norm", "use LayerNorm.apply, or call it", x, weight, bias)
     device, code, kind, width = _norm_sizes(x, weight, bias)
     rows = _rows(x)
     shape = x.shape

@@ -904,3 +904,26 @@ def test_autograd_sees_what_is_written_in_place():
         ops.delta_rule_step(*args, pool)
     pool.sum().backward()
     assert bool((leaf.grad == 2).all())
+
+
+def test_plain_calls_refuse_inputs_that_require_a_gradient():
+    """They cannot be followed by autograd: without a refusal the gradient of such an input would silently be missing."""
+    x = make([4], 1, 1, 64, 64, torch.float32, True)
+    names = ("q", "k", "v", "g", "beta")
+    plain = [x[n] for n in names]
+    calls = []
+    for i in range(5):
+        args = [t.clone().requires_grad_() if j == i else t for j, t in enumerate(plain)]
+        calls += [("DeltaRule.apply", lambda a=args: ops.delta_rule(*a)), ("delta_rule_step", lambda a=args: ops.delta_rule_step(*a, torch.zeros(4, 1, 64, 64)))]
+    calls += [("DeltaRule.apply", lambda: ops.delta_rule(*plain, initial_state=x["initial"].clone().requires_grad_())),
+              ("DeltaRule.apply", lambda: ops.delta_rule(plain[0].clone().requires_grad_() * 2, *plain[1:], keep=True))]
+    w = torch.ones(64, requires_grad=True)
+    calls += [("LayerNorm.apply", lambda: ops.layer_norm(x["v"].clone().requires_grad_())), ("LayerNorm.apply", lambda: ops.layer_norm(x["v"], w)),
+              ("LayerNorm.apply", lambda: ops.layer_norm(x["v"], None, w))]
+    for match, call in calls:
+        with pytest.raises(RuntimeError, match=match):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+        with torch.inference_mode(), pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
