@@ -453,6 +453,11 @@ def layer_norm_backward(dy, x, weight, mean, rstd, bias=True):
     return dx, dweight, dbias
 
 
+def _recorded(*inputs):
+    """Whether autograd records a call on these inputs."""
+    return torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in inputs)
+
+
 def _no_capture(what):
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("%s under autograd cannot be captured into a graph: torch would add into gradients of leaves that "
@@ -461,19 +466,24 @@ def _no_capture(what):
 
 class DeltaRule(torch.autograd.Function):
     """delta_rule under autograd: DeltaRule.apply(q, k, v, g, beta, scale, initial_state, offsets) -> (o, final_state).
-    Keeps the forward call's states for the backward pass.  Neither pass may be captured: the explicit calls may."""
+    Keeps the forward call's states for the backward pass where gradients are recorded; neither pass may be captured then (the
+    explicit calls may).  Otherwise it is the plain call."""
+
+    @classmethod
+    def apply(cls, q, k, v, g, beta, scale=None, initial_state=None, offsets=None):
+        if _recorded(q, k, v, g, beta, initial_state):
+            return super().apply(q, k, v, g, beta, scale, initial_state, offsets)
+        return delta_rule(q, k, v, g, beta, scale, initial_state, offsets)
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, scale=None, initial_state=None, offsets=None):
         _no_capture("DeltaRule")
-        keep = any(ctx.needs_input_grad)
-        got = delta_rule(q, k, v, g, beta, scale, initial_state, offsets, keep=keep)
-        if keep:
-            if isinstance(offsets, (list, tuple)):
-                offsets = torch.tensor(offsets, dtype=torch.int64)
-            ctx.scale = scale
-            ctx.save_for_backward(q, k, v, g, beta, initial_state, offsets, got[2])
-        return got[0], got[1]
+        o, final, saved = delta_rule(q, k, v, g, beta, scale, initial_state, offsets, keep=True)
+        if isinstance(offsets, (list, tuple)):
+            offsets = torch.tensor(offsets, dtype=torch.int64)
+        ctx.scale = scale
+        ctx.save_for_backward(q, k, v, g, beta, initial_state, offsets, saved)
+        return o, final
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -485,8 +495,14 @@ class DeltaRule(torch.autograd.Function):
 
 
 class LayerNorm(torch.autograd.Function):
-    """layer_norm under autograd: LayerNorm.apply(x, weight, bias, eps) -> y.  Neither pass may be captured: the explicit calls
-    may."""
+    """layer_norm under autograd: LayerNorm.apply(x, weight, bias, eps) -> y.  Where gradients are recorded neither pass may be
+    captured (the explicit calls may); otherwise it is the plain call."""
+
+    @classmethod
+    def apply(cls, x, weight=None, bias=None, eps=1e-5):
+        if _recorded(x, weight, bias):
+            return super().apply(x, weight, bias, eps)
+        return layer_norm(x, weight, bias, eps)[0]
 
     @staticmethod
     def forward(ctx, x, weight=None, bias=None, eps=1e-5):

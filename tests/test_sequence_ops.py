@@ -927,3 +927,46 @@ def test_plain_calls_refuse_inputs_that_require_a_gradient():
             call()
         with torch.inference_mode(), pytest.raises(RuntimeError, match="no CPU fallback"):
             call()
+
+
+@pytest.mark.gpu
+def test_autograd_forms_are_captured_where_nothing_is_recorded():
+    """Under no_grad, and without an input that requires a gradient: nothing to record, so the plain calls."""
+    x = gpu(make([70, 10], 1, 2, 64, 64, torch.bfloat16, True, seed=29))
+    off = torch.tensor([0, 70, 80], dtype=torch.int32, device="cuda")
+    w = torch.randn(64, generator=torch.Generator().manual_seed(1)).cuda().requires_grad_()
+    leaves = [x[n].clone().requires_grad_() for n in ("q", "k", "v", "g", "beta")]
+    plain = [x[n] for n in ("q", "k", "v", "g", "beta")]
+    with torch.no_grad():
+        want = ops.delta_rule(*plain, initial_state=x["initial"], offsets=off)
+        want += ops.layer_norm(want[0], w)[:1]
+
+    def under_no_grad():
+        with torch.no_grad():
+            o, s = ops.DeltaRule.apply(*leaves, None, x["initial"], off)
+            return o, s, ops.LayerNorm.apply(o, w)
+
+    def without_leaves():
+        o, s = ops.DeltaRule.apply(*plain, None, x["initial"], off)
+        return o, s, ops.LayerNorm.apply(o, w.detach())
+    for call in (under_no_grad, without_leaves):
+        got = call()
+        assert not any(t.requires_grad for t in got) and all(torch.equal(a, b) for a, b in zip(got, want))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = call()
+        for _ in range(3):
+            for t in got:
+                t.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            assert all(torch.equal(a, b) for a, b in zip(call(), want))
+    # with gradients recorded all five and the state's are there, and for one leaf alone its own
+    o, s = ops.DeltaRule.apply(*leaves, None, x["initial"], off)
+    o.backward(x["do"])
+    grads = ops.delta_rule_backward(x["do"], *plain, initial_state=x["initial"], offsets=off)
+    assert all(torch.equal(t.grad, b) for t, b in zip(leaves, grads))
+    beta = x["beta"].clone().requires_grad_()
+    ops.DeltaRule.apply(*plain[:4], beta, None, x["initial"], off)[0].backward(x["do"])
+    assert torch.equal(beta.grad, grads[4])
