@@ -384,6 +384,7 @@ def _norm_sizes(x, weight, bias):
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
     """Layer norm over the last dimension: y = (x - mean) rstd weight + bias with rstd = 1 / sqrt(var + eps).
     x [..., width] float32, bfloat16 or float16, weight / bias [width] of x's type or float32.  Rows of any stride and alignment; `out` may be x itself.
+    Rows longer than 16 KiB: less than 2^24 of them in one call.
     -> (y, mean, rstd), mean and rstd float32 [...] for layer_norm_backward."""
     _in_place("out", out)
     _plain("layer_norm", "use LayerNorm.apply, or call it", x, weight, bias)

@@ -358,6 +358,7 @@ int helen_delta_rule_step(const HelenDeltaStep* op, void* stream);
  *   x, y, dy, dx   [rows, width], rows `*_stride` elements apart, any alignment of their type; y may be x
  *   weight, bias   [width] of weight_dtype (dtype's own or float32), either may be NULL (one, zero)
  *   mean, rstd     float32 [rows]: written by the forward call (or NULL), read by the backward call
+ *   rows           less than 2^36, and less than 2^24 where a row is longer than 16 KiB; width at most 2^28
  * Backward: dx, and dweight / dbias of weight_dtype, either NULL if not wanted: sums over all rows in a fixed order
  * (workspace of helen_layer_norm_bytes).
  */

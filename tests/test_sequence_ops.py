@@ -970,3 +970,42 @@ def test_autograd_forms_are_captured_where_nothing_is_recorded():
     beta = x["beta"].clone().requires_grad_()
     ops.DeltaRule.apply(*plain[:4], beta, None, x["initial"], off)[0].backward(x["do"])
     assert torch.equal(beta.grad, grads[4])
+
+
+# ---------------------------------------------------------------------------------------------------- how much one call takes
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("dtype, width, rows, text", [
+    (1, 64, 2 ** 24, b"null"), (0, 4096, 2 ** 24, b"null"), (1, 8192, 2 ** 24, b"null"), (1, 128, 2 ** 36 - 1, b"null"),
+    (1, 128, 2 ** 36, b"more than one call"), (0, 4097, 2 ** 24 - 1, b"null"), (0, 4097, 2 ** 24, b"more than one call"),
+    (2, 8193, 2 ** 24, b"more than one call"),
+])
+def test_layer_norm_takes_rows_up_to_its_kernels_limits(backward, dtype, width, rows, text):
+    lib = _lib.load()
+    c = _lib.HelenLayerNormC()
+    c.struct_size = ctypes.sizeof(c)
+    c.dtype, c.weight_dtype, c.width, c.rows, c.eps = dtype, dtype, width, rows, 1e-5
+    rc = lib.helen_layer_norm_backward(ctypes.byref(c), None, 0, None) if backward else lib.helen_layer_norm_forward(ctypes.byref(c), None)
+    assert rc == -1 and text in lib.helen_last_error(), lib.helen_last_error()
+
+
+@pytest.mark.gpu
+def test_layer_norm_of_more_than_2_24_rows():
+    """Rows do not depend on each other: those of one call are those of two, and the sums over all rows those of 64 bits."""
+    rows, width, cut = 2 ** 24 + 5, 16, 2 ** 23 + 1
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x, dy = (torch.randn(rows, width, generator=gen, device="cuda").bfloat16() for _ in range(2))
+    w, b = (torch.randn(width, generator=gen, device="cuda") for _ in range(2))
+    y, mean, rstd = ops.layer_norm(x, w, b)
+    dx, dw, db = ops.layer_norm_backward(dy, x, w, mean, rstd)
+    for part in (slice(0, cut), slice(cut, rows)):
+        got = ops.layer_norm(x[part], w, b)
+        assert all(torch.equal(p, q[part]) for p, q in zip(got, (y, mean, rstd)))
+        assert torch.equal(ops.layer_norm_backward(dy[part], x[part], w, *got[1:])[0], dx[part])
+    sums = torch.zeros(4, width, dtype=torch.float64, device="cuda")
+    for at in range(0, rows, 2 ** 21):
+        g, h = dy[at:at + 2 ** 21].double(), (x[at:at + 2 ** 21].double() - mean[at:at + 2 ** 21, None]) * rstd[at:at + 2 ** 21, None]
+        sums += torch.stack([(g * h).sum(0), (g * h).abs().sum(0), g.sum(0), g.abs().sum(0)])
+    # a column's sum passes a lane (rows over 512 x 16 of them), 16 lanes, 512 workgroups one after another; h itself is off by 3 u
+    n = rows / (512 * 16) + 16 + 512 + 3
+    for got, want, size in ((dw, sums[0], sums[1]), (db, sums[2], sums[3])):
+        assert bool(((got.double() - want).abs() <= n * U * size + U * want.abs()).all())
