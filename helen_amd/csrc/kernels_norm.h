@@ -370,31 +370,35 @@ __global__ __launch_bounds__(256) void norm_backward_strip_kernel(const NormArgs
         }
 }
 
-// the workgroups' sums, added in a fixed order: 32 columns and 32 runs of groups a workgroup
+// the workgroups' sums, added in a fixed order: 32 columns and 32 runs of groups a workgroup, which goes on with the columns
+// gridDim.x strips further where the grid is smaller than the row
 template <typename W>
 __global__ __launch_bounds__(1024) void norm_reduce_kernel(const NormArgs a) {
     __shared__ float part[32][33];
     const int c = threadIdx.x & 31, run = threadIdx.x >> 5;
-    const long at = blockIdx.x * 32l + c;
-    float x = 0.f;
-    if (at < 2l * a.width) {
-        const float* p = a.partial + at;
-        for (int g = run; g < a.groups; g += 32 * 16) {
-            float y[16];
+    for (long first = blockIdx.x * 32l; first < 2l * a.width; first += gridDim.x * 32l) {
+        const long at = first + c;
+        float x = 0.f;
+        if (at < 2l * a.width) {
+            const float* p = a.partial + at;
+            for (int g = run; g < a.groups; g += 32 * 16) {
+                float y[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) y[i] = g + 32 * i < a.groups ? p[(long)(g + 32 * i) * 2 * a.width] : 0.f;
+                for (int i = 0; i < 16; ++i) y[i] = g + 32 * i < a.groups ? p[(long)(g + 32 * i) * 2 * a.width] : 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x += y[i];
+                for (int i = 0; i < 16; ++i) x += y[i];
+            }
         }
-    }
-    part[run][c] = x;
-    lds_barrier();
-    if (run == 0 && at < 2l * a.width) {
-        float sum = 0.f;
+        part[run][c] = x;
+        lds_barrier();
+        if (run == 0 && at < 2l * a.width) {
+            float sum = 0.f;
 #pragma unroll
-        for (int r = 0; r < 32; ++r) sum += part[r][c];
-        void* to = at < a.width ? a.dw : a.db;
-        if (to) ((typename W::raw*)to)[at < a.width ? at : at - a.width] = W::from_f32(sum);
+            for (int r = 0; r < 32; ++r) sum += part[r][c];
+            void* to = at < a.width ? a.dw : a.db;
+            if (to) ((typename W::raw*)to)[at < a.width ? at : at - a.width] = W::from_f32(sum);
+        }
+        lds_barrier();
     }
 }
 

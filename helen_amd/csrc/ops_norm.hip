@@ -119,7 +119,8 @@ void launch_norm(const HelenLayerNorm& op, const NormArgs& a, bool backward, hip
 }
 template <typename W>
 void launch_reduce(const NormArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL(norm_reduce_kernel<W>, dim3((2u * a.width + 31) / 32), dim3(1024), 0, s, a);
+    const unsigned strips = (2u * a.width + 31) / 32, most = 1u << 20;       // (threads of a launch are counted in 32 bits)
+    hipLaunchKernelGGL(norm_reduce_kernel<W>, dim3(strips < most ? strips : most), dim3(1024), 0, s, a);
 }
 
 }  // namespace

@@ -1009,3 +1009,20 @@ def test_layer_norm_of_more_than_2_24_rows():
     n = rows / (512 * 16) + 16 + 512 + 3
     for got, want, size in ((dw, sums[0], sums[1]), (db, sums[2], sums[3])):
         assert bool(((got.double() - want).abs() <= n * U * size + U * want.abs()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, width", [("bf16", 2 ** 24 + 3), ("bf16", 2 ** 26 + 37)])
+def test_layer_norm_gradient_of_very_wide_rows(dtype, width):
+    """The sums over the rows of more columns than one launch has threads for (64 threads a column and gradient); one row, so
+    they are dy h and dy themselves."""
+    gen = torch.Generator(device="cuda").manual_seed(width)
+    x, dy = (torch.randn(1, width, generator=gen, device="cuda").to(TYPES[dtype]) for _ in range(2))
+    w = torch.ones(width, device="cuda", dtype=TYPES[dtype])
+    mean, rstd = torch.tensor([0.25], device="cuda"), torch.tensor([0.5], device="cuda")
+    dx, dw, db = ops.layer_norm_backward(dy, x, w, mean, rstd)
+    assert torch.equal(db, dy[0])
+    # x - 1/4 and its half are rounded to 24 bits at most once, the product too, and dw to its own type
+    want = dy[0].double() * (x[0].double() - 0.25) * 0.5
+    assert bool(((dw.double() - want).abs() <= (half(dw.dtype) + 3 * U) * want.abs() + 1e-38).all())
+    assert bool(dx.isfinite().all())
