@@ -42,7 +42,10 @@ inline bool aligned(const void* p, const int64_t* stride, int size, int bytes) {
     return (uintptr_t)p % bytes == 0 && stride[0] * size % bytes == 0 && stride[1] * size % bytes == 0;
 }
 
-// a 1-D grid of workgroups of 256: the runtime counts threads in 32 bits
-inline bool grid_fits(int64_t groups) { return groups >= 0 && groups < (int64_t(1) << 24); }
+// a 1-D grid of a x b workgroups of `threads`, and `more`: the runtime counts threads in 32 bits
+inline bool grid_fits(int64_t a, int64_t b, int threads, int more = 0) {
+    const int64_t most = ((int64_t(1) << 32) - 1) / threads - more;
+    return a >= 0 && b >= 0 && (b == 0 || a <= most / b);
+}
 
 }  // namespace helen

@@ -69,8 +69,9 @@ int describe(const HelenDeltaRule* op, Check level, DeltaArgs* a) {
     if (!op->offsets && op->tokens % op->sequences)
         return fail(HELEN_EINVAL, "delta rule: %d tokens are no %d sequences of one length", op->tokens, op->sequences);
     const int64_t slots = (int64_t)op->tokens / kDeltaChunk + op->sequences + 1;
-    const int64_t chains = (int64_t)op->sequences * op->heads_v * (op->width_v / 16);
-    if (slots > INT32_MAX || !grid_fits(slots * op->heads_k) || !grid_fits(chains + 8))
+    // launches: preparation and gradients by (slot, key head), chains by column groups of a state (256 threads where they are many)
+    if (slots > INT32_MAX || !grid_fits(slots, op->heads_k, backward ? 4 * op->width_k : 256) ||
+        !grid_fits(op->sequences, (int64_t)op->heads_v * (op->width_v / (16 * kColumnTiles)), 256, 7))
         return fail(HELEN_EINVAL, "delta rule: %d tokens x %d heads in %d sequences are more than one call takes", op->tokens,
                     op->heads_v, op->sequences);
     const int size = type_size(op->dtype);

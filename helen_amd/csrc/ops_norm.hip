@@ -66,7 +66,7 @@ int check(const HelenLayerNorm* op, bool backward) {
     if (!(op->eps >= 0.f)) return fail(HELEN_EINVAL, "layer norm: eps %g", (double)op->eps);
     // a workgroup a row only in the wide kernels; the others' bound is what mean and rstd could be stored for
     const bool wide = !norm_plan(op->width, op->dtype).lanes;
-    if (wide ? !grid_fits(op->rows) : op->rows >= int64_t(1) << 36)
+    if (wide ? !grid_fits(op->rows, 1, 256) : op->rows >= int64_t(1) << 36)
         return fail(HELEN_EINVAL, "layer norm: %lld rows of width %d are more than one call takes", (long long)op->rows, op->width);
     if (op->rows > 0) {
         if (!op->x || (!backward && !op->y)) return fail(HELEN_EINVAL, "layer norm: null input or output");
@@ -141,7 +141,7 @@ int helen_delta_rule_step(const HelenDeltaStep* op, void* stream) {
     if (op->rows < 0 || op->pool < 0 || (!op->slots && op->rows > op->pool))
         return fail(HELEN_EINVAL, "delta step: %d rows over a pool of %d states", op->rows, op->pool);
     if (op->rows == 0) return HELEN_OK;
-    if (!grid_fits((int64_t)op->rows * op->heads_v * (op->width_v / 64)))
+    if (!grid_fits(op->rows, (int64_t)op->heads_v * (op->width_v / 64), 256))
         return fail(HELEN_EINVAL, "delta step: %d rows x %d heads are more than one call takes", op->rows, op->heads_v);
     if (!op->q || !op->k || !op->v || !op->g || !op->beta || !op->o || (!op->state && op->pool > 0))
         return fail(HELEN_EINVAL, "delta step: null input or output");

@@ -1026,3 +1026,30 @@ def test_layer_norm_gradient_of_very_wide_rows(dtype, width):
     want = dy[0].double() * (x[0].double() - 0.25) * 0.5
     assert bool(((dw.double() - want).abs() <= (half(dw.dtype) + 3 * U) * want.abs() + 1e-38).all())
     assert bool(dx.isfinite().all())
+
+
+@pytest.mark.parametrize("change, backward, text", [
+    # 64 tokens a slot: 9,000,002 slots fit launches of 256 threads a slot and key head, but not the gradients' 512 (width_k 128)
+    (dict(tokens=576000000, heads_k=1, heads_v=1), False, b"null input"),
+    (dict(tokens=576000000, heads_k=1, heads_v=1), True, b"more than one call"),
+    (dict(tokens=576000000, heads_k=1, heads_v=1, width_k=64), True, b"null input"),
+    (dict(tokens=1152000000, heads_k=1, heads_v=1), False, b"more than one call"),
+    # 4 x 2^22 groups of 32 columns, less the room for rounding up, and one sequence more
+    (dict(tokens=0, sequences=2 ** 22 - 2, heads_k=1, heads_v=1, offsets=4096), False, b"workspace"),
+    (dict(tokens=0, sequences=2 ** 22, heads_k=1, heads_v=1, offsets=4096), False, b"more than one call"),
+    (dict(tokens=0, sequences=2 ** 31 - 2, heads_k=2 ** 30, heads_v=2 ** 30, offsets=4096), False, b"more than one call"),
+])
+def test_delta_rule_takes_what_its_launches_can_count(change, backward, text):
+    lib = _lib.load()
+    c = ctypes.byref(description(**change))
+    rc = lib.helen_delta_rule_backward(c, None, 0, None, 0, None) if backward else lib.helen_delta_rule_forward(c, 0, None, 0, None)
+    assert rc == -1 and text in lib.helen_last_error(), lib.helen_last_error()
+
+
+def test_delta_step_refuses_more_rows_than_its_launch_can_count():
+    lib = _lib.load()
+    c = _lib.HelenDeltaStepC()
+    c.struct_size = ctypes.sizeof(c)
+    c.heads_k, c.heads_v, c.width_k, c.width_v, c.rows, c.pool = 1, 2 ** 30, 128, 256, 2 ** 30, 2 ** 30
+    assert lib.helen_delta_rule_step(ctypes.byref(c), None) == -1
+    assert b"more than one call" in lib.helen_last_error(), lib.helen_last_error()
