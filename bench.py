@@ -668,6 +668,13 @@ def plan_only(args, rank, world):
     return out
 
 
+def no_end_to_end(world, **why):
+    """The `end_to_end` object of a leg that did not run to its end: no value, no windows, and why."""
+    out = {"value": None, "n_ranks": world, "windows": 0}
+    out.update(why)
+    return out
+
+
 def end_to_end(windows_per_rank, workers, batch, weights, rank, world, single_device, dist, may_shrink=False):
     """The product's commands over `world` ranks on a SIMULATED ASSEMBLY (helen_amd.synthetic.write_assembly_dir: contigs cut
     into 2400-position regions of three images, insert rows, short last images; pileups from the read-vote noise model;
@@ -712,8 +719,8 @@ def end_to_end(windows_per_rank, workers, batch, weights, rank, world, single_de
         dist.broadcast_object_list(box, src=0)
     d, windows_per_rank, need = box
     if d is None:
-        return {"value": None, "skipped": "/dev/shm may take %.1f GB, the %d-rank leg needs %.1f GB"
-                                          % (ram_backed_budget_bytes() / 1e9, world, need / 1e9)} if rank == 0 else None
+        return no_end_to_end(world, skipped="/dev/shm may take %.1f GB, the %d-rank leg needs %.1f GB"
+                                            % (ram_backed_budget_bytes() / 1e9, world, need / 1e9)) if rank == 0 else None
     together = os.path.join(d, "together")
     try:
         img_dir = os.path.join(d, "img")
@@ -732,7 +739,7 @@ def end_to_end(windows_per_rank, workers, batch, weights, rank, world, single_de
         if dist is not None:            # doubles as the barrier: every rank learns whether all inputs exist
             write_error = next((e for e in gather_strings(dist, world, write_error or "") if e), None)
         if write_error:
-            return {"value": None, "error": "writing the synthetic inputs failed: " + write_error} if rank == 0 else None
+            return no_end_to_end(world, error="writing the synthetic inputs failed: " + write_error) if rank == 0 else None
         others = gather_strings(dist, world, str(os.getpid()))[1:] if dist is not None else []
         if rank != 0:                   # (a rank that ends while another is still inside the exchange breaks its connection)
             while not os.path.exists(together):
@@ -1222,7 +1229,9 @@ def main():
             e2e = end_to_end(e2e_windows, args.e2e_workers, B, trained_weights(), rank, world,
                              args.single_device, dist, may_shrink=args.e2e is None)
         except (Exception, SystemExit) as e:    # noqa: BLE001 -- this leg must not take the headline down with it (call_consensus exits on bad input)
-            e2e = {"value": None, "error": "%s: %s" % (type(e).__name__, e)}
+            import traceback
+            sys.stderr.write("bench.py: rank %d: the end-to-end leg failed:\n%s" % (rank, traceback.format_exc()))
+            e2e = no_end_to_end(world, error="%s: %s" % (type(e).__name__, e))
     if rank == 0:
         if e2e is not None:
             out["end_to_end"] = e2e

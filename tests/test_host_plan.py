@@ -375,3 +375,28 @@ def test_bench_clock_report_reads_hwmon_and_never_raises(tmp_path, monkeypatch):
     calls = []
     out = bench.sustained_clock(lambda n: calls.append(n), "cuda:0", seconds=0.05)
     assert isinstance(out, dict) and ("error" in out or "sclk_mhz" in out)
+
+
+def _bench():
+    import importlib.util
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    spec = importlib.util.spec_from_file_location("bench_for_leg", os.path.join(root, "bench.py"))
+    bench = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(bench)
+    return bench
+
+
+def test_an_end_to_end_leg_that_did_not_run_says_for_how_many_ranks_and_why(monkeypatch):
+    """A line whose leg was skipped or failed has the keys that a whole one is looked at by, and the reason."""
+    bench = _bench()
+    monkeypatch.setattr(bench, "e2e_size", lambda *a, **k: (8192, 31 << 30, None, 1 << 30))
+    got = bench.end_to_end(8192, 8, 256, None, 0, 8, True, None)
+    assert got["n_ranks"] == 8 and got["windows"] == 0 and got["value"] is None and "needs 33.3 GB" in got["skipped"], got
+    assert bench.end_to_end(8192, 8, 256, None, 0, 1, True, None)["n_ranks"] == 1
+    monkeypatch.setattr(bench, "e2e_size", lambda n, world, may_shrink: (n, 1 << 20, "tmp", 1 << 30))
+
+    def broken(*a, **k):
+        raise OSError("no space")
+    monkeypatch.setattr("helen_amd.synthetic.write_assembly_dir", broken)
+    got = bench.end_to_end(64, 1, 16, None, 0, 1, True, None)
+    assert got["n_ranks"] == 1 and got["windows"] == 0 and "OSError: no space" in got["error"], got
