@@ -675,6 +675,12 @@ def no_end_to_end(world, **why):
     return out
 
 
+def wait_until_released(directory):
+    """A rank that is not the first one: until rank 0 says that all ranks have met (or has given up and removed the directory)."""
+    while os.path.isdir(directory) and not os.path.exists(os.path.join(directory, "together")):
+        time.sleep(0.05)
+
+
 def end_to_end(windows_per_rank, workers, batch, weights, rank, world, single_device, dist, may_shrink=False):
     """The product's commands over `world` ranks on a SIMULATED ASSEMBLY (helen_amd.synthetic.write_assembly_dir: contigs cut
     into 2400-position regions of three images, insert rows, short last images; pileups from the read-vote noise model;
@@ -742,8 +748,7 @@ def end_to_end(windows_per_rank, workers, batch, weights, rank, world, single_de
             return no_end_to_end(world, error="writing the synthetic inputs failed: " + write_error) if rank == 0 else None
         others = gather_strings(dist, world, str(os.getpid()))[1:] if dist is not None else []
         if rank != 0:                   # (a rank that ends while another is still inside the exchange breaks its connection)
-            while not os.path.exists(together):
-                time.sleep(0.05)
+            wait_until_released(d)
             return None
         open(together, "w").close()
         limit = time.time() + 20.0

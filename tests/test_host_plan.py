@@ -400,3 +400,21 @@ def test_an_end_to_end_leg_that_did_not_run_says_for_how_many_ranks_and_why(monk
     monkeypatch.setattr("helen_amd.synthetic.write_assembly_dir", broken)
     got = bench.end_to_end(64, 1, 16, None, 0, 1, True, None)
     assert got["n_ranks"] == 1 and got["windows"] == 0 and "OSError: no space" in got["error"], got
+
+
+def test_a_rank_that_waits_for_the_first_one_ends_when_it_has_given_up(tmp_path):
+    import shutil
+    import threading
+    bench = _bench()
+    for release in (lambda d: open(os.path.join(d, "together"), "w").close(), shutil.rmtree):
+        d = str(tmp_path / "leg")
+        os.makedirs(d, exist_ok=True)
+        waiting = threading.Thread(target=bench.wait_until_released, args=(d,), daemon=True)
+        waiting.start()
+        time.sleep(0.2)
+        assert waiting.is_alive()
+        release(d)
+        waiting.join(5)
+        assert not waiting.is_alive()
+        if os.path.isdir(d):
+            shutil.rmtree(d)
