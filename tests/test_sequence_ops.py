@@ -1053,3 +1053,106 @@ def test_delta_step_refuses_more_rows_than_its_launch_can_count():
     c.heads_k, c.heads_v, c.width_k, c.width_v, c.rows, c.pool = 1, 2 ** 30, 128, 256, 2 ** 30, 2 ** 30
     assert lib.helen_delta_rule_step(ctypes.byref(c), None) == -1
     assert b"more than one call" in lib.helen_last_error(), lib.helen_last_error()
+
+
+# ----------------------------------------------------------------------------------------- resets, long chains, equal lengths
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("lengths, heads, decay", [([130], 3, 1.0), ([200, 1, 64], 3, 25.0), ([70, 64, 1, 131, 33], 16, 1.0)])
+def test_delta_rule_gradients_at_resets_and_strong_decays(dtype, lengths, heads, decay):
+    """All gradients against the reference where the state is held (g = 0), all but forgotten (-80) and forgotten: e^-200 has a
+    derivative in 64 bits, and is as good as zero there.  -inf in its place gives the same bits.  (16 heads of 5 sequences: 320
+    chains, the kernel for many.)"""
+    x = make(lengths, 1 if heads == 3 else 16, heads, 64, 64, TYPES[dtype], True, seed=31, decay=decay)
+    x["g"][:, 0] = 0.0
+    x["g"][::17, 1] = -80.0
+    far = torch.zeros(x["g"].shape, dtype=torch.bool)
+    far[0, 2] = far[40, 2] = far[64, 2] = far[65, 2] = far[-1, 2] = True
+    x["g"][far] = -200.0
+    check_delta(x, lengths)
+    d = gpu(x)
+    off = torch.tensor(ends(lengths), dtype=torch.int32, device="cuda")
+
+    def run(g):
+        args, kw = (d["q"], d["k"], d["v"], g, d["beta"]), dict(initial_state=d["initial"], offsets=off)
+        o, s, saved = ops.delta_rule(*args, keep=True, **kw)
+        return (o, s) + ops.delta_rule_backward(d["do"], *args, d_final_state=d["ds"], saved=saved, **kw)
+    near = run(d["g"])
+    for a, b in zip(run(d["g"].masked_fill(far.cuda(), -math.inf)), near):
+        assert torch.equal(a, b)
+    assert not near[5][0, 2].any()            # a reset before the first token: the initial state has no part in anything
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("lengths", [[2600, 1111], [2600] + [3] * 50], ids=["few chains", "many chains"])
+def test_delta_rule_long_chains(dtype, lengths):
+    """41 chunks in a row, with the kernels for few chains (24 of 16 columns) and for many (612).  Head 0 never forgets (g = 0): an
+    error made in a chunk may stay, so the bounds count all chunks.  The slowest other head decays by e^-0.025|N| a token, e^-1.3 a
+    chunk on average: beside what a chunk adds, what is left of those before it makes up 1 / (e^1.3 - 1) = 0.4 of it, so two are
+    counted.  The float32 results (state, dg, dbeta, d_initial) are held to that without a rounding to hide in."""
+    hv, count = 3, 41
+    x = make(lengths, 1, hv, 64, 64, TYPES[dtype], True, seed=len(lengths))
+    n = x["g"].shape[0]
+    x["g"] = -torch.randn(n, hv, generator=torch.Generator().manual_seed(5)).abs() * torch.tensor([0.0, 0.025, 0.5])
+    d = gpu(x)
+    off = torch.tensor(ends(lengths), dtype=torch.int32, device="cuda")
+    args, kw = (d["q"], d["k"], d["v"], d["g"], d["beta"]), dict(scale=x["scale"], initial_state=d["initial"], offsets=off)
+    o, s, saved = ops.delta_rule(*args, keep=True, **kw)
+    got = (o, s) + ops.delta_rule_backward(d["do"], *args, d_final_state=d["ds"], saved=saved, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(ops.delta_rule(*args, **kw), got))
+    leaves = [x[m].double().requires_grad_() for m in ("q", "k", "v", "g", "beta")]
+    # dq and dk are summed over the heads: here they are wanted a head at a time, so every head gets keys of its own
+    leaves[0], leaves[1] = (t.detach().repeat_interleave(hv, 1).requires_grad_() for t in leaves[:2])
+    first = x["initial"].double().requires_grad_()
+    ro, rs = delta_reference(*leaves, x["scale"], first, lengths)
+    loss = (ro * x["do"].double()).sum() + (rs * x["ds"].double()).sum()
+    want = dict(zip(("o", "final_state", "dq", "dk", "dv", "dg", "dbeta", "d_initial"),
+                    (ro, rs) + torch.autograd.grad(loss, leaves + [first])))
+    products = 64 + 64 + 64
+    for name, a in zip(("o", "final_state", "dq", "dk", "dv", "dg", "dbeta", "d_initial"), got):
+        b = want[name]
+        if name in ("dq", "dk"):
+            close(name, a, b.sum(1, keepdim=True), products, count)
+            continue
+        for head, chunks in ((slice(0, 1), count), (slice(1, hv), 2)):
+            close("%s of heads %s" % (name, head), a[:, head], b[:, head], products, chunks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sequences, length, hk, hv", [(3, 70, 1, 2), (40, 33, 2, 4), (2, 64, 1, 1), (7, 1, 1, 2)])
+def test_delta_rule_sequences_of_one_length_without_offsets(sequences, length, hk, hv):
+    """The C entries with offsets NULL: the results of the same call with offsets, bit for bit."""
+    dk = dv = 64
+    lengths = [length] * sequences
+    x = gpu(make(lengths, hk, hv, dk, dv, torch.bfloat16, True, seed=sequences))
+    tokens = sequences * length
+    off = torch.tensor(ends(lengths), dtype=torch.int32, device="cuda")
+    args, kw = (x["q"], x["k"], x["v"], x["g"], x["beta"]), dict(scale=x["scale"], initial_state=x["initial"], offsets=off)
+    o, s, saved = ops.delta_rule(*args, keep=True, **kw)
+    want = (o, s) + ops.delta_rule_backward(x["do"], *args, d_final_state=x["ds"], saved=saved, **kw)
+    lib = _lib.load()
+    c = _lib.HelenDeltaRuleC()
+    c.struct_size, c.device, c.dtype = ctypes.sizeof(c), x["q"].get_device(), _lib.HELEN_TYPE_BF16
+    c.heads_k, c.heads_v, c.width_k, c.width_v, c.tokens, c.sequences, c.scale = hk, hv, dk, dv, tokens, sequences, x["scale"]
+    sizes = [ctypes.c_size_t() for _ in range(3)]
+    _lib.check(lib.helen_delta_rule_bytes(ctypes.byref(c), *(ctypes.byref(t) for t in sizes)))
+    plain, kept, own = (torch.empty(t.value, dtype=torch.uint8, device="cuda") for t in sizes)
+    got = [torch.full_like(t, 7.0) for t in want]
+    pair = lambda t: (ctypes.c_int64 * 2)(*t.stride()[:2])  # noqa: E731
+    for name, t in zip(("q", "k", "v", "g", "beta"), args):
+        setattr(c, name, t.data_ptr())
+        setattr(c, name + "_stride", pair(t))
+    c.initial_state, c.d_o, c.d_o_stride, c.d_final_state = x["initial"].data_ptr(), x["do"].data_ptr(), pair(x["do"]), x["ds"].data_ptr()
+    c.o, c.o_stride, c.final_state = got[0].data_ptr(), pair(got[0]), got[1].data_ptr()
+    for name, t in zip(("grad_q", "grad_k", "grad_v", "grad_g", "grad_beta", "grad_initial_state"), got[2:]):
+        setattr(c, name, t.data_ptr())
+    stream = torch.cuda.current_stream().cuda_stream
+    call = ctypes.byref(c)
+    _lib.check(lib.helen_delta_rule_forward(call, 0, plain.data_ptr(), plain.numel(), stream))
+    assert torch.equal(got[0], o) and torch.equal(got[1], s)
+    got[0].fill_(7.0)
+    _lib.check(lib.helen_delta_rule_forward(call, 1, kept.data_ptr(), kept.numel(), stream))
+    _lib.check(lib.helen_delta_rule_backward(call, kept.data_ptr(), kept.numel(), own.data_ptr(), own.numel(), stream))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
