@@ -78,19 +78,22 @@ def _like(t):
 _wrote = torch.autograd.graph.increment_version      # (writes through a pointer are not seen by autograd otherwise)
 
 
-def _in_place(name, t):
-    """`t` will be written: refused where autograd would take it for the result of what made it."""
-    if torch.is_grad_enabled() and getattr(t, "requires_grad", False):
-        raise RuntimeError("%s requires a gradient and is written in place: call under torch.no_grad(), or pass a tensor that "
-                           "does not" % name)
+_requires = torch._C._any_requires_grad if hasattr(torch._C, "_any_requires_grad") else (
+    lambda *inputs: any(getattr(t, "requires_grad", False) for t in inputs))
 
 
-def _plain(what, use, *inputs):
-    """A call that autograd cannot follow: refused where it would cut a graph without a word."""
-    if torch.is_grad_enabled():
-        for t in inputs:
-            if getattr(t, "requires_grad", False):
-                raise RuntimeError("%s records no gradients and an input requires one: %s under torch.no_grad()" % (what, use))
+def _recorded(*inputs):
+    """Whether autograd records a call on these inputs."""
+    return torch.is_grad_enabled() and _requires(*inputs)
+
+
+def _outside(what, use, *written):
+    """Refuses a call that autograd cannot follow: it would cut an input's graph without a word, or take what is written for the
+    result of what made it."""
+    if _requires(*written):
+        raise RuntimeError("what %s writes requires a gradient and is written in place: call it under torch.no_grad(), or pass a "
+                           "tensor that does not" % what)
+    raise RuntimeError("%s records no gradients and an input requires one: %s under torch.no_grad()" % (what, use))
 
 
 def _ptr(t):
@@ -254,8 +257,8 @@ def delta_rule(q, k, v, g, beta, scale=None, initial_state=None, offsets=None, o
     over 64 tokens is a float32.  Tokens are worked on in chunks of 64 (from the sequence's start): a NaN or an infinity in a
     token's q, k, v, g or beta reaches the results of its whole chunk, earlier tokens included, and what follows it, in its own
     sequence and heads; other sequences and heads stay as they are."""
-    _in_place("out", out)
-    _plain("delta_rule", "use DeltaRule.apply, or call it", q, k, v, g, beta, initial_state)
+    if _recorded(q, k, v, g, beta, initial_state, out):
+        _outside("delta_rule", "use DeltaRule.apply, or call it", out)
     call = _Call(q, k, v, g, beta, scale, initial_state, offsets)
     shape = (call.tokens, call.hv, call.dv)
     if out is None:
@@ -303,9 +306,8 @@ def delta_rule_step(q, k, v, g, beta, state, slots=None, scale=None, out=None):
               zero.  Rows that name the same entry are successive tokens of one stream, taken in the order of the rows.  Any
               other number outside the pool makes that row's output NaN and changes no state
     -> o [rows, heads_v, width_v]."""
-    _in_place("state", state)
-    _in_place("out", out)
-    _plain("delta_rule_step", "call it", q, k, v, g, beta)
+    if _recorded(q, k, v, g, beta, state, out):
+        _outside("delta_rule_step", "call it", state, out)
     device, code, n, hk, hv, dk, dv = _heads(q, k, v, g, beta)
     _same_gpu("state", state, device)
     s_shape = state.shape
@@ -386,8 +388,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
     x [..., width] float32, bfloat16 or float16, weight / bias [width] of x's type or float32.  Rows of any stride and alignment; `out` may be x itself.
     Rows longer than 16 KiB: less than 2^24 of them in one call.
     -> (y, mean, rstd), mean and rstd float32 [...] for layer_norm_backward."""
-    _in_place("out", out)
-    _plain("layer_norm", "use LayerNorm.apply, or call it", x, weight, bias)
+    if _recorded(x, weight, bias, out):
+        _outside("layer_norm", "use LayerNorm.apply, or call it", out)
     device, code, kind, width = _norm_sizes(x, weight, bias)
     rows = _rows(x)
     shape = x.shape
@@ -452,11 +454,6 @@ def layer_norm_backward(dy, x, weight, mean, rstd, bias=True):
     if rc:
         _lib.check(rc)
     return dx, dweight, dbias
-
-
-def _recorded(*inputs):
-    """Whether autograd records a call on these inputs."""
-    return torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in inputs)
 
 
 def _no_capture(what):
