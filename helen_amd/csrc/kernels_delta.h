@@ -23,6 +23,9 @@
 // U, R) becomes the next product's B operand without any exchange: two stacked D tiles lie in the accumulators as element
 // e = 0 .. 7 of lane quarter q.  Over tokens that is k = 32 s + (e < 4 ? 4 q + e : 16 + 4 q + e - 4); over dk the rows of S go to the
 // tiles in such an order (state_row) that it is k = 32 s + 8 q + e, eight neighbours of a row of K or Q.
+//
+// Times of kernels here and in kernels_delta_bwd.h are the fastest of six launches under a kernel trace (the first ones, on cold
+// caches and clocks, are up to a fifth longer); shares of the matrix pipe, waits and bytes come from its counters.
 #pragma once
 #include "kernels_common.h"
 
@@ -366,9 +369,9 @@ constexpr int kTriStride = 68;    // floats per row of a 64 x 64 matrix in LDS: 
 // What becomes a left-hand operand is computed transposed, (Q K^T)^T = K Q^T: a result tile then already lies as that operand
 // (lane = row, four neighbouring columns), so P goes from the accumulators to memory, and A to LDS and back in whole
 // fragments.  K^T comes from the matrix pipe too: K times a selection of 16 columns is K's tile with lane = dk.
-// What bounds it: bandwidth, mostly its own writing.  16,384 tokens, 16 key and 32 value heads of 128, bf16: 0.65 GB in 117 us,
-// 5.6 TB/s, what a large copy reaches; the four workgroups a CU (35 KB of LDS, 128 registers) took it there (from 140 us to 109, then with
-// P in two terms).
+// What bounds it: bandwidth, mostly its own writing.  16,384 tokens, 16 key and 32 value heads of 128, bf16: 0.10 GB read and 0.50
+// written in 117 us, 5.1 TB/s, what a large copy reaches; the four workgroups a CU (35 KB of LDS, 128 registers) took it there
+// (from 140 us to 109, then with P in two terms).
 // ------------------------------------------------------------------------------------------------
 template <typename In, int DK, bool BWD>
 __global__ __launch_bounds__(256, In::kTerms == 1 ? (BWD ? 3 : 4) : 1) void delta_prep_kernel(const DeltaArgs a) {
@@ -786,9 +789,9 @@ struct ChainAddress {
 };
 // Row tile w of K or Q straight from the inputs: in bf16 the rows are the fragments; dead rows stand for the last live one (what
 // comes of them meets zeros).  The preparation then writes 32 KB less a key head and chunk, and the loads are of 64 bytes a row.
-// 64 sequences of 1000 tokens, 4 heads of 128: preparation 88 -> 60 us, chain 169 -> 176.  Chains that also write their states lose more
-// than that (32 x 1000 tokens: 97 -> 84, 230 -> 247, reverse 235 -> 243), and so do the eight-wave ones (16,384 tokens: 116 -> 91,
-// 473 -> 555): they take the fragments.
+// 64 sequences of 1000 tokens, 4 heads of 128: preparation 88 -> 60 us, chain 169 -> 176 (here and below with P and U in two terms;
+// it is 66 and 188 with three).  Chains that also write their states lose more than that (32 x 1000 tokens: 97 -> 84, 230 ->
+// 247, reverse 235 -> 243), and so do the eight-wave ones (16,384 tokens: 116 -> 91, 473 -> 555): they take the fragments.
 template <typename In, int DK>
 struct InputRows {
     typedef typename In::raw raw;
@@ -861,11 +864,12 @@ __device__ __forceinline__ void load_state(const float* state, const void* zeros
 // operand (S, R, U) come through LDS as bf16 terms, three barriers a chunk; every left-hand fragment is read by
 // one wave only, straight into registers, and the next chunk's are loaded into the registers the present chunk is done with.
 // What bounds it: the way through a chunk.  Two workgroups fit a CU (registers), so a SIMD has two waves to hide behind each other
-// 120 products of 16 cycles, some 400 VALU instructions (the splits), 85 LDS accesses and 45 loads a wave and chunk.  64
-// sequences of 1000 tokens, 4 heads of 128, bf16: 188 us, 134 TFLOP/s of the recurrence's own 6 Dk Dv a token (176 us with P
-// and U in two terms, when bf16 results were 1.1e-4 of their norm from a float32 evaluation's, not 3.5e-5).  Two column tiles
-// share every left-hand fragment; with one it was 244 us instead of 169, and keeping the states 370 instead of 232 (32 x 1000, 8
-// heads; both with fragments of K and Q, and two terms).
+// 120 products of 16 cycles, some 400 VALU instructions (the splits), 85 LDS accesses and 45 loads a wave and chunk: the matrix
+// pipe is busy for 30 % of the time, and a wave waits for a quarter of it.  fp16 and fp32 at width 128 have one workgroup a CU
+// (280 and more registers).  64 sequences of 1000 tokens, 4 heads of 128, bf16: 188 us, 134 TFLOP/s of the recurrence's own 6 Dk Dv a
+// token (176 us with P and U in two terms, when bf16 results were 1.1e-4 of their norm from a float32 evaluation's, not 3.5e-5).
+// Two column tiles share every left-hand fragment; with one it was 244 us instead of 169, and keeping the states 370 instead of
+// 232 (32 x 1000, 8 heads; both with fragments of K and Q, and two terms).
 // ------------------------------------------------------------------------------------------------
 template <typename In, int DK, bool KEEP>
 __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_kernel(const DeltaArgs a) {
@@ -1062,15 +1066,16 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_forward_ke
 // every 5 to 9 cycles, and the chain is as long as what its waves have to issue; so waves 0 .. 3 do only what the next chunk
 // waits for (R, E and S), and waves 4 .. 7, one on each SIMD beside them, the output and every store: from S, E and U as they
 // pass by in LDS, a phase later.  Waves whose row tile of T and P has one k step run code of their own (without: 510 us, not 473).
-// What bounds it: a chunk is 4,000 to 4,400 cycles, in which the CU's loads come back in order, 83 KB of them, 64 bytes a cycle at
-// best.  16,384 tokens, 32 heads of 128, bf16: 498 us, 103 TFLOP/s (473 with P, U and S in two terms for the
-// output); the four-wave kernel on 256 chains takes 1.4 times as long.
+// What bounds it: a chunk is 4,100 cycles, of which the matrix pipe works for 870 and the waves wait for half.  The CU's loads, 89 KB
+// of fragments and rows a chunk, take 1,400 at the 64 bytes a cycle of its L1, and three barriers keep them and the products from
+// each other.  16,384 tokens, 32 heads of 128, bf16: 498 us, 103 TFLOP/s (473 with P, U and S in two terms for the output); the
+// four-wave kernel on 256 chains takes 1.4 times as long (one sequence of 2048 tokens, 32 heads: 118 us a call against 84).
+// fp32 at width 128 spills 8 registers, 10 where it keeps the states.
 // ------------------------------------------------------------------------------------------------
-// Fetches a chunk's fragments into the XCD's L2 before the workgroups of its head need them.  They all come by at the same time, and
-// loads that miss there run at half the rate of loads that hit (28 - 35 against 16 cycles a KiB and CU).  Each of the head's
-// waves takes another part: one load, a lane a line of 128 bytes.  The value is handed to `settle` a chunk later.  8191 tokens in two
-// sequences, 16 heads of 128: forward chain 215 us without, 194 with, reverse chain 226 and 182; 16,384 tokens x 32 heads: no
-// difference.
+// Fetches a chunk's fragments into the XCD's L2 before the workgroups of its head need them.  They all come by at the same time,
+// and what misses there comes at a lower rate.  Each of the head's waves takes another part: one load, a lane a line of 128 bytes.
+// The value is handed to `settle` a chunk later.  8191 tokens in two sequences, 16 heads of 128: forward chain 215 us without, 194
+// with, reverse chain 226 and 182; 16,384 tokens x 32 heads: no difference.
 struct Piece {
     const bf16x8* at;
     int kib;
@@ -1338,10 +1343,11 @@ __global__ __launch_bounds__(512) void delta_forward_long_kernel(const DeltaArgs
     else w < 2 ? output(Is<false>()) : output(Is<true>());
 }
 
-// Which of the two: the eight-wave kernel while each of its workgroups has a CU to itself.  One sequence of 2048 tokens, bf16, width
-// 128, forward / forward + keep / backward in us, four waves against eight: 256 chains 104, 120, 205 against 75, 95, 170; 288
-// chains 108, 140, 244 against 123, 168, 255; 512 chains 116, 192, 312 against 135, 228, 341 (fp16, fp32 and width 64 cross
-// over at the same place, ragged sequences too).
+// Which of the two: the eight-wave kernel while each of its workgroups has a CU to itself.  One sequence of 2048 tokens, bf16, widths
+// 128, forward / forward + keep / backward calls in us, four waves against eight: 256 chains 118, 147, 211 against 84, 119, 176;
+// 288 chains 124, 154, 236 against 120, 177, 242; 512 chains 134, 205, 324 against 164, 271, 348 (fp16, fp32 and width_k 64 cross
+// over at the same place, with the forward call of bf16 at 288 chains alone on the other side).  Chains are counted, not their
+// lengths: many short sequences beside a few long ones go to the kernel for many.
 constexpr int kComputeUnits = 256;
 inline bool chains_are_few(const DeltaArgs& a) { return (long)a.nseq * a.hv * (a.dv_width / 16) <= kComputeUnits; }
 inline unsigned chain_grid(const DeltaArgs& a, int columns) {      // columns of the state a workgroup takes

@@ -15,7 +15,7 @@
 namespace helen {
 
 // The reverse chain, built like delta_forward_kernel: wave w owns token tile w of dO, dU and Z and its quarter of dS's rows.  Bound
-// as that one is, and it writes dS and Z: 32 sequences of 1000 tokens, 8 heads of 128, bf16: 231 us, 0.4 GB of them.
+// as that one is, and it writes dS and Z: 32 sequences of 1000 tokens, 8 heads of 128, bf16: 231 us, 0.46 GB of them.
 template <typename In, int DK>
 __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_kernel(const DeltaArgs a) {
     constexpr int NC = kColumnTiles, NI = In::kTerms, KS = DK / 32, MW = DK / 64;
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(256, In::kTerms == 1 ? 2 : 1) void delta_backward_k
 
 // The reverse chain for few long ones, as delta_forward_long_kernel: waves 0 .. 3 do what the next chunk waits for, waves 4 .. 7
 // what comes from dO alone, one chunk ahead (P^T dO and Q^T (scale e^b dO), handed over as fp32 tiles), and the stores.  8191
-// tokens in two sequences, 16 heads of 128, bf16: 182 us, 2.3 us a chunk of the longer one.
+// tokens in two sequences, 16 heads of 128, bf16: 182 us, 2.3 us a chunk of the longer one.  fp32 at width 128 spills 7 registers.
 template <typename In, int DK>
 __global__ __launch_bounds__(512) void delta_backward_long_kernel(const DeltaArgs a) {
     constexpr int NI = In::kTerms, KS = DK / 32, MW = DK / 64;
@@ -495,9 +495,10 @@ __device__ __forceinline__ float sum_from(float x, int lane) {        // over th
 // dv is walked 32 columns a step: Z, E and dO of the step as fragments in LDS (two buffers, one barrier a step), the rows of
 // S0 and dS1 straight into the registers of the one wave that needs them.  What it waits for is memory, so loads run two
 // steps ahead, over the ends of the heads too, and every wave stages as much as the others.
-// What bounds it: one workgroup a CU (128 KB of LDS, 256 registers) has nothing to hide its start (a sixth of its time) and its
-// 64 x 64 part (a third) behind; products and LDS reads of the steps are 40 % of it.  32 x 1000 tokens, 4 key and 8 value heads
-// of 128, bf16: 375 us for 0.85 GB of states, Z and E, 2.3 TB/s (500 us with loads one step ahead).
+// What bounds it: one workgroup a CU (128 KB of LDS, 256 registers; with shared key heads 9 of them spilled at width 128, 7 for fp16
+// and 12 for fp32) has nothing to hide its start and its 64 x 64 part behind: its waves wait for half of the time, the matrix pipe is
+// busy for 20 % of it.  32 x 1000 tokens, 4 key and 8 value heads of 128, bf16: 375 us for 0.54 GB read and 0.11 written, 1.7 TB/s
+// (500 us with loads one step ahead).
 // ------------------------------------------------------------------------------------------------
 template <typename In, int DK, bool SHARED>
 __global__ __launch_bounds__(DK * 4) void delta_grads_kernel(const DeltaArgs a) {

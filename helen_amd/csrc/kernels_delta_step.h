@@ -6,7 +6,8 @@
 // Bound by bandwidth: 252 streams, 32 heads of 128 x 128: 1.06 GB in 211 us, 5.0 TB/s.  One stream is a launch and its host side:
 // 10.2 us a call, where a fill of one line costs 3.8.
 // A workgroup takes 64 columns of one row's head; rows of the call that name the same slot are successive tokens of one stream and
-// are taken in order by the workgroup of the first of them.
+// are taken in order by the workgroup of the first of them.  To find them each workgroup reads all of `slots`: nothing beside its
+// state up to some thousand rows, but at 4,000 rows of 64 x 64 states as many bytes (from the caches), and growing with their square.
 #pragma once
 #include "kernels_delta.h"
 

@@ -1156,3 +1156,24 @@ def test_delta_rule_sequences_of_one_length_without_offsets(sequences, length, h
     _lib.check(lib.helen_delta_rule_backward(call, kept.data_ptr(), kept.numel(), own.data_ptr(), own.numel(), stream))
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_delta_rule_under_a_checkpoint_keeps_nothing_and_has_the_same_gradients():
+    from torch.utils.checkpoint import checkpoint
+    x = gpu(make([640], 2, 4, 128, 128, torch.bfloat16, True, seed=37))
+    names = ("q", "k", "v", "g", "beta")
+    grads, held = [], []
+    for again in (False, True):
+        leaves = [x[n].clone().requires_grad_() for n in names] + [x["initial"].clone().requires_grad_()]
+        before = torch.cuda.memory_allocated()
+        if again:
+            o, s = checkpoint(lambda *a: ops.DeltaRule.apply(*a[:5], None, a[5]), *leaves, use_reentrant=False)
+        else:
+            o, s = ops.DeltaRule.apply(*leaves[:5], None, leaves[5])
+        held.append(torch.cuda.memory_allocated() - before)
+        torch.autograd.backward([o, s], [x["do"], x["ds"]])
+        grads.append([t.grad for t in leaves])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    kept = ops._rule_bytes(_lib.HELEN_TYPE_BF16, 2, 4, 128, 128, 640, 1)[1]
+    assert held[0] - held[1] >= kept
