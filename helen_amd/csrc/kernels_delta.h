@@ -369,8 +369,8 @@ constexpr int kTriStride = 68;    // floats per row of a 64 x 64 matrix in LDS: 
 // What becomes a left-hand operand is computed transposed, (Q K^T)^T = K Q^T: a result tile then already lies as that operand
 // (lane = row, four neighbouring columns), so P goes from the accumulators to memory, and A to LDS and back in whole
 // fragments.  K^T comes from the matrix pipe too: K times a selection of 16 columns is K's tile with lane = dk.
-// What bounds it: bandwidth, mostly its own writing.  16,384 tokens, 16 key and 32 value heads of 128, bf16: 0.10 GB read and 0.50
-// written in 117 us, 5.1 TB/s, what a large copy reaches; the four workgroups a CU (35 KB of LDS, 128 registers) took it there
+// What bounds it: bandwidth, mostly its own writing.  16,384 tokens, 16 key and 32 value heads of 128, bf16: 0.10 GB read and 0.52
+// written in 117 us, 5.3 TB/s, what a large copy reaches; the four workgroups a CU (35 KB of LDS, 128 registers) took it there
 // (from 140 us to 109, then with P in two terms).
 // ------------------------------------------------------------------------------------------------
 template <typename In, int DK, bool BWD>

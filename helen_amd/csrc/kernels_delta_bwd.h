@@ -497,7 +497,7 @@ __device__ __forceinline__ float sum_from(float x, int lane) {        // over th
 // steps ahead, over the ends of the heads too, and every wave stages as much as the others.
 // What bounds it: one workgroup a CU (128 KB of LDS, 256 registers; with shared key heads 9 of them spilled at width 128, 7 for fp16
 // and 12 for fp32) has nothing to hide its start and its 64 x 64 part behind: its waves wait for half of the time, the matrix pipe is
-// busy for 20 % of it.  32 x 1000 tokens, 4 key and 8 value heads of 128, bf16: 375 us for 0.54 GB read and 0.11 written, 1.7 TB/s
+// busy for 20 % of it.  32 x 1000 tokens, 4 key and 8 value heads of 128, bf16: 377 us for 0.56 GB read and 0.12 written, 1.8 TB/s
 // (500 us with loads one step ahead).
 // ------------------------------------------------------------------------------------------------
 template <typename In, int DK, bool SHARED>

@@ -252,8 +252,8 @@ def delta_rule(q, k, v, g, beta, scale=None, initial_state=None, offsets=None, o
                      they are there, and zero in a fresh o
       keep           True: also return what delta_rule_backward needs of this call: per 64 tokens and at widths of 128
                      169 KB a value head (states, errors and triangles in float32 or three bf16 terms) and 84 KB a key head in
-                     bf16 (148 in fp16, 212 in float32); 32 sequences of 1000 tokens with 4 / 8 heads in bf16 keep 921 MB where q, k and v are 131.  The
-                     backward call takes 96 KB a value head more while it runs
+                     bf16 (148 in fp16, 212 in float32); 32 sequences of 1000 tokens with 4 / 8 heads in bf16 keep 921 MB where
+                     q, k and v are 131.  The backward call takes 96 KB a value head more while it runs
     -> (o, final_state) or (o, final_state, saved).  All arithmetic is float32-class whatever the type of q, k, v: o is the float32
     result rounded once, states are float32.
 
