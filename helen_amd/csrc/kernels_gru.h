@@ -39,9 +39,10 @@ __device__ __forceinline__ float gru_cell(float ar, float az, float an, float gr
     return ng + zg * (hp - ng);  // (1-z)*n + z*h
 }
 
-// Gate math of four cells at once, as two packed pairs: measured alone on a gfx950 SIMD a v_pk_{add,mul,fma}_f32
-// costs 5.2 cycles against 4.8 for ONE scalar add / mul / fma (v_exp_f32 / v_rcp_f32: 8.6 each, no packed form),
-// and none of it overlaps with the fp32 MFMAs (scripts/ubench/f32_mfma_valu_overlap.hip).  Per component this is
+// Gate math of four cells at once, as two pairs.  (Written for packed instructions: alone on a gfx950 SIMD a v_pk_{add,mul,fma}_f32
+// costs 5.2 cycles against 4.8 for ONE scalar add / mul / fma, v_exp_f32 / v_rcp_f32 8.6 each without a packed form.  The build
+// leaves the packed forms out, see the Makefile: the same bits, fp32 calls 1 % slower, bf16 ones 2 %, fp32x3 ones not.)  None of
+// it overlaps with the fp32 MFMAs (scripts/ubench/f32_mfma_valu_overlap.hip).  Per component this is
 // exactly:  r = sigmoid(ar + gr), z = sigmoid(az + gz), n = tanh(fma(r, an, gn)), h' = fma(z, h - n, n)
 // with sigmoid(x) = rcp(1 + exp2(-log2e x)), tanh(x) = fma(-2, rcp(1 + exp2(2 log2e x)), 1).
 typedef float f32x2 __attribute__((ext_vector_type(2)));

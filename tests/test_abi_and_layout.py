@@ -159,3 +159,14 @@ def test_dispatch_table_dry_run(monkeypatch):
     src = open(os.path.join(ROOT, "helen_amd", "csrc", "api.hip")).read()
     assert src.count("getenv(") == 1 and "use_pair_recurrence" not in src and "use_split" not in src
 
+
+
+def test_all_device_code_is_compiled_without_packed_fp32():
+    """Every compilation of a .hip file that the Makefile would run carries the flag that leaves v_pk_{add,mul,fma}_f32 out."""
+    import subprocess
+    out = subprocess.run(["make", "-n", "-B", "-C", os.path.join(ROOT, "helen_amd", "csrc"), "libhelen_hip.so"], check=True,
+                         capture_output=True, text=True, env={k: v for k, v in os.environ.items() if k != "HIPFLAGS"}).stdout
+    compiled = [ln for ln in out.splitlines() if re.search(r"\.hip\b", ln)]
+    assert len(compiled) == len([f for f in os.listdir(os.path.join(ROOT, "helen_amd", "csrc")) if f.endswith(".hip")]), out
+    for ln in compiled:
+        assert "-Xclang -target-feature -Xclang -packed-fp32-ops" in ln, ln
