@@ -281,7 +281,7 @@ enum { HELEN_TYPE_FP32 = 0, HELEN_TYPE_BF16 = 1, HELEN_TYPE_FP16 = 2 };
  *                  multiple of sequences and all have the same length.  Offsets that break this give wrong values, never an
  *                  access out of range.
  *   g              a decay: at most 0, -inf included.  Positive values work as long as e to their sum over 64 tokens is finite.
- *                  A NaN or an infinity in a token's inputs reaches its whole chunk of 64 tokens (counted from the sequence's
+ *                  A NaN or an infinity in an initial state is not forgotten; one in a token's inputs reaches its whole chunk of 64 tokens (counted from the sequence's
  *                  start), earlier ones included, and what follows, in its own sequence and heads alone.
  *   q, k           [tokens, heads_k, width_k];  v, o, d_o  [tokens, heads_v, width_v];  g, beta  [tokens, heads_v];
  *                  stride[0] between tokens, stride[1] between heads.  q, k, v, d_o: 16-byte aligned, strides too.
@@ -294,7 +294,7 @@ enum { HELEN_TYPE_FP32 = 0, HELEN_TYPE_BF16 = 1, HELEN_TYPE_FP16 = 2 };
  * grad_initial_state or NULL.
  *
  *   helen_delta_rule_bytes      workspace of a forward call (keep = 0), of one that keeps what the backward pass reads
- *                               (keep = 1), and of the backward call itself
+ *                               (keep = 1), and of the backward call itself; each 256-byte aligned
  *   helen_delta_rule_forward    keep = 1: `workspace` holds, afterwards, what helen_delta_rule_backward takes as `kept`
  *   helen_delta_rule_backward   the same description, inputs included, as the forward call that filled `kept`
  */
@@ -331,7 +331,8 @@ int helen_delta_rule_backward(const HelenDeltaRule* op, const void* kept, size_t
  *   state    float32 [pool, heads_v, width_k, width_v]; state_stride (a multiple of 4) between entries of the pool
  *   slots    int32 [rows]: the entry of each row, or NULL (row i is entry i, rows <= pool).  -1: a padded row, its output is
  *            zero.  Rows that name the same entry are successive tokens of one stream, taken in the order of the rows.  Any
- *            other number outside the pool: that row's output is NaN and no state changes.
+ *            other number outside the pool: that row's output is NaN and no state changes.  Some thousand rows at most: finding
+ *            equal ones takes time with the square of the rows.
  *   q, k [rows, heads_k, width_k], v, o [rows, heads_v, width_v], g, beta [rows, heads_v]; v is aligned to four elements
  */
 typedef struct HelenDeltaStep {
@@ -360,7 +361,7 @@ int helen_delta_rule_step(const HelenDeltaStep* op, void* stream);
  *   mean, rstd     float32 [rows]: written by the forward call (or NULL), read by the backward call
  *   rows           less than 2^36, and less than 2^24 where a row is longer than 16 KiB; width at most 2^28
  * Backward: dx, and dweight / dbias of weight_dtype, either NULL if not wanted: sums over all rows in a fixed order
- * (workspace of helen_layer_norm_bytes).
+ * (workspace of helen_layer_norm_bytes, 16-byte aligned).
  */
 typedef struct HelenLayerNorm {
     size_t struct_size;          /* sizeof(HelenLayerNorm) */

@@ -1177,3 +1177,178 @@ def test_delta_rule_under_a_checkpoint_keeps_nothing_and_has_the_same_gradients(
     assert all(torch.equal(a, b) for a, b in zip(*grads))
     kept = ops._rule_bytes(_lib.HELEN_TYPE_BF16, 2, 4, 128, 128, 640, 1)[1]
     assert held[0] - held[1] >= kept
+
+
+# ------------------------------------------------------------------------------------------------ calls that the documents allow
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("heads, lengths", [(2, [70, 130]), (16, [70, 64, 1, 131, 33])], ids=["few chains", "many chains"])
+def test_delta_rule_into_rows_that_begin_anywhere(dtype, heads, lengths):
+    """`out` needs a contiguous last dimension and no alignment; what lies around it stays."""
+    x = gpu(make(lengths, heads, heads, 64, 64, TYPES[dtype], True, seed=41))
+    n = sum(lengths)
+    kw = dict(initial_state=x["initial"], offsets=torch.tensor(ends(lengths), dtype=torch.int32, device="cuda"))
+    args = (x["q"], x["k"], x["v"], x["g"], x["beta"])
+    want = ops.delta_rule(*args, **kw)
+    step = ops.delta_rule_step(*(t[:7] for t in args), torch.zeros(7, heads, 64, 64, device="cuda"))
+    for lead in (1, 3):
+        around = torch.full((n, heads, 64 + 2 * lead + 1), 5.0, device="cuda", dtype=TYPES[dtype])
+        o, s = ops.delta_rule(*args, out=around[:, :, lead:lead + 64], **kw)
+        assert torch.equal(o, want[0]) and torch.equal(s, want[1])
+        assert bool((around[:, :, :lead] == 5).all()) and bool((around[:, :, lead + 64:] == 5).all())
+        o = ops.delta_rule_step(*(t[:7] for t in args), torch.zeros(7, heads, 64, 64, device="cuda"), out=around[:7, :, lead:lead + 64])
+        assert torch.equal(o, step) and bool((around[:, :, :lead] == 5).all()) and bool((around[:, :, lead + 64:] == 5).all())
+
+
+@pytest.mark.gpu
+def test_delta_rule_captured_once_and_replayed_with_other_lengths():
+    """Offsets on the GPU are read when the kernels run: a graph takes whatever lengths are in them at a replay."""
+    x = gpu(make([200], 2, 4, 64, 64, torch.bfloat16, False, seed=43))
+    first = torch.randn(3, 4, 64, 64, generator=torch.Generator().manual_seed(1)).cuda()
+    off = torch.tensor([0, 70, 130, 200], dtype=torch.int32, device="cuda")
+    args, kw = (x["q"], x["k"], x["v"], x["g"], x["beta"]), dict(initial_state=first, offsets=off)
+
+    def work():
+        o, s, saved = ops.delta_rule(*args, keep=True, **kw)
+        return (o, s) + ops.delta_rule_backward(x["do"], *args, saved=saved, **kw)
+    work()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    for at in ([0, 70, 130, 200], [0, 0, 1, 64], [0, 128, 128, 199], [0, 0, 0, 0], [0, 0, 0, 200], [0, 70, 130, 200]):
+        off.copy_(torch.tensor(at, dtype=torch.int32))
+        want = work()
+        for t in got:
+            t.fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), at
+        assert not got[0][at[-1]:].any() and not got[2][at[-1]:].any()
+
+
+@pytest.mark.gpu
+def test_delta_rule_of_tokens_in_no_sequence():
+    x = gpu(make([10], 1, 2, 64, 64, torch.float32, False, seed=47))
+    args = (x["q"], x["k"], x["v"], x["g"], x["beta"])
+    first = torch.randn(2, 2, 64, 64, generator=torch.Generator().manual_seed(1)).cuda()
+    for off in ([0, 0, 0], torch.zeros(3, dtype=torch.int64, device="cuda")):
+        o, s, saved = ops.delta_rule(*args, initial_state=first, offsets=off, keep=True)
+        assert not o.any() and torch.equal(s, first)
+        got = ops.delta_rule_backward(x["do"], *args, initial_state=first, offsets=off, d_final_state=first, saved=saved)
+        assert not any(t.any() for t in got[:5]) and torch.equal(got[5], first)
+
+
+@pytest.mark.gpu
+def test_delta_rule_with_a_state_that_grows():
+    """Positive g, as long as e to their sum over 64 tokens is a float32: of 64 tokens two thirds have up to 0.3."""
+    lengths = [64, 40]
+    x = make(lengths, 1, 2, 64, 64, torch.float32, True, seed=53)
+    x["g"] = x["g"].abs().clamp(max=0.3)
+    x["g"][::3] *= -1.0
+    check_delta(x, lengths)
+
+
+@pytest.mark.gpu
+def test_delta_rule_backward_keeps_a_nan_in_its_sequence_and_head():
+    lengths = [70, 80]
+    d = gpu(make(lengths, 2, 2, 64, 64, torch.bfloat16, False, seed=59))
+    off = torch.tensor(ends(lengths), dtype=torch.int32, device="cuda")
+    names = ("q", "k", "v", "g", "beta")
+    want = ops.delta_rule_backward(d["do"], *(d[n] for n in names), offsets=off)
+    for where in ("v", "do"):
+        spoiled = dict(d)
+        spoiled[where] = d[where].clone()
+        spoiled[where][66, 1, 3] = math.nan
+        got = ops.delta_rule_backward(spoiled["do"], *(spoiled[n] for n in names), offsets=off)
+        for a, b in zip(got[:5], want):
+            assert torch.equal(a[:, 0], b[:, 0]) and torch.equal(a[70:], b[70:])
+        assert torch.equal(got[5][1], want[5][1]) and torch.equal(got[5][0, 0], want[5][0, 0])
+        assert bool(got[1][:70, 1].isnan().any())
+
+
+@pytest.mark.gpu
+def test_delta_step_over_an_empty_pool_and_padded_rows_alone():
+    x = gpu(make([5], 1, 2, 64, 64, torch.bfloat16, False, seed=61))
+    args = (x["q"], x["k"], x["v"], x["g"], x["beta"])
+    slots = torch.full((5,), -1, dtype=torch.int32, device="cuda")
+    assert not ops.delta_rule_step(*args, torch.zeros(0, 2, 64, 64, device="cuda"), slots=slots).any()
+    state = torch.randn(3, 2, 64, 64, generator=torch.Generator().manual_seed(1)).cuda()
+    kept = state.clone()
+    assert not ops.delta_rule_step(*args, state, slots=slots).any() and torch.equal(state, kept)
+    slots[2] = 0
+    o = ops.delta_rule_step(*args, torch.zeros(0, 2, 64, 64, device="cuda"), slots=slots)
+    assert bool(o[2].isnan().all()) and not o[[0, 1, 3, 4]].any()
+
+
+@pytest.mark.gpu
+def test_layer_norm_autograd_with_a_bias_alone_and_a_broadcast_gradient():
+    gen = torch.Generator().manual_seed(3)
+    x = torch.randn(6, 5, 40, generator=gen).bfloat16().cuda()
+    for kind in (torch.bfloat16, torch.float32):
+        leaf, b = x.clone().requires_grad_(), torch.randn(40, generator=gen).to(kind).cuda().requires_grad_()
+        ops.LayerNorm.apply(leaf, None, b).sum().backward()
+        assert b.grad.dtype == kind and bool((b.grad == 30).all())
+        # a sum over the row of what has no mean: zero up to the rounding of dy and of the two means
+        assert leaf.grad.shape == x.shape and float(leaf.grad.float().abs().max()) <= 8 * 40 * U * float(1 / x.float().std(-1, correction=0).min())
+    w = torch.ones(40, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    dy = torch.ones(40, device="cuda", dtype=torch.bfloat16).expand(6, 5, 40)
+    y = ops.LayerNorm.apply(x, w)
+    y.backward(dy)
+    _, mean, rstd = ops.layer_norm(x)
+    assert torch.equal(w.grad, ops.layer_norm_backward(dy.contiguous(), x, w.detach(), mean, rstd)[1])
+
+
+@pytest.mark.gpu
+def test_c_entries_without_what_may_be_null():
+    """No initial, final or d_final state, no gradient of the initial one, no statistics and no gradient of the weight or the bias."""
+    x = gpu(make([130], 1, 2, 64, 64, torch.float32, False, seed=67))
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    args = (x["q"], x["k"], x["v"], x["g"], x["beta"])
+    o, s, saved = ops.delta_rule(*args, scale=0.5, keep=True)
+    want = ops.delta_rule_backward(x["do"], *args, scale=0.5, saved=saved)
+    c = _lib.HelenDeltaRuleC()
+    c.struct_size, c.device, c.dtype = ctypes.sizeof(c), x["q"].get_device(), _lib.HELEN_TYPE_FP32
+    c.heads_k, c.heads_v, c.width_k, c.width_v, c.tokens, c.sequences, c.scale = 1, 2, 64, 64, 130, 1, 0.5
+    pair = lambda t: (ctypes.c_int64 * 2)(*t.stride()[:2])  # noqa: E731
+    for name, t in zip(("q", "k", "v", "g", "beta", "d_o"), args + (x["do"],)):
+        setattr(c, name, t.data_ptr())
+        setattr(c, name + "_stride", pair(t))
+    sizes = [ctypes.c_size_t() for _ in range(3)]
+    _lib.check(lib.helen_delta_rule_bytes(ctypes.byref(c), *(ctypes.byref(t) for t in sizes)))
+    kept, own = (torch.empty(t.value, dtype=torch.uint8, device="cuda") for t in sizes[1:])
+    out, state = torch.full_like(o, 7.0), torch.full_like(s, 7.0)
+    got = [torch.full_like(t, 7.0) for t in want[:5]]
+    for name, t in zip(("grad_q", "grad_k", "grad_v", "grad_g", "grad_beta"), got):
+        setattr(c, name, t.data_ptr())
+    c.final_state = state.data_ptr()                      # the states alone
+    _lib.check(lib.helen_delta_rule_forward(ctypes.byref(c), 1, kept.data_ptr(), kept.numel(), stream))
+    assert torch.equal(state, s)
+    c.o, c.o_stride, c.final_state = out.data_ptr(), pair(out), None      # the outputs alone
+    _lib.check(lib.helen_delta_rule_forward(ctypes.byref(c), 1, kept.data_ptr(), kept.numel(), stream))
+    _lib.check(lib.helen_delta_rule_backward(ctypes.byref(c), kept.data_ptr(), kept.numel(), own.data_ptr(), own.numel(), stream))
+    assert torch.equal(out, o) and all(torch.equal(a, b) for a, b in zip(got, want))
+    rows, width = 300, 100
+    gen = torch.Generator().manual_seed(5)
+    y, dy, w = (torch.randn(*shape, generator=gen).cuda() for shape in ((rows, width), (rows, width), (width,)))
+    norm, mean, rstd = ops.layer_norm(y, w, w)
+    dx, dw, db = ops.layer_norm_backward(dy, y, w, mean, rstd)
+    n = _lib.HelenLayerNormC()
+    n.struct_size, n.device, n.width, n.rows, n.eps = ctypes.sizeof(n), y.get_device(), width, rows, 1e-5
+    n.x, n.x_stride, n.weight, n.bias = y.data_ptr(), width, w.data_ptr(), w.data_ptr()
+    out, grad, sums = torch.empty_like(y), torch.empty_like(y), torch.full((2, width), 7.0, device="cuda")
+    n.y, n.y_stride = out.data_ptr(), width
+    _lib.check(lib.helen_layer_norm_forward(ctypes.byref(n), stream))
+    assert torch.equal(out, norm)
+    n.mean, n.rstd, n.dy, n.dy_stride, n.dx, n.dx_stride = mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), width, grad.data_ptr(), width
+    need = ctypes.c_size_t()
+    _lib.check(lib.helen_layer_norm_bytes(ctypes.byref(n), ctypes.byref(need)))
+    work = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    for a, b in ((None, None), (sums[0], None), (None, sums[1])):
+        grad.fill_(7.0)
+        sums.fill_(7.0)
+        n.dweight, n.dbias = (None if t is None else t.data_ptr() for t in (a, b))
+        _lib.check(lib.helen_layer_norm_backward(ctypes.byref(n), work.data_ptr(), work.numel(), stream))
+        assert torch.equal(grad, dx)
+        assert torch.equal(sums[0], torch.full_like(dw, 7.0) if a is None else dw)
+        assert torch.equal(sums[1], torch.full_like(db, 7.0) if b is None else db)
